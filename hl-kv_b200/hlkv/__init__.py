@@ -10,6 +10,8 @@ Module layout mirrors the reference's host API:
   * :class:`Table` -- hl::alloc::HeteroBlockTable (statuses as ``Status`` ints);
   * :class:`DeviceTables` -- the persistent device descriptor table + id arena;
   * :func:`gather_dequant`, :func:`append_encode`, :func:`apply_delta` -- kernels (1)-(3);
+  * :class:`BatchPlan`, :func:`batch_plan`, :func:`rotary_append`, :func:`batch_attention` -- a
+    layer's step of a ragged batch: block table and slot map, rotary + append, attention;
   * :func:`dequantize_fp8_to_fp16`, :func:`dequantize_to_fp16`, :func:`quantize` -- flat codecs.
 """
 from __future__ import annotations
@@ -39,6 +41,7 @@ ERR_NONFINITE = 1 << 9
 ERR_TOKEN_RANGE = 1 << 10
 ERR_PATCH_RANGE = 1 << 11
 ERR_OUT_ALIGN = 1 << 12
+ERR_PLAN_RANGE = 1 << 13
 
 
 class Status:
@@ -93,6 +96,20 @@ class Layout(C.Structure):
                 ("layout_id", C.c_uint32)]
 
 
+class PlanArrays(C.Structure):
+    """HlkvBatchPlan."""
+    _fields_ = [("nseq", C.c_uint32), ("max_query", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32),
+                ("block_cap", C.c_uint32), ("token_cap", C.c_uint32), ("block_first", C.c_void_p),
+                ("block_count", C.c_void_p), ("token_first", C.c_void_p), ("context", C.c_void_p),
+                ("blocks", C.c_void_p), ("targets", C.c_void_p), ("positions", C.c_void_p)]
+
+
+class Rotary(C.Structure):
+    """HlkvRotary."""
+    _fields_ = [("rotary_dim", C.c_uint32), ("interleaved", C.c_uint32), ("axes", C.c_uint32), ("factor", C.c_float),
+                ("inv_freq", C.c_float * 128), ("pair_axis", C.c_uint8 * 128)]
+
+
 class PoolConfig(C.Structure):
     _fields_ = [("format", C.c_uint32), ("slot_bytes", C.c_uint32), ("num_slots", C.c_uint32)]
 
@@ -122,7 +139,7 @@ class Handle(C.Structure):
 
 INVALID_HANDLE = Handle(0xFFFFFFFF, 0)
 
-_vp, _u32, _u64, _sz, _int = C.c_void_p, C.c_uint32, C.c_uint64, C.c_size_t, C.c_int
+_vp, _u32, _u64, _i64, _sz, _int = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int64, C.c_size_t, C.c_int
 _P = C.POINTER
 
 # (name, restype, argtypes) for every entry point of include/hlkv.h.
@@ -146,6 +163,12 @@ SIGNATURES: list[tuple[str, object, list]] = [
     ("hlkv_transcode", _int, [_P(Pools), _P(Layout), _vp, _u32, _vp, _vp]),
     ("hlkv_append_encode", _int, [_P(Pools), _P(Layout), _vp, _u32, _vp, _u32, _vp, _vp, _vp]),
     ("hlkv_apply_delta", _int, [_vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _vp]),
+    ("hlkv_batch_plan", _int, [_P(PlanArrays), _P(Layout), _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp]),
+    ("hlkv_rotary_append", _int, [_P(Pools), _P(Layout), _vp, _u32, _vp, _u32, _P(Rotary), _vp, _i64, _i64, _vp, _u32,
+                                  _u64, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp]),
+    ("hlkv_batch_attention_workspace_bytes", _sz, [_P(PlanArrays), _P(Layout), _u32]),
+    ("hlkv_batch_attention", _int, [_P(Pools), _P(Layout), _P(PlanArrays), _vp, _u32, _u64, C.c_float, _vp, _sz, _vp,
+                                    _u64, _vp, _vp]),
     ("hlkv_dequantize_fp8_to_fp16", _int, [_int, _vp, _sz, _vp, _sz, _vp, _vp]),
     ("hlkv_dequantize_to_fp16", _int, [_int, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _vp]),
     ("hlkv_quantize", _int, [_int, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp]),
@@ -655,6 +678,157 @@ def decode_attention_split_noalloc(pools: Pools, layout: Layout, table_ptr: int,
                                                    nseq, _ptr(q), q_heads, softmax_scale, splits, _ptr(out),
                                                    _ptr(err), _stream_handle(stream))
     check(st, "hlkv_decode_attention_split_noalloc")
+    return st
+
+
+# ---- a layer's step of a ragged batch ---------------------------------------------------------------
+def _need(cond: bool, what: str) -> None:
+    if not cond:
+        raise HlkvError(what)
+
+
+def _on_device_of(t, fn, *args, **kwargs):
+    """Runs fn with t's device current (the C entry points launch on the current device)."""
+    import torch
+    with torch.cuda.device(t.device):
+        return fn(*args, **kwargs)
+
+
+def _current_device() -> int:
+    import torch
+    return torch.cuda.current_device()
+
+
+class BatchPlan:
+    """The device arrays of one HlkvBatchPlan (all int32 tensors, views of one allocation):
+    block_first, block_count, context [nseq], token_first [nseq + 1], blocks [block_cap, 4]
+    (slot, info, scale_ref, start), targets [token_cap, 2], positions [token_cap].
+
+    max_query: the most new tokens of a sequence; window: 0, or the tokens that a new token sees;
+    sinks: first tokens that stay visible behind the window."""
+
+    def __init__(self, nseq: int, block_cap: int, token_cap: int, max_query: int = 1, window: int = 0, sinks: int = 0,
+                 device="cuda"):
+        import torch
+        _need(min(nseq, block_cap, token_cap, window, sinks) >= 0 and max_query >= 1, "BatchPlan: negative size")
+        parts, total = [], 0
+        for n in (4 * block_cap, 2 * token_cap, token_cap, nseq, nseq, nseq + 1, nseq):
+            parts.append((total, n))
+            total += (n + 3) // 4 * 4
+        buf = torch.zeros(max(total, 4), dtype=torch.int32, device=device)
+        v = [buf[o:o + n] for o, n in parts]
+        self.blocks, self.targets, self.positions = v[0].view(-1, 4), v[1].view(-1, 2), v[2]
+        self.block_first, self.block_count, self.token_first, self.context = v[3:]
+        at = [buf.data_ptr() + 4 * o for o, _ in parts]
+        self.c = PlanArrays(nseq, max_query, window, sinks, block_cap, token_cap, at[3], at[4], at[5], at[6], at[0],
+                            at[1], at[2])
+        self.device = buf.device
+
+
+def batch_plan(plan: BatchPlan, layout: Layout, table_ptr: int, table_size: int, arena_ptr: int, arena_size: int,
+               segs, query_lens, err, stream=None) -> int:
+    """Fills the plan from the device tables.  segs: device int32 [nseq, 2]; query_lens: device int32
+    [nseq], or None for one new token each.  Raises on a non-OK status."""
+    if plan.device.index != _current_device():
+        return _on_device_of(plan.blocks, batch_plan, plan, layout, table_ptr, table_size, arena_ptr, arena_size, segs,
+                             query_lens, err, stream)
+    n = plan.c.nseq
+    _need(tuple(segs.shape) == (n, 2) and segs.is_contiguous() and segs.element_size() == 4 and segs.device == plan.device,
+          "batch_plan: segs is a contiguous int32 [nseq, 2] on the plan's device")
+    _need(query_lens is None or (query_lens.numel() == n and query_lens.is_contiguous() and query_lens.element_size() == 4
+                                 and query_lens.device == plan.device),
+          "batch_plan: query_lens is a contiguous int32 [nseq] on the plan's device")
+    st = lib().hlkv_batch_plan(C.byref(plan.c), C.byref(layout), table_ptr or None, table_size, arena_ptr or None,
+                               arena_size, segs.data_ptr(), _ptr(query_lens), _ptr(err), _stream_handle(stream))
+    check(st, "hlkv_batch_plan")
+    return st
+
+
+def make_rotary(inv_freq, axes: int | None = None, pair_axis=None, interleaved: bool = False,
+                factor: float = 1.0) -> Rotary:
+    """inv_freq: one frequency per pair (rotary_dim / 2 of them); pair_axis: each pair's axis (default 0)."""
+    n = len(inv_freq)
+    _need(8 <= n <= 128, "make_rotary: 8 to 128 pairs")
+    r = Rotary(2 * n, int(interleaved), 0, factor)
+    r.inv_freq[:n] = [float(f) for f in inv_freq]
+    if pair_axis is not None:
+        _need(len(pair_axis) == n, "make_rotary: an axis for every pair")
+        r.pair_axis[:n] = [int(a) for a in pair_axis]
+    r.axes = max(r.pair_axis[:n]) + 1 if axes is None else axes
+    return r
+
+
+def _heads(t, what: str, layout: Layout, n: int | None = None, heads: int | None = None) -> None:
+    _need(t.dim() == 3 and t.shape[2] == layout.head_dim and t.element_size() == 2
+          and (t.shape[1] <= 1 or t.stride(1) == layout.head_dim) and t.stride(2) == 1
+          and (n is None or t.shape[0] == n) and (heads is None or t.shape[1] == heads),
+          f"{what} is a 16-bit [tokens, heads, head_dim] with contiguous heads")
+
+
+def _token_stride(t) -> int:
+    """A tensor of at most one token may have any stride: the row's length then."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def rotary_append(pools: Pools, layout: Layout, table_ptr: int, table_size: int, targets, rotary: Rotary, positions,
+                  q, k, v, q_out, err, stream=None) -> int:
+    """Rotates q and k by their positions, writes q to q_out (which may be q) and stores k and v in
+    the targets' blocks.  targets: device int32 [n, 2]; positions: device int32 [n] or [n, axes], any
+    strides; q, q_out: device 16-bit [n, q_heads, head_dim] (or None); k, v: [n, kv_heads, head_dim];
+    token strides are free (slices of a fused projection).  Raises on a non-OK status."""
+    if k.device.index != _current_device():
+        return _on_device_of(k, rotary_append, pools, layout, table_ptr, table_size, targets, rotary, positions, q, k, v,
+                             q_out, err, stream)
+    n = int(targets.shape[0])
+    _heads(k, "rotary_append: k", layout, n, layout.kv_heads)
+    _heads(v, "rotary_append: v", layout, n, layout.kv_heads)
+    _need(targets.is_contiguous() and targets.element_size() == 4 and targets.dim() == 2 and targets.shape[1] == 2,
+          "rotary_append: targets is a contiguous int32 [n, 2]")
+    _need(positions.element_size() == 4 and positions.shape[0] == n
+          and (positions.dim() == 2 and positions.shape[1] >= rotary.axes or positions.dim() == 1 and rotary.axes == 1),
+          "rotary_append: positions is an int32 [n] or [n, axes]")
+    heads = 0
+    if q is not None:
+        heads = int(q.shape[1])
+        _heads(q, "rotary_append: q", layout, n)
+        _heads(q_out, "rotary_append: q_out", layout, n, heads)
+    for t in (targets, positions, v, q, q_out, err):
+        _need(t is None or t.device == k.device, "rotary_append: tensors on one device")
+    st = lib().hlkv_rotary_append(C.byref(pools), C.byref(layout), table_ptr or None, table_size, targets.data_ptr(), n,
+                                  C.byref(rotary), positions.data_ptr(), positions.stride(0),
+                                  positions.stride(1) if positions.dim() == 2 else 0, _ptr(q), heads,
+                                  _token_stride(q) if heads else 0, k.data_ptr(), _token_stride(k), v.data_ptr(),
+                                  _token_stride(v), _ptr(q_out), _token_stride(q_out) if heads else 0, _ptr(err),
+                                  _stream_handle(stream))
+    check(st, "hlkv_rotary_append")
+    return st
+
+
+def batch_attention_workspace_bytes(plan: BatchPlan, layout: Layout, q_heads: int) -> int:
+    """Workspace that batch_attention needs for this plan on its device."""
+    if plan.device.index != _current_device():
+        return _on_device_of(plan.blocks, batch_attention_workspace_bytes, plan, layout, q_heads)
+    return lib().hlkv_batch_attention_workspace_bytes(C.byref(plan.c), C.byref(layout), q_heads)
+
+
+def batch_attention(pools: Pools, layout: Layout, plan: BatchPlan, q, softmax_scale: float, out, err, workspace=None,
+                    stream=None) -> int:
+    """Attention of the plan's new tokens over their sequences' blocks.  q, out: device 16-bit
+    [token_cap, q_heads, head_dim] with free token strides; workspace: a device tensor of
+    batch_attention_workspace_bytes(...) bytes.  Raises on a non-OK status."""
+    if plan.device.index != _current_device():
+        return _on_device_of(plan.blocks, batch_attention, pools, layout, plan, q, softmax_scale, out, err, workspace,
+                             stream)
+    heads = int(q.shape[1])
+    _heads(q, "batch_attention: q", layout, plan.c.token_cap)
+    _heads(out, "batch_attention: out", layout, plan.c.token_cap, heads)
+    _need(q.device == plan.device and out.device == plan.device and err.device == plan.device
+          and (workspace is None or workspace.device == plan.device), "batch_attention: tensors on the plan's device")
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    st = lib().hlkv_batch_attention(C.byref(pools), C.byref(layout), C.byref(plan.c), q.data_ptr(), heads,
+                                    _token_stride(q), softmax_scale, _ptr(workspace) if ws_bytes else None, ws_bytes,
+                                    out.data_ptr(), _token_stride(out), _ptr(err), _stream_handle(stream))
+    check(st, "hlkv_batch_attention")
     return st
 
 

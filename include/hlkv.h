@@ -80,7 +80,10 @@ enum {
   HLKV_ERR_NONFINITE = 1u << 9,       /* a group with a non-finite value was skipped  */
   HLKV_ERR_TOKEN_RANGE = 1u << 10,    /* append target token >= block_tokens          */
   HLKV_ERR_PATCH_RANGE = 1u << 11,    /* delta patch target out of range              */
-  HLKV_ERR_OUT_ALIGN = 1u << 12       /* output offset not a multiple of 8 elements   */
+  HLKV_ERR_OUT_ALIGN = 1u << 12,      /* output offset not a multiple of 8 elements   */
+  HLKV_ERR_PLAN_RANGE = 1u << 13      /* a sequence that a batch plan cannot hold, or
+                                         with more new tokens than max_query or than
+                                         it has tokens                                */
 };
 
 /* ---- ABI records (byte-identical to hl::alloc, block_descriptor.hpp:137-150 and
@@ -329,6 +332,138 @@ int hlkv_decode_attention_split_noalloc(const HlkvPools* pools, const HlkvLayout
                                         const HlkvSegment* d_segs, uint32_t nseq, const uint16_t* d_q,
                                         uint32_t q_heads, float softmax_scale, uint32_t splits,
                                         uint16_t* d_out, uint32_t* d_err, hlkv_stream_t stream);
+
+/* ---- batch plan: block tables, slot map and positions of a step, built on the GPU --------- */
+/* A block that a plan's sequence reads: the descriptor's first three words, and the position
+ * (in the sequence) of the block's first token. */
+typedef struct {
+  uint32_t slot;
+  uint32_t info; /* as HlkvExecDescriptor.info */
+  uint32_t scale_ref;
+  uint32_t start;
+} HlkvPlanBlock;
+
+/*
+ * A ragged batch of sequences, each with some new tokens at its end (a prompt, a chunk of one,
+ * one decoded token, a few proposed ones): the arrays that hlkv_batch_plan fills and that every
+ * layer's hlkv_rotary_append (targets, positions) and hlkv_batch_attention read.  The caller
+ * owns the device arrays and sets all fields before hlkv_batch_plan.
+ *   window  0, or the tokens that a new token sees up to and including its own;
+ *   sinks   the first tokens that stay visible behind the window.
+ */
+typedef struct {
+  uint32_t nseq;
+  uint32_t max_query; /* no sequence has more new tokens (>= 1) */
+  uint32_t window;
+  uint32_t sinks;
+  uint32_t block_cap; /* entries of d_blocks  */
+  uint32_t token_cap; /* entries of d_targets and d_positions */
+  uint32_t* d_block_first;     /* [nseq] first entry of the sequence in d_blocks: the packed
+                                  prefix sum of the segment lengths, at most block_cap */
+  uint32_t* d_block_count;     /* [nseq] blocks listed (the visible ones) */
+  uint32_t* d_token_first;     /* [nseq + 1] prefix sum of the new tokens, at most token_cap */
+  uint32_t* d_context;         /* [nseq] tokens of the sequence, the new ones included */
+  HlkvPlanBlock* d_blocks;     /* [block_cap], 16-byte aligned */
+  HlkvAppendTarget* d_targets; /* [token_cap], 8-byte aligned: where each new token goes */
+  int32_t* d_positions;        /* [token_cap]: its position in its sequence */
+} HlkvBatchPlan;
+
+/*
+ * Fills a plan from the device tables: sequence i has the blocks of d_segs[i], its context is
+ * the sum of their valid tokens, and its last d_query_lens[i] tokens are the new ones (NULL: one
+ * each).  New tokens count as valid already: grow the blocks on the host table
+ * (set_valid_tokens, append_block, or hlkv_table_append_tokens) and apply the delta first.
+ *  - A block lists when it holds a token that some new token of its sequence sees: all blocks
+ *    with tokens for window 0, else those with a token at a position < sinks or >= context -
+ *    new - window + 1.  Listed blocks keep their order; entries of d_blocks behind a sequence's
+ *    count stay as they were.
+ *  - The checks of kernel (1) that need no pool (arena, block id, descriptor, format 15 or above
+ *    3, layout tag, block-wide parameters, valid tokens) are made here: a block that fails has
+ *    no tokens and its HLKV_ERR_* bit is set.  Slots are checked by the plan's readers.
+ *  - d_targets and d_positions of new token r of sequence i are at d_token_first[i] + r.  Rows
+ *    behind the last token get the target {0xFFFFFFFF, 0xFFFFFFFF}, which hlkv_rotary_append
+ *    skips, and position 0, so that a captured step may run with a padded token array.
+ *  - A sequence whose blocks or new tokens do not fit the arrays, or that has more than
+ *    max_query new tokens, is planned as empty (context 0, no blocks, its rows padding) with
+ *    HLKV_ERR_PLAN_RANGE.  New tokens beyond a sequence's tokens are padding, with the same bit.
+ * block_cap * block_tokens is below 2^31 (positions are int32).
+ * The device form of hlkv_table_build_exec_table (hetero_block_table.cpp:406-433) and of
+ * hlkv_table_append_tokens' targets; the reference builds neither on the device.
+ */
+int hlkv_batch_plan(const HlkvBatchPlan* plan, const HlkvLayout* layout, const HlkvExecDescriptor* d_table,
+                    uint32_t table_size, const uint32_t* d_arena, uint32_t arena_size,
+                    const HlkvSegment* d_segs, const uint32_t* d_query_lens, uint32_t* d_err,
+                    hlkv_stream_t stream);
+
+/* ---- rotary append: rotate Q and K, store K and V ------------------------------------------- */
+/*
+ * A rotary embedding (host memory, read during the call).  Pair j < rotary_dim / 2 of a head is
+ * (x[j], x[j + rotary_dim / 2]), or (x[2 j], x[2 j + 1]) when interleaved; it turns by the angle
+ *   a_j = position[pair_axis[j]] * inv_freq[j]
+ * and elements from rotary_dim on stay.  Images and video give each token a position per axis
+ * (time, height, width); text has one axis.
+ */
+typedef struct {
+  uint32_t rotary_dim;     /* a multiple of 16, <= head_dim */
+  uint32_t interleaved;    /* 0 or 1 */
+  uint32_t axes;           /* 1 .. 4 */
+  float factor;            /* multiplies cos and sin (1 for plain rotary embeddings) */
+  float inv_freq[128];     /* magnitude at most 65536 */
+  uint8_t pair_axis[128];  /* < axes */
+} HlkvRotary;
+
+/*
+ * For every new token k < n: with c_j = binary32(factor cos a_j) and s_j likewise (a_j in
+ * binary64, exact for positions below 2^29), each pair (x, y) of its Q and K heads becomes
+ *   (x c - y s, y c + x s), every operation in binary32.
+ * Q is rounded to binary16 into d_q_out; K is encoded from the binary32 values, and V from its
+ * binary16 values, into token slot d_targets[k] (a plan's d_targets, or any list of distinct
+ * targets).  An FP16 block takes them rounded once; a quantized row follows quantize_reference's
+ * rules as hlkv_append_encode does, with the scale computed as amax * (1 / max_finite) or range *
+ * (1 / 15), the reciprocal in binary32: within two units in the last place of its quotient, so
+ * that a value midway between two codes may take the other one.
+ *  - d_q, d_k, d_v, d_q_out: binary16, heads of head_dim contiguous per token ([q_heads] or
+ *    [kv_heads]), token strides in elements (multiples of 8); 16-byte aligned.  Slices of a fused
+ *    projection need no copy.  d_q_out may be d_q with the same stride, and overlaps nothing else.
+ *    q_heads 0: K and V only (d_q and d_q_out unused).
+ *  - d_positions[k * position_token_stride + a * position_axis_stride], int32.
+ *  - A target {0xFFFFFFFF, 0xFFFFFFFF} is padding: the row is skipped, its d_q_out left as it was.
+ *  - A target failing hlkv_append_encode's checks stores nothing and sets its bit (Q is still
+ *    written); a quantized row with a non-finite value is skipped with HLKV_ERR_NONFINITE.
+ * No counterpart in the reference.
+ */
+int hlkv_rotary_append(const HlkvPools* pools, const HlkvLayout* layout, const HlkvExecDescriptor* d_table,
+                       uint32_t table_size, const HlkvAppendTarget* d_targets, uint32_t n,
+                       const HlkvRotary* rotary, const int32_t* d_positions, int64_t position_token_stride,
+                       int64_t position_axis_stride, const uint16_t* d_q, uint32_t q_heads,
+                       uint64_t q_stride, const uint16_t* d_k, uint64_t k_stride, const uint16_t* d_v,
+                       uint64_t v_stride, uint16_t* d_q_out, uint64_t q_out_stride, uint32_t* d_err,
+                       hlkv_stream_t stream);
+
+/* ---- batch attention: ragged queries over the quantized blocks ------------------------------- */
+/*
+ * Every new token of a plan attends to its sequence's cached tokens (its own included):
+ *   out[i][qh] = softmax_t(softmax_scale <q, k_t>) . v_t   over the t with
+ *   t <= p  and  (window == 0  or  p - t < window  or  t < sinks),   p = the token's position.
+ * K and V are the values of the codes under their parameters (code * scale, or code * scale +
+ * bias), not rounded to binary16 first; sums, maxima and the running state are binary32; the
+ * result is rounded to binary16.  A row that sees no token is zeros.  Tokens that a row does not
+ * see do not touch it, whatever they hold.
+ *  - d_q and d_out: binary16, token rows at the plan's d_token_first[i] + r, heads contiguous
+ *    ([q_heads][head_dim]), token strides in elements (multiples of 8), 16-byte aligned.  Rows
+ *    behind the last new token are left as they were.
+ *  - head_dim 64 or 128; q_heads / kv_heads 1 .. 32; softmax_scale finite and > 0.
+ *  - d_workspace: 16-byte aligned, hlkv_batch_attention_workspace_bytes(plan, layout, q_heads)
+ *    bytes, needing no initial value.  Calls that overlap on the GPU must not share one.
+ *  - A listed block whose pool or slot is missing is left out, with its HLKV_ERR_* bit.
+ * No counterpart in the reference.
+ */
+size_t hlkv_batch_attention_workspace_bytes(const HlkvBatchPlan* plan, const HlkvLayout* layout,
+                                            uint32_t q_heads);
+int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* layout, const HlkvBatchPlan* plan,
+                         const uint16_t* d_q, uint32_t q_heads, uint64_t q_stride, float softmax_scale,
+                         void* d_workspace, size_t workspace_bytes, uint16_t* d_out, uint64_t out_stride,
+                         uint32_t* d_err, hlkv_stream_t stream);
 
 /* ---- format-change transcode ------------------------------------------------------------ */
 typedef struct {
