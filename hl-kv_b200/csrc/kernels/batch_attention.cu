@@ -6,54 +6,13 @@
 //   x_t = softmax_scale log2(e) <q, k_t>,  m = max x_t,  out = sum 2^(x_t - m) v_t / sum 2^(x_t - m),
 // in one pass with a running maximum.  k_t and v_t are the values of the codes under their
 // parameters, in binary32.
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
 #include <cmath>
-#include <cstdint>
 
-#include "codec.cuh"
-#include "common.cuh"
-#include "hlkv.h"
+#include "batch_attention.cuh"
 
 namespace hlkv {
+namespace battn {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kMaxGroup = 32;
-
-struct DevPool {
-  const uint8_t* base;
-  uint64_t slot_bytes;
-  uint32_t num_slots;
-};
-
-struct Params {
-  DevPool pool[4];
-  uint64_t code_bytes[4];
-  const uint32_t *block_first, *block_count, *token_first, *context;
-  const uint4* blocks;
-  const uint16_t* q;
-  uint16_t* out;
-  uint64_t q_stride, out_stride;
-  uint32_t* err;
-  uint32_t nseq, T, H, q_heads, group, window, sinks, block_cap;
-  float qscale;  // softmax_scale * log2(e)
-};
-
-// The pool checks of a listed block; returns the format (4 = left out) and the slot's address.
-__device__ __forceinline__ uint32_t open_block(const Params& p, uint4 b, const uint8_t** payload) {
-  const uint32_t f = b.y & 0xFu;
-  uint32_t bad = 0;
-  if (f > 3 || p.pool[f].base == nullptr) bad = dev::kErrBadFormat;
-  else if (b.x >= p.pool[f].num_slots) bad = dev::kErrSlotRange;
-  if (bad) {
-    atomicOr(p.err, bad);
-    return 4;
-  }
-  *payload = p.pool[f].base + uint64_t{b.x} * p.pool[f].slot_bytes;
-  return f;
-}
 
 // kN consecutive elements of a row from element e, and the row's {scale, bias}: the codes' values
 // without the parameters.
@@ -109,6 +68,7 @@ __global__ void __launch_bounds__(kRowThreads) batch_attention_rows(const Params
     if (p.token_first[mid] <= token) lo = mid; else hi = mid;
   }
   const uint32_t q_len = p.token_first[lo + 1] - p.token_first[lo], ctx = p.context[lo];
+  if (uint64_t{q_len} * p.group <= kStreamRows) return;  // the stream kernel's
   const int64_t pos = int64_t{ctx} - q_len + (token - p.token_first[lo]);
 
   float q[kN], acc[kN];
@@ -118,7 +78,8 @@ __global__ void __launch_bounds__(kRowThreads) batch_attention_rows(const Params
     acc[i] = 0.0f;
   }
   float m = -INFINITY, l = 0.0f;
-  const uint32_t first = p.block_first[lo], count = min(p.block_count[lo], p.block_cap - first);
+  uint32_t first;
+  const uint32_t count = count_of(p, lo, &first);
   for (uint32_t j = 0; j < count; ++j) {
     const uint4 b = __ldg(p.blocks + first + j);
     const uint32_t vt = min((b.y >> 10) & 0x3FFu, p.T);
@@ -157,14 +118,19 @@ __global__ void __launch_bounds__(kRowThreads) batch_attention_rows(const Params
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
+}  // namespace battn
 }  // namespace hlkv
 
 extern "C" size_t hlkv_batch_attention_workspace_bytes(const HlkvBatchPlan* plan, const HlkvLayout* layout,
                                                        uint32_t q_heads) {
-  (void)plan;
-  (void)layout;
-  (void)q_heads;
-  return 0;
+  if (plan == nullptr || layout == nullptr || plan->nseq == 0 || plan->token_cap == 0 || layout->kv_heads == 0 ||
+      q_heads < layout->kv_heads || (layout->head_dim != 64 && layout->head_dim != 128)) {
+    return 0;
+  }
+  const uint64_t rows = uint64_t{plan->max_query} * (q_heads / layout->kv_heads);
+  return hlkv::battn::stream_workspace(plan->nseq, layout->kv_heads, layout->head_dim,
+                                       static_cast<uint32_t>(rows < 0xFFFFFFFFu ? rows : 0xFFFFFFFFu),
+                                       static_cast<uint32_t>(hlkv::sm_count()));
 }
 
 extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* layout, const HlkvBatchPlan* plan,
@@ -172,6 +138,7 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
                                     void* d_workspace, size_t workspace_bytes, uint16_t* d_out, uint64_t out_stride,
                                     uint32_t* d_err, hlkv_stream_t stream) {
   using namespace hlkv;
+  using namespace hlkv::battn;
   if (pools == nullptr || plan == nullptr || !layout_ok(layout) || d_err == nullptr) return HLKV_INVALID_ARGUMENT;
   const uint64_t D = layout->head_dim;
   if (D != 64 && D != 128) return HLKV_INVALID_ARGUMENT;
@@ -180,7 +147,8 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   if (!(softmax_scale > 0.0f) || !std::isfinite(softmax_scale)) return HLKV_INVALID_ARGUMENT;
   if (plan->nseq == 0 || plan->token_cap == 0) return HLKV_OK;
   if (plan->d_block_first == nullptr || plan->d_block_count == nullptr || plan->d_token_first == nullptr ||
-      plan->d_context == nullptr || (plan->block_cap > 0 && plan->d_blocks == nullptr) || !aligned16(plan->d_blocks) ||
+      plan->d_context == nullptr || plan->d_cost == nullptr ||
+      (plan->block_cap > 0 && (plan->d_blocks == nullptr || plan->d_block_cost == nullptr)) || !aligned16(plan->d_blocks) ||
       plan->max_query == 0 || d_q == nullptr || d_out == nullptr || !aligned16(d_q) || !aligned16(d_out) ||
       q_stride % 8 != 0 || out_stride % 8 != 0 || q_stride < q_heads * D || out_stride < q_heads * D) {
     return HLKV_INVALID_ARGUMENT;
@@ -201,6 +169,8 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
     }
     p.pool[f] = DevPool{static_cast<const uint8_t*>(q.base), q.slot_bytes, q.num_slots};
   }
+  const uint64_t rows = uint64_t{plan->token_cap} * q_heads;
+  if (rows > 0x7FFFFFFFull || uint64_t{plan->nseq} * H > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
   p.block_first = plan->d_block_first;
   p.block_count = plan->d_block_count;
   p.token_first = plan->d_token_first;
@@ -219,11 +189,18 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   p.window = plan->window;
   p.sinks = plan->sinks;
   p.block_cap = plan->block_cap;
+  p.block_cost = plan->d_block_cost;
+  p.cost = plan->d_cost;
+  p.token_cap = plan->token_cap;
+  const uint64_t max_rows = uint64_t{plan->max_query} * p.group;
+  p.max_rows = static_cast<uint32_t>(max_rows < 0xFFFFFFFFu ? max_rows : 0xFFFFFFFFu);
   p.qscale = softmax_scale * kLog2e;
-  const uint64_t rows = uint64_t{plan->token_cap} * q_heads;
-  if (rows > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
-  const unsigned grid = static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32));
+  p.ctas = static_cast<uint32_t>(sm_count());
+  stream_layout(&p, d_workspace);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = launch_stream(layout->head_dim, p, s);
+  if (e != cudaSuccess || p.max_rows <= kStreamRows) return cuda_status(e);
+  const unsigned grid = static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32));
   if (D == 64) batch_attention_rows<64><<<grid, kRowThreads, 0, s>>>(p);
   else batch_attention_rows<128><<<grid, kRowThreads, 0, s>>>(p);
   return cuda_status(cudaGetLastError());

@@ -45,17 +45,29 @@ struct Params {
   uint32_t prefix_done;  // d_block_first and d_token_first are filled already
 };
 
-// Tokens and non-empty blocks, added as one.
+// Tokens, non-empty blocks and their cost to the attention, added as one.
 struct Sum {
-  uint32_t tokens, blocks;
-  __device__ __forceinline__ Sum operator+(const Sum& o) const { return {tokens + o.tokens, blocks + o.blocks}; }
+  uint32_t tokens, blocks, cost;
+  __device__ __forceinline__ Sum operator+(const Sum& o) const {
+    return {tokens + o.tokens, blocks + o.blocks, cost + o.cost};
+  }
 };
+
+// What a block of v tokens costs the attention, which works on tiles of 16 tokens: in proportion to
+// its bytes (FP16 : FP8 : INT4 = 256 : 132 : 72 for heads of 128).
+__device__ __forceinline__ uint32_t block_cost(uint32_t info, uint32_t v) {
+  const uint32_t f = info & 0xFu;
+  return (v + 15) / 16 * (f == dev::kFp16 ? 14u : f == dev::kInt4 ? 4u : 7u);
+}
+__device__ __forceinline__ Sum block_sum(uint32_t info, uint32_t v) {
+  return v > 0 ? Sum{v, 1u, block_cost(info, v)} : Sum{0u, 0u, 0u};
+}
 
 struct Shared {
   Sum warp[kWarps];
   Sum cta[2][kMaxCluster];  // every CTA's total, written by its owner into each CTA (two rounds' worth)
   uint64_t prefix[2][kWarps];
-  uint32_t border[2];  // P and S
+  uint32_t border[4];  // P and S, and the cost before each
 };
 
 // Checks block j of the segment as kernel (1) does, without the pools; its descriptor in *d.
@@ -118,13 +130,14 @@ __device__ __forceinline__ Sum cluster_scan(cg::cluster_group& cluster, Shared& 
   Sum x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, x.tokens, o), b = __shfl_up_sync(0xFFFFFFFFu, x.blocks, o);
-    if (lane >= static_cast<uint32_t>(o)) x = x + Sum{t, b};
+    const Sum y{__shfl_up_sync(0xFFFFFFFFu, x.tokens, o), __shfl_up_sync(0xFFFFFFFFu, x.blocks, o),
+                __shfl_up_sync(0xFFFFFFFFu, x.cost, o)};
+    if (lane >= static_cast<uint32_t>(o)) x = x + y;
   }
   __syncthreads();  // the warp totals of the call before have been read
   if (lane == 31) s.warp[warp] = x;
   __syncthreads();
-  Sum before{0, 0}, all{0, 0};
+  Sum before{0, 0, 0}, all{0, 0, 0};
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < static_cast<int>(warp)) before = before + s.warp[w];
@@ -134,14 +147,14 @@ __device__ __forceinline__ Sum cluster_scan(cg::cluster_group& cluster, Shared& 
   if (n > 1) {
     if (threadIdx.x < n) cluster.map_shared_rank(&s, threadIdx.x)->cta[phase & 1][rank] = all;
     cluster.sync();
-    all = Sum{0, 0};
+    all = Sum{0, 0, 0};
     for (uint32_t c = 0; c < n; ++c) {
       if (c < rank) before = before + s.cta[phase & 1][c];
       all = all + s.cta[phase & 1][c];
     }
   }
   *total = all;
-  return Sum{before.tokens + x.tokens - v.tokens, before.blocks + x.blocks - v.blocks};
+  return Sum{before.tokens + x.tokens - v.tokens, before.blocks + x.blocks - v.blocks, before.cost + x.cost - v.cost};
 }
 
 __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
@@ -179,18 +192,18 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
     }
   };
   auto own_sum = [&]() {
-    Sum x{0, 0};
+    Sum x{0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) x = x + Sum{v[k], v[k] > 0 ? 1u : 0u};
+    for (int k = 0; k < kItems; ++k) x = x + block_sum(d[k].y, v[k]);
     return x;
   };
 
-  Sum before{0, 0}, total{0, 0};
+  Sum before{0, 0, 0}, total{0, 0, 0};
   if (one_round) {
     load(0);
     before = cluster_scan(cluster, s, own_sum(), phase++, &total);
   } else {
-    Sum x{0, 0};
+    Sum x{0, 0, 0};
     for (uint64_t base = 0; base < n; base += round) {
       load(static_cast<uint32_t>(base));
       x = x + own_sum();
@@ -204,10 +217,13 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
   const uint32_t low = plan.window != 0 && seen_from + 1u > plan.window ? seen_from + 1u - plan.window : 0u;
   const bool trimmed = low > 0;
   uint32_t n_first = total.blocks, n_skip = 0;  // P and S; without a trim every block is one of the first
-  Sum carry{0, 0};
+  uint32_t cost_first = total.cost, cost_skip = 0;
+  Sum carry{0, 0, 0};
   const uint32_t token_base = static_cast<uint32_t>(tfirst);  // used for rows of a sequence that fits only
   const uint32_t missing = q > context ? q - context : 0u;    // new tokens that the sequence does not have
-  if (threadIdx.x < 2) s.border[threadIdx.x] = threadIdx.x == 0 ? total.blocks : 0xFFFFFFFFu;
+  if (threadIdx.x < 4) {
+    s.border[threadIdx.x] = threadIdx.x == 0 ? total.blocks : threadIdx.x == 2 ? total.cost : 0xFFFFFFFFu;
+  }
   for (uint64_t base64 = 0; base64 < n; base64 += round) {
     if (!one_round) {
       load(static_cast<uint32_t>(base64));
@@ -222,28 +238,44 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
         __syncthreads();
         if (n_ctas > 1) cluster.sync();  // every CTA has set its borders
       }
-      uint32_t behind = 0xFFFFFFFFu, within = 0xFFFFFFFFu;
+      uint32_t behind = 0xFFFFFFFFu, within = 0xFFFFFFFFu, cost_behind = 0xFFFFFFFFu, cost_within = 0xFFFFFFFFu;
       Sum x = before;
 #pragma unroll
       for (int k = 0; k < kItems; ++k) {
         if (v[k] == 0) continue;
-        if (x.tokens >= plan.sinks) behind = min(behind, x.blocks);
-        if (x.tokens + v[k] > low) within = min(within, x.blocks);
-        x = x + Sum{v[k], 1u};
+        if (x.tokens >= plan.sinks) {
+          behind = min(behind, x.blocks);
+          cost_behind = min(cost_behind, x.cost);
+        }
+        if (x.tokens + v[k] > low) {
+          within = min(within, x.blocks);
+          cost_within = min(cost_within, x.cost);
+        }
+        x = x + block_sum(d[k].y, v[k]);
       }
       behind = __reduce_min_sync(0xFFFFFFFFu, behind);
       within = __reduce_min_sync(0xFFFFFFFFu, within);
+      cost_behind = __reduce_min_sync(0xFFFFFFFFu, cost_behind);
+      cost_within = __reduce_min_sync(0xFFFFFFFFu, cost_within);
       if ((threadIdx.x & 31) < n_ctas) {
         Shared* o = cluster.map_shared_rank(&s, threadIdx.x & 31);
-        if (behind != 0xFFFFFFFFu) atomicMin(&o->border[0], behind);
-        if (within != 0xFFFFFFFFu) atomicMin(&o->border[1], within);
+        if (behind != 0xFFFFFFFFu) {
+          atomicMin(&o->border[0], behind);
+          atomicMin(&o->border[2], cost_behind);
+        }
+        if (within != 0xFFFFFFFFu) {
+          atomicMin(&o->border[1], within);
+          atomicMin(&o->border[3], cost_within);
+        }
       }
       if (n_ctas > 1) cluster.sync();
       else __syncthreads();
       n_first = s.border[0];
       n_skip = s.border[1];
+      cost_first = s.border[2];
+      cost_skip = s.border[3];
     }
-    const uint32_t skip = max(n_skip, n_first);
+    const uint32_t skip = max(n_skip, n_first), cost_gap = max(cost_skip, cost_first) - cost_first;
     Sum x = before;
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
@@ -252,6 +284,8 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
       if (r < n_first || r >= n_skip) {
         const uint32_t at = static_cast<uint32_t>(first) + (r < n_first ? r : n_first + r - skip);
         reinterpret_cast<uint4*>(plan.d_blocks)[at] = make_uint4(d[k].x, d[k].y, d[k].z, start);
+        const uint32_t cost = x.cost + block_cost(d[k].y, v[k]);
+        plan.d_block_cost[at] = r < n_first ? cost : cost - cost_gap;
       }
       const uint32_t end = start + v[k];
       for (uint32_t t = max(start, seen_from); t < end; ++t) {
@@ -259,7 +293,7 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
         reinterpret_cast<uint2*>(plan.d_targets)[row] = make_uint2(d[k].w, t - start);
         plan.d_positions[row] = static_cast<int32_t>(t);
       }
-      x = x + Sum{v[k], 1u};
+      x = x + block_sum(d[k].y, v[k]);
     }
   }
 
@@ -281,6 +315,8 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
       if (fits && missing) atomicOr(p.err, dev::kErrPlanRange);
       plan.d_block_count[i] = trimmed ? (n_skip == 0xFFFFFFFFu ? n_first : n_first + total.blocks - max(n_skip, n_first))
                                       : total.blocks;
+      plan.d_cost[i] = trimmed ? (n_skip == 0xFFFFFFFFu ? cost_first : cost_first + total.cost - max(cost_skip, cost_first))
+                               : total.cost;
       plan.d_context[i] = context;
       if (!p.prefix_done) {
         plan.d_block_first[i] = static_cast<uint32_t>(min(first, uint64_t{plan.block_cap}));
@@ -351,7 +387,8 @@ extern "C" int hlkv_batch_plan(const HlkvBatchPlan* plan, const HlkvLayout* layo
   if (plan == nullptr || !layout_ok(layout) || d_err == nullptr || plan->max_query == 0) return HLKV_INVALID_ARGUMENT;
   if (plan->nseq == 0) return HLKV_OK;
   if (plan->d_block_first == nullptr || plan->d_block_count == nullptr || plan->d_token_first == nullptr ||
-      plan->d_context == nullptr || d_segs == nullptr || (plan->block_cap > 0 && plan->d_blocks == nullptr) ||
+      plan->d_context == nullptr || d_segs == nullptr || plan->d_cost == nullptr ||
+      (plan->block_cap > 0 && (plan->d_blocks == nullptr || plan->d_block_cost == nullptr)) ||
       (plan->token_cap > 0 && (plan->d_targets == nullptr || plan->d_positions == nullptr)) ||
       (table_size > 0 && d_table == nullptr) || (arena_size > 0 && d_arena == nullptr) ||
       (reinterpret_cast<uintptr_t>(plan->d_blocks) & 15u) != 0 || (reinterpret_cast<uintptr_t>(plan->d_targets) & 7u) != 0) {
@@ -359,8 +396,10 @@ extern "C" int hlkv_batch_plan(const HlkvBatchPlan* plan, const HlkvLayout* layo
   }
   // Grids stay below 2^31 CTAs with any cluster size.
   if (plan->nseq > 0x7FFFFFFFu / kMaxCluster) return HLKV_INVALID_ARGUMENT;
-  // Positions are 31 bits.
-  if (uint64_t{plan->block_cap} * layout->block_tokens > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
+  // Positions are 31 bits, and the sum of the costs (at most 14 per 16 tokens or block) 32.
+  if (uint64_t{plan->block_cap} * layout->block_tokens > 0x7FFFFFFFull || plan->block_cap > (1u << 27)) {
+    return HLKV_INVALID_ARGUMENT;
+  }
   Params p{};
   p.plan = *plan;
   p.table = reinterpret_cast<const uint4*>(d_table);

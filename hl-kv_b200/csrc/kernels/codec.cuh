@@ -37,6 +37,7 @@ enum : uint32_t {
   kErrPatchRange = 1u << 11,
   kErrOutAlign = 1u << 12,
   kErrPlanRange = 1u << 13,
+  kErrInternal = 1u << 14,
 };
 
 __device__ __forceinline__ uint32_t f16_bits(float x) { return __half_as_ushort(__float2half_rn(x)); }

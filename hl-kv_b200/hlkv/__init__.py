@@ -42,6 +42,7 @@ ERR_TOKEN_RANGE = 1 << 10
 ERR_PATCH_RANGE = 1 << 11
 ERR_OUT_ALIGN = 1 << 12
 ERR_PLAN_RANGE = 1 << 13
+ERR_INTERNAL = 1 << 14
 
 
 class Status:
@@ -101,7 +102,8 @@ class PlanArrays(C.Structure):
     _fields_ = [("nseq", C.c_uint32), ("max_query", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32),
                 ("block_cap", C.c_uint32), ("token_cap", C.c_uint32), ("block_first", C.c_void_p),
                 ("block_count", C.c_void_p), ("token_first", C.c_void_p), ("context", C.c_void_p),
-                ("blocks", C.c_void_p), ("targets", C.c_void_p), ("positions", C.c_void_p)]
+                ("blocks", C.c_void_p), ("targets", C.c_void_p), ("positions", C.c_void_p),
+                ("block_cost", C.c_void_p), ("cost", C.c_void_p)]
 
 
 class Rotary(C.Structure):
@@ -702,7 +704,8 @@ def _current_device() -> int:
 class BatchPlan:
     """The device arrays of one HlkvBatchPlan (all int32 tensors, views of one allocation):
     block_first, block_count, context [nseq], token_first [nseq + 1], blocks [block_cap, 4]
-    (slot, info, scale_ref, start), targets [token_cap, 2], positions [token_cap].
+    (slot, info, scale_ref, start), targets [token_cap, 2], positions [token_cap]; and block_cost
+    [block_cap], cost [nseq], by which batch_attention cuts its work.
 
     max_query: the most new tokens of a sequence; window: 0, or the tokens that a new token sees;
     sinks: first tokens that stay visible behind the window."""
@@ -712,16 +715,16 @@ class BatchPlan:
         import torch
         _need(min(nseq, block_cap, token_cap, window, sinks) >= 0 and max_query >= 1, "BatchPlan: negative size")
         parts, total = [], 0
-        for n in (4 * block_cap, 2 * token_cap, token_cap, nseq, nseq, nseq + 1, nseq):
+        for n in (4 * block_cap, 2 * token_cap, token_cap, nseq, nseq, nseq + 1, nseq, block_cap, nseq):
             parts.append((total, n))
             total += (n + 3) // 4 * 4
         buf = torch.zeros(max(total, 4), dtype=torch.int32, device=device)
         v = [buf[o:o + n] for o, n in parts]
         self.blocks, self.targets, self.positions = v[0].view(-1, 4), v[1].view(-1, 2), v[2]
-        self.block_first, self.block_count, self.token_first, self.context = v[3:]
+        self.block_first, self.block_count, self.token_first, self.context, self.block_cost, self.cost = v[3:]
         at = [buf.data_ptr() + 4 * o for o, _ in parts]
         self.c = PlanArrays(nseq, max_query, window, sinks, block_cap, token_cap, at[3], at[4], at[5], at[6], at[0],
-                            at[1], at[2])
+                            at[1], at[2], at[7], at[8])
         self.device = buf.device
 
 

@@ -81,9 +81,11 @@ enum {
   HLKV_ERR_TOKEN_RANGE = 1u << 10,    /* append target token >= block_tokens          */
   HLKV_ERR_PATCH_RANGE = 1u << 11,    /* delta patch target out of range              */
   HLKV_ERR_OUT_ALIGN = 1u << 12,      /* output offset not a multiple of 8 elements   */
-  HLKV_ERR_PLAN_RANGE = 1u << 13      /* a sequence that a batch plan cannot hold, or
+  HLKV_ERR_PLAN_RANGE = 1u << 13,     /* a sequence that a batch plan cannot hold, or
                                          with more new tokens than max_query or than
                                          it has tokens                                */
+  HLKV_ERR_INTERNAL = 1u << 14        /* a wait inside a kernel ran out of tries: a fault of
+                                         this library, the call's outputs are not valid */
 };
 
 /* ---- ABI records (byte-identical to hl::alloc, block_descriptor.hpp:137-150 and
@@ -366,6 +368,9 @@ typedef struct {
   HlkvPlanBlock* d_blocks;     /* [block_cap], 16-byte aligned */
   HlkvAppendTarget* d_targets; /* [token_cap], 8-byte aligned: where each new token goes */
   int32_t* d_positions;        /* [token_cap]: its position in its sequence */
+  uint32_t* d_block_cost;      /* [block_cap]: for the attention's cut, the cost of the sequence's
+                                  listed blocks up to and including this one */
+  uint32_t* d_cost;            /* [nseq]: of all of them */
 } HlkvBatchPlan;
 
 /*
@@ -386,7 +391,7 @@ typedef struct {
  *  - A sequence whose blocks or new tokens do not fit the arrays, or that has more than
  *    max_query new tokens, is planned as empty (context 0, no blocks, its rows padding) with
  *    HLKV_ERR_PLAN_RANGE.  New tokens beyond a sequence's tokens are padding, with the same bit.
- * block_cap * block_tokens is below 2^31 (positions are int32).
+ * block_cap * block_tokens is below 2^31 (positions are int32), and block_cap at most 2^27.
  * The device form of hlkv_table_build_exec_table (hetero_block_table.cpp:406-433) and of
  * hlkv_table_append_tokens' targets; the reference builds neither on the device.
  */

@@ -48,7 +48,8 @@ def _check(hlkv, segs, arena, table, qlens, T, cap_b=None, cap_t=None, max_query
     cap_t = int(sum(qlens)) if cap_t is None else cap_t
     max_query = max([1, *map(int, qlens)]) if max_query is None else max_query
     plan = hlkv.BatchPlan(nseq, cap_b, cap_t, max_query, window, sinks)
-    for t in (plan.blocks, plan.targets, plan.positions, plan.block_first, plan.block_count, plan.token_first, plan.context):
+    for t in (plan.blocks, plan.targets, plan.positions, plan.block_first, plan.block_count, plan.token_first, plan.context,
+              plan.block_cost, plan.cost):
         t.fill_(0x5A5A5A5A)
     err = torch.zeros(1, dtype=torch.int32, device="cuda")
     d_table, d_arena = _dev(table), _dev(arena)
@@ -70,6 +71,11 @@ def _check(hlkv, segs, arena, table, qlens, T, cap_b=None, cap_t=None, max_query
             if s["blocks"]:
                 blocks[b:b + len(s["blocks"])] = np.array(s["blocks"], np.uint32)
         assert np.array_equal(u(plan.blocks), blocks)
+        cost = np.full(cap_b, 0x5A5A5A5A, np.uint32)
+        for b, s in zip(bf, seqs):
+            cost[b:b + len(s["cost"])] = s["cost"]
+        assert np.array_equal(u(plan.block_cost), cost)
+        assert u(plan.cost).tolist() == [s["cost"][-1] if s["cost"] else 0 for s in seqs]
         assert np.array_equal(u(plan.targets), targets)
         assert np.array_equal(u(plan.positions).view(np.int32), positions)
 

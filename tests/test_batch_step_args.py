@@ -10,7 +10,7 @@ ODD = C.c_void_p(4100)
 
 def _plan(hlkv, **kw):
     d = dict(nseq=2, max_query=4, window=0, sinks=0, block_cap=8, token_cap=8, block_first=4096, block_count=4096,
-             token_first=4096, context=4096, blocks=4096, targets=4096, positions=4096)
+             token_first=4096, context=4096, blocks=4096, targets=4096, positions=4096, block_cost=4096, cost=4096)
     d.update(kw)
     return hlkv.PlanArrays(*d.values())
 
@@ -24,7 +24,7 @@ def test_plan_arguments(hlkv_lib):
     assert call(_plan(hlkv_lib, nseq=0)) == hlkv_lib.OK
     for kw in (dict(max_query=0), dict(block_first=None), dict(block_count=None), dict(token_first=None), dict(context=None),
                dict(blocks=None), dict(targets=None), dict(positions=None), dict(blocks=4104), dict(targets=4100),
-               dict(nseq=1 << 29), dict(block_cap=1 << 28)):
+               dict(nseq=1 << 29), dict(block_cap=1 << 28), dict(block_cost=None), dict(cost=None)):
         assert call(_plan(hlkv_lib, **kw)) == INV, kw
     assert call(_plan(hlkv_lib), err=None) == INV
     assert call(_plan(hlkv_lib), segs=None) == INV
@@ -89,6 +89,8 @@ def test_attention_arguments(hlkv_lib):
                dict(scale=float("nan")), dict(layout=hlkv_lib.Layout(16, 8, 256, 1)), dict(layout=hlkv_lib.Layout(1024, 8, 128, 1)),
                dict(plan=_plan(hlkv_lib, blocks=None)), dict(plan=_plan(hlkv_lib, blocks=4104)),
                dict(plan=_plan(hlkv_lib, context=None)), dict(plan=_plan(hlkv_lib, token_first=None)),
-               dict(plan=_plan(hlkv_lib, max_query=0)), dict(plan=_plan(hlkv_lib, token_cap=1 << 30))):
+               dict(ws=None), dict(ws=ODD), dict(plan=_plan(hlkv_lib, max_query=0)), dict(plan=_plan(hlkv_lib, block_cost=None)), dict(plan=_plan(hlkv_lib, cost=None)), dict(plan=_plan(hlkv_lib, token_cap=1 << 30))):
         assert call(**kw) == INV, kw
     assert L.hlkv_last_cuda_error() == 0
+    need = L.hlkv_batch_attention_workspace_bytes(C.byref(_plan(hlkv_lib)), C.byref(hlkv_lib.Layout(16, 8, 128, 1)), 32)
+    assert need > 0 and call(ws_bytes=need - 1) == hlkv_lib.BUFFER_TOO_SMALL
