@@ -5,7 +5,7 @@
 //
 // One CTA per SM takes an equal share of the batch's cost (the plan's per-block costs, in proportion
 // to the bytes), whatever the sequences' lengths: its range of the line on which all (sequence, head
-// group) units lie end to end.  A producer warp copies the blocks' codes and parameters as they are,
+// group) units lie end to end.  Two producer warps (K, V) copy the blocks' codes and parameters as they are,
 // by bulk copies, into a byte ring in shared memory: tiles of 16 tokens of a block, all heads of the
 // group (up to 8) at once, so that a copy is one long piece of the slot; a ring of bytes, not of
 // fixed stages, keeps as many INT4 bytes in flight as FP16 ones.  Consumer warps take one (tile, head)
@@ -20,6 +20,7 @@
 // The order of contraction is free, so every lane takes contiguous bytes of a row and pairs them
 // where they lie: K elements (j, j + 4) of each 8, V tokens (2q, 2q + 1).
 #include <cmath>
+#include <cstddef>
 
 #include "batch_attention.cuh"
 
@@ -28,44 +29,50 @@ namespace battn {
 namespace {
 
 constexpr uint32_t kStages = 16;
-constexpr uint32_t kTiles = 8;  // (tile, head) units of a stage: one per warp of a consumer group
+constexpr uint32_t kTiles = 8;  // (tile, head) units of a stage: one per warp of a consumer group, or a pair
 
-struct Tile {
-  uint32_t fn;   // format | tokens << 8 | scale mode << 16 | parameters in global memory << 24
-  uint32_t pos;  // position of its first token
-  uint32_t kc, vc;  // ring offsets of the K and V codes: [tokens][heads][row bytes]
-  uint32_t kp, vp;  // ring offsets of the first row's parameters, or the two halves of the K row's address
+// A tile's description (words at fixed offsets: consumers read them by address).
+struct alignas(16) Tile {
+  uint32_t fn;      // format | tokens << 8 | (1 << 16: every row sees all its tokens)
+  uint32_t pos;     // position of its first token
+  uint32_t kc, kp;  // shared-memory addresses of the K codes, [tokens][heads][row bytes], and of the first row's parameters
+  uint32_t vc, vp;  // the same for V
+  uint32_t row_step, token_step;  // bytes from a head's parameters to the next head's, and the next token's (0: block-wide)
   float ws, wb;     // block-wide parameters
+  uint32_t unused[2];
 };
-enum : uint32_t { kFirst = 1, kLast = 2, kDone = 4, kDirect = 8 };
-struct Stage {
-  Tile tile[kTiles];
-  uint32_t tiles, flags;
-  uint32_t seq, head0, heads, unit_slot;
+enum : uint32_t { kFirst = 1, kLast = 2, kDone = 4, kDirect = 8, kFirstStages = 16 };
+struct alignas(16) Stage {
+  Tile tile[2 * kTiles];
+  uint32_t tiles, flags, seq, head0;
+  uint32_t heads, unit_slot;
+  uint32_t pairs;  // two tiles a warp, of one format, 16 tokens each and seen whole
 };
 
 template <int kD, int kNB>
 struct Config {
   static constexpr int kWarps = kNB == 1 ? 16 : 8;  // consumers: 56 to 100 registers a lane hold the state of 8 or 16 rows
   static constexpr int kGroups = kWarps / 8;
-  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kThreads = (kWarps + 4) * 32;  // and a warpgroup of which one warp produces
   static constexpr int kRowsPad = kD + 4;  // floats of a row in the merge buffer: outputs, max, sum
-  static constexpr uint32_t kMergeBytes = kWarps * 8 * kNB * kRowsPad * 4;
-  static constexpr uint32_t kRing = (226u * 1024u - kMergeBytes - static_cast<uint32_t>(sizeof(Stage)) * kStages - 1024u) / 128u * 128u;
-  static constexpr uint32_t kSmem = kRing + kMergeBytes + sizeof(Stage) * kStages + 1024;
+  static constexpr uint32_t kMergeBytes = 8 * 8 * kNB * kRowsPad * 4;  // one consumer group's state
+  static constexpr uint32_t kQueryBytes = kWarps * (kNB * (kD / 32) * 512 + kNB * 64 + 16);  // WarpRows
+  static constexpr uint32_t kOther = kMergeBytes + static_cast<uint32_t>(sizeof(Stage)) * kStages + kQueryBytes;
+  static constexpr uint32_t kRing = (226u * 1024u - kOther) / 256u * 128u;  // of each half
+  static constexpr uint32_t kSmem = 2 * kRing + kOther;
 };
 
 struct Shared {
-  uint64_t full[kStages], empty[kStages], merged;
-  uint32_t offset[kStages];  // ring offsets of the stages' data
-  uint64_t warp_sum[17];
+  uint64_t full[2][kStages], empty[2][kStages], merged;  // of a stage's K half and its V half
+  uint32_t offset[2][kStages];  // ring offsets of the halves' data
+  uint64_t warp_sum[20];
   uint64_t total, base;  // cost of the batch; of the sequences before `seq`
   uint32_t seq;
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -73,10 +80,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 // Transposes an 8x8 matrix of binary16 held two columns to a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t m, uint32_t o) { return (a & m) | o; }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -116,6 +122,24 @@ __device__ __forceinline__ bool has_nonfinite(uint32_t h2) {
 template <int kD, uint32_t kF>
 constexpr uint32_t kRow = kF == dev::kFp16 ? kD * 2 : kF == dev::kInt4 ? kD / 2 : kD;
 
+// 1024 + c and 1024 + 16 c from masks -> (c - 8) / 8 by (1024 + c) / 8 - 129 and (1024 + 16 c) / 128 - 9: exact.
+// One logic operation holds one immediate, the mask; the other constant comes in a register.
+__device__ __forceinline__ uint32_t magic1024() {
+  uint32_t m;
+  asm("mov.b32 %0, 0x64006400;" : "=r"(m));
+  return m;
+}
+__device__ __forceinline__ uint32_t nibble_lo(uint32_t x, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(magic));
+  return hfma2(r, 0x30003000u, 0xD808D808u);
+}
+__device__ __forceinline__ uint32_t nibble_hi(uint32_t x, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(magic));
+  return hfma2(r, 0x20002000u, 0xC880C880u);
+}
+
 // Four pairs (j, j + 4) of the 8 elements at `w`, as binary16 (INT4: the code times 2^-24, binary16's
 // smallest step, so that masking a code is its conversion).
 template <uint32_t kF>
@@ -153,14 +177,14 @@ __device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, ui
       v[2 * j + 1] = __byte_perm(a[j], b[j], 0x7632);
     }
   } else if constexpr (kF == dev::kInt4) {
-    // 1024 + c and 1024 + 16 c by masks, then (1024 + c) / 8 - 129 and (1024 + 16 c) / 128 - 9: exact.
+    const uint32_t magic = magic1024();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint32_t x = __byte_perm(a[0], b[0], j == 0 ? 0x5410 : 0x7632), y = x >> 8;
-      v[4 * j] = hfma2(lop_and_or(x, 0x000F000Fu, 0x64006400u), 0x30003000u, 0xD808D808u);
-      v[4 * j + 1] = hfma2(lop_and_or(x, 0x00F000F0u, 0x64006400u), 0x20002000u, 0xC880C880u);
-      v[4 * j + 2] = hfma2(lop_and_or(y, 0x000F000Fu, 0x64006400u), 0x30003000u, 0xD808D808u);
-      v[4 * j + 3] = hfma2(lop_and_or(y, 0x00F000F0u, 0x64006400u), 0x20002000u, 0xC880C880u);
+      v[4 * j] = nibble_lo(x, magic);
+      v[4 * j + 1] = nibble_hi(x, magic);
+      v[4 * j + 2] = nibble_lo(y, magic);
+      v[4 * j + 3] = nibble_hi(y, magic);
     }
   } else {
     constexpr uint32_t kDown = kF == dev::kE4M3 ? 0x1C001C00u : 0x02000200u;  // 2^-8, 2^-15
@@ -182,22 +206,56 @@ constexpr float kValueUnit = kF == dev::kFp16 ? 1.0f : kF == dev::kE4M3 ? 0x1p8f
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
+// Loads by shared-memory address: 32 bits of address where a generic pointer takes 64.
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  const uint2 v = lds64(a);
+  return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+}
+
 // A warp's state for one (unit, head): lane (g, q) = (lane / 4, lane % 4) holds query columns 2q and
 // 2q + 1 of each column block, and head elements [g kD/8, (g + 1) kD/8).
 template <int kD, int kNB>
 struct State {
-  uint32_t q[kNB][kD / 16][2];  // Q^T fragments: column g, pairs (j, j + 4) of elements [quad kD/4, ...)
-  float acc[kNB][kD / 16][4];   // [.][mt]: element 2 mt of columns 2q, 2q + 1, then element 2 mt + 1; units of 2^E
+  float acc[kNB][kD / 16][4];  // [.][mt]: element 2 mt of columns 2q, 2q + 1, then element 2 mt + 1; units of 2^E
   float m[kNB][2], l[kNB][2], bias[kNB][2];  // l and bias: this lane's tokens only
-  float qsum[kNB][2];
-  int32_t pos[kNB][2];  // positions of the columns' tokens
   int E;
 };
 constexpr int kNoExponent = -1000;
 
+// What a warp keeps in shared memory for a piece: its Q^T fragments, and per column the scaled sum of q
+// and the position.
 template <int kD, int kNB>
-__device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, Rows rows, uint32_t context, uint32_t head,
-                                            uint32_t lane) {
+struct WarpRows {
+  uint4 q[kNB * (kD / 32)][32];  // column g, pairs (j, j + 4) of the 8-element groups of a quarter row
+  float qsum[8 * kNB];
+  int32_t pos[8 * kNB];
+  uint4 place;  // heads, head, first tile of a stage, tiles per round
+};
+
+// The warp's place in a stage.
+struct Place {
+  uint32_t rows;  // address of its WarpRows
+  uint32_t heads, head_i, lane;
+};
+
+template <int kD, int kNB>
+__device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, WarpRows<kD, kNB>* wr, Rows rows, uint32_t context,
+                                            uint32_t head, uint32_t lane) {
   const uint32_t g = lane >> 2, quad = lane & 3;
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
@@ -213,19 +271,21 @@ __device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, 
       const uint32_t x[4] = {w.x, w.y, w.z, w.w};
       uint32_t a[4];
       k_pairs<dev::kFp16>(x, a);
+      wr->q[nb * (kD / 32) + i][lane] = make_uint4(a[0], a[1], a[2], a[3]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s.q[nb][2 * i + j / 2][j % 2] = a[j];
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[j]));
         sum += f.x + f.y;
       }
     }
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+    if (quad == 0) {
+      wr->qsum[r] = sum * p.qscale;
+      wr->pos[r] = static_cast<int32_t>(context - rows.q + tok);
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      s.qsum[nb][c] = __shfl_sync(0xFFFFFFFFu, sum, (quad * 2 + c) * 4) * p.qscale;
-      s.pos[nb][c] = static_cast<int32_t>(context - rows.q + (nb * 8 + quad * 2 + c) / p.group);
       s.m[nb][c] = -INFINITY;
       s.l[nb][c] = s.bias[nb][c] = 0.0f;
     }
@@ -233,86 +293,120 @@ __device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, 
     for (int mt = 0; mt < kD / 16; ++mt) s.acc[nb][mt][0] = s.acc[nb][mt][1] = s.acc[nb][mt][2] = s.acc[nb][mt][3] = 0.0f;
   }
   s.E = kNoExponent;
+  __syncwarp();
 }
 
-// One tile (up to 16 tokens of one block and head).  `whole`: every row sees all its tokens.
-template <int kD, int kNB, uint32_t kF>
-__device__ __forceinline__ void tile_step(const Params& p, State<kD, kNB>& s, const uint8_t* kc, const uint8_t* vc,
-                                          uint32_t token_bytes, float2 (&kp)[2], float2 (&vp)[2], uint32_t n, uint32_t tile_pos,
-                                          bool whole, uint32_t lane) {
-  const uint32_t g = lane >> 2, quad = lane & 3;
+// 2^x by the hardware's approximation (2^-22 of the result; subnormal results are 0).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// {scale, bias} of the rows of tokens g and g + 8; `at` names the parameters' address in the description.
+// Rows behind the tile's tokens give what lies there in shared memory: their weights are 0.
+template <uint32_t kF>
+__device__ __forceinline__ void row_params(uint32_t t, uint32_t word, const Place& at, float2 (&out)[2]) {
+  if constexpr (kF == dev::kFp16) {
+    out[0] = out[1] = make_float2(1.0f, 0.0f);
+  } else {
+    const uint2 step = lds64(t + 24);
+    const uint32_t a = lds32(t + word) + at.head_i * step.x + (at.lane >> 2) * step.y, b = a + 8 * step.y;
+    if constexpr (kF == dev::kInt4) {
+      out[0] = lds_f2(a);
+      out[1] = lds_f2(b);
+    } else {
+      out[0] = make_float2(__uint_as_float(lds32(a)), 0.0f);
+      out[1] = make_float2(__uint_as_float(lds32(b)), 0.0f);
+    }
+  }
+}
+
+// Scores of tiles t[] in units of log2: lane (g, quad) has tokens g, g + 8 of columns 2 quad, 2 quad + 1.
+template <int kD, int kNB, uint32_t kF, int kNT>
+__device__ __forceinline__ void scores(const Params& p, const uint32_t (&t)[kNT], const Place& at, float (&sc)[kNT][kNB][4]) {
+  const uint32_t g = at.lane >> 2, quad = at.lane & 3;
+  constexpr uint32_t kRb = kRow<kD, kF>;
   constexpr int kW = kWords<kF>;
-  // ---- scores
-  float sc[kNB][4];
+  constexpr int kG8 = kD / 32;           // groups of 8 elements in a lane's quarter row
+  constexpr uint32_t kBytes = kRb / 4;  // of a quarter row: 8 to 64
+  constexpr int kPer = kF == dev::kFp16 ? 1 : kF == dev::kInt4 ? kG8 : 2;  // groups per load
+  const uint32_t row = (at.head_i + g * at.heads) * kRb + quad * kBytes, eight = 8 * at.heads * kRb;
+  uint32_t r0[kNT];
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.0f;
-  {
-    constexpr int kG8 = kD / 32;                 // groups of 8 elements in a lane's quarter row
-    constexpr uint32_t kBytes = kRow<kD, kF> / 4;  // of a quarter row: 8 to 64
-    const uint8_t* r0 = kc + g * token_bytes + quad * kBytes;
-    const uint8_t* r1 = r0 + 8 * token_bytes;
-    constexpr int kPer = kF == dev::kFp16 ? 1 : kF == dev::kInt4 ? kG8 : 2;  // groups per load
+  for (int k = 0; k < kNT; ++k) {
+    r0[k] = lds32(t[k] + 8) + row;
 #pragma unroll
-    for (int i = 0; i < kG8; i += kPer) {
-      uint32_t w0[kPer * kW], w1[kPer * kW];
-      if constexpr (kPer * kW == 4) {
-        *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(r0 + i * kW * 4);
-        *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(r1 + i * kW * 4);
-      } else {
-        *reinterpret_cast<uint2*>(w0) = *reinterpret_cast<const uint2*>(r0 + i * kW * 4);
-        *reinterpret_cast<uint2*>(w1) = *reinterpret_cast<const uint2*>(r1 + i * kW * 4);
+    for (int nb = 0; nb < kNB; ++nb) sc[k][nb][0] = sc[k][nb][1] = sc[k][nb][2] = sc[k][nb][3] = 0.0f;
+  }
+  const uint32_t qa = at.rows + at.lane * 16;
+#pragma unroll
+  for (int i = 0; i < kG8; i += kPer) {
+    uint32_t w[kNT][2][kPer * kW];
+#pragma unroll
+    for (int k = 0; k < kNT; ++k) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t r = r0[k] + (h ? eight : 0u) + i * kW * 4;
+        if constexpr (kPer * kW == 4) *reinterpret_cast<uint4*>(w[k][h]) = lds128(r);
+        else *reinterpret_cast<uint2*>(w[k][h]) = lds64(r);
       }
+    }
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < kPer; ++j) {
+#pragma unroll
+      for (int k = 0; k < kNT; ++k) {
         uint32_t a[4], b[4];
-        k_pairs<kF>(w0 + j * kW, a);
-        k_pairs<kF>(w1 + j * kW, b);
+        k_pairs<kF>(w[k][0] + j * kW, a);
+        k_pairs<kF>(w[k][1] + j * kW, b);
 #pragma unroll
         for (int nb = 0; nb < kNB; ++nb) {
-          mma16816(sc[nb], a[0], b[0], a[1], b[1], s.q[nb][2 * (i + j)][0], s.q[nb][2 * (i + j)][1]);
-          mma16816(sc[nb], a[2], b[2], a[3], b[3], s.q[nb][2 * (i + j) + 1][0], s.q[nb][2 * (i + j) + 1][1]);
+          const uint4 q = lds128(qa + (nb * kG8 + i + j) * 512);
+          mma16816(sc[k][nb], a[0], b[0], a[1], b[1], q.x, q.y);
+          mma16816(sc[k][nb], a[2], b[2], a[3], b[3], q.z, q.w);
         }
       }
     }
   }
-  // ---- softmax; this lane: tokens g and g + 8 (t), columns 2 quad and 2 quad + 1 (c)
-  float pr[kNB][4];
-  const bool v0 = g < n, v1 = g + 8 < n;
-  const float k0 = kp[0].x * (p.qscale * kKeyUnit<kF>), k1 = kp[1].x * (p.qscale * kKeyUnit<kF>);
-  bool grow = false;
-  float mx[kNB][2];
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int k = 0; k < kNT; ++k) {
+    float2 kp[2];
+    row_params<kF>(t[k], 12, at, kp);
+    const float unit = p.qscale * kKeyUnit<kF>, k0 = kp[0].x * unit, k1 = kp[1].x * unit;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float x0 = sc[nb][c] * k0, x1 = sc[nb][2 + c] * k1;
-      if constexpr (kF != dev::kFp16) {
-        x0 = fmaf(kp[0].y, s.qsum[nb][c], x0);
-        x1 = fmaf(kp[1].y, s.qsum[nb][c], x1);
+    for (int nb = 0; nb < kNB; ++nb) {
+      float2 qs = make_float2(0.0f, 0.0f);
+      if constexpr (kF == dev::kInt4) qs = lds_f2(at.rows + kNB * kG8 * 512 + (nb * 8 + quad * 2) * 4);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        sc[k][nb][c] *= k0;
+        sc[k][nb][2 + c] *= k1;
+        if constexpr (kF == dev::kInt4) {
+          sc[k][nb][c] = fmaf(kp[0].y, c ? qs.y : qs.x, sc[k][nb][c]);
+          sc[k][nb][2 + c] = fmaf(kp[1].y, c ? qs.y : qs.x, sc[k][nb][2 + c]);
+        }
       }
-      bool s0 = v0, s1 = v1;
-      if (!whole) {
-        const int32_t d0 = s.pos[nb][c] - static_cast<int32_t>(tile_pos + g), d1 = d0 - 8;
-        s0 = s0 && d0 >= 0 && (p.window == 0 || static_cast<uint32_t>(d0) < p.window || tile_pos + g < p.sinks);
-        s1 = s1 && d1 >= 0 && (p.window == 0 || static_cast<uint32_t>(d1) < p.window || tile_pos + g + 8 < p.sinks);
-      }
-      pr[nb][c] = s0 ? x0 : -INFINITY;
-      pr[nb][2 + c] = s1 ? x1 : -INFINITY;
-      float v = fmaxf(pr[nb][c], pr[nb][2 + c]);
-      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
-      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
-      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
-      mx[nb][c] = v;
-      grow = grow || v > s.m[nb][c] + 8.0f;
     }
   }
-  // The reference maximum moves only when a score passes it by 8: weights reach 2^8 at most.
+}
+
+// The reference maximum moves only when a score passes it by 8: weights reach 2^8 at most.  `top`: this
+// lane's largest scores.
+template <int kD, int kNB>
+__device__ __forceinline__ void follow_maximum(State<kD, kNB>& s, float (&top)[kNB][2]) {
+  bool grow = false;
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) grow = grow || top[nb][0] > s.m[nb][0] + 8.0f || top[nb][1] > s.m[nb][1] + 8.0f;
   if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float mn = fmaxf(s.m[nb][c], mx[nb][c]);
+        float v = top[nb][c];
+        v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
+        v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
+        v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
+        const float mn = fmaxf(s.m[nb][c], v);
         const float a = mn == -INFINITY ? 1.0f : exp2f(s.m[nb][c] - mn);
         s.m[nb][c] = mn;
         s.l[nb][c] *= a;
@@ -325,267 +419,447 @@ __device__ __forceinline__ void tile_step(const Params& p, State<kD, kNB>& s, co
       }
     }
   }
-  // ---- the tile's exponent: of the largest finite value scale among its tokens
-  const float u0 = v0 ? vp[0].x * kValueUnit<kF> : 0.0f, u1 = v1 ? vp[1].x * kValueUnit<kF> : 0.0f;
-  const uint32_t b0 = __float_as_uint(u0) & 0x7FFFFFFFu, b1 = __float_as_uint(u1) & 0x7FFFFFFFu;
-  const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(b0 < 0x7F800000u ? b0 : 0u, b1 < 0x7F800000u ? b1 : 0u));
-  // (scales beyond 2^60 or below 2^-60 are taken as those)
-  const int e = min(max(static_cast<int>(top >> 23) - 127, -60), 60);
-  if (e > s.E + 6 || (e < s.E - 6 && top != 0)) {
-    if (s.E != kNoExponent) {
-      const float f = exp2f(static_cast<float>(s.E - e));
+}
+
+// The accumulators' unit follows a tile's exponent: that of the largest value scale among its tokens, `top`
+// its bits (scales beyond 2^60 or below 2^-60 are taken as those).
+template <int kD, int kNB>
+__device__ __forceinline__ void follow_exponent(State<kD, kNB>& s, uint32_t top) {
+  const int d = static_cast<int>(top >> 23) - 127 - s.E;
+  if (d > 6 || d < -6) {
+    const int e = min(max(static_cast<int>(top >> 23) - 127, -60), 60);
+    if (e > s.E || top != 0) {
+      if (s.E != kNoExponent) {
+        const float f = exp2f(static_cast<float>(s.E - e));
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) {
+        for (int nb = 0; nb < kNB; ++nb) {
 #pragma unroll
-        for (int mt = 0; mt < kD / 16; ++mt) {
+          for (int mt = 0; mt < kD / 16; ++mt) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s.acc[nb][mt][k] *= f;
+            for (int k = 0; k < 4; ++k) s.acc[nb][mt][k] *= f;
+          }
+        }
+      }
+      s.E = e;
+    }
+  }
+}
+
+// A lane's chunk of 8 elements (i-th of kD / 64) of tokens 2 quad, + 1, + 8, + 9 of a tile at `base` -> pairs of
+// the first two and of the last two.  kShort: tokens from n on are taken as zeros.
+template <int kD, uint32_t kF, bool kShort>
+struct Chunks {
+  static constexpr int kW = kWords<kF>, kOnce = kF == dev::kFp16 ? 1 : kD / 64;  // in one load where it is at most 16 bytes
+  uint32_t w[4][kOnce * kW];
+  __device__ __forceinline__ void take(uint32_t base, uint32_t token_bytes, int i, uint32_t quad, uint32_t n, uint32_t (&lo)[8],
+                                       uint32_t (&hi)[8]) {
+    if (i % kOnce == 0) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t tok = (t & 1) + (t & 2) * 4, r = base + tok * token_bytes + i * kW * 4;
+        if constexpr (kOnce * kW == 4) *reinterpret_cast<uint4*>(w[t]) = lds128(r);
+        else if constexpr (kOnce * kW == 2) *reinterpret_cast<uint2*>(w[t]) = lds64(r);
+        else w[t][0] = lds32(r);
+        if (kShort && 2 * quad + tok >= n) {
+#pragma unroll
+          for (int k = 0; k < kOnce * kW; ++k) w[t][k] = 0u;
         }
       }
     }
-    s.E = e;
+    v_pairs<kF>(w[0] + i % kOnce * kW, w[1] + i % kOnce * kW, lo);
+    v_pairs<kF>(w[2] + i % kOnce * kW, w[3] + i % kOnce * kW, hi);
   }
+};
+
+// Scores and exponentials of kNT tiles of one format that every row sees whole; kShort: with n[] tokens.
+// The K half of the stage is given back after the scores, if empty_k names it.
+template <int kD, int kNB, uint32_t kF, int kNT, bool kShort>
+__device__ __forceinline__ bool step(const Params& p, State<kD, kNB>& s, const uint32_t (&t)[kNT], const uint32_t (&n)[kNT],
+                                     const Place& at, uint64_t* empty_k, uint64_t* full_v, uint32_t parity) {
+  const uint32_t g = at.lane >> 2, quad = at.lane & 3;
+  constexpr uint32_t kRb = kRow<kD, kF>;
+  float pr[kNT][kNB][4];
+  scores<kD, kNB, kF, kNT>(p, t, at, pr);
+  if (kNT == 2 || empty_k != nullptr) {
+    __syncwarp();
+    if (at.lane == 0) mbar_arrive(empty_k);
+  }
+  float top[kNB][2];
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      top[nb][c] = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kNT; ++k) {
+        if constexpr (kShort) {
+          if (g >= n[k]) pr[k][nb][c] = -INFINITY;
+          if (g + 8 >= n[k]) pr[k][nb][2 + c] = -INFINITY;
+        }
+        top[nb][c] = fmaxf(top[nb][c], fmaxf(pr[k][nb][c], pr[k][nb][2 + c]));
+      }
+    }
+  }
+  follow_maximum(s, top);
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float ref = s.m[nb][c];
+      if (kShort && ref == -INFINITY) ref = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kNT; ++k) {
+        pr[k][nb][c] = ex2(pr[k][nb][c] - ref);
+        pr[k][nb][2 + c] = ex2(pr[k][nb][2 + c] - ref);
+        s.l[nb][c] += pr[k][nb][c] + pr[k][nb][2 + c];
+      }
+    }
+  }
+  if (!mbar_wait(full_v, parity)) return false;
+#pragma unroll
+  for (int k = 0; k < kNT; ++k) {
+    if (kShort && n[k] == 0) continue;
+    // ---- weights: the exponential times the value row's scale, in units of 2^E
+    float2 vp[2];
+    row_params<kF>(t[k], 20, at, vp);
+    if constexpr (kShort) {
+      if (g >= n[k]) vp[0] = make_float2(0.0f, 0.0f);
+      if (g + 8 >= n[k]) vp[1] = make_float2(0.0f, 0.0f);
+    }
+    const float u0 = vp[0].x * kValueUnit<kF>, u1 = vp[1].x * kValueUnit<kF>;
+    follow_exponent(s, kF == dev::kFp16 ? 0x3F800000u
+                                        : __reduce_max_sync(0xFFFFFFFFu, max(__float_as_uint(u0) & 0x7FFFFFFFu,
+                                                                             __float_as_uint(u1) & 0x7FFFFFFFu)));
+    const float down = pow2(-s.E), f0 = u0 * down, f1 = u1 * down;
+    const float beta0 = fmaf(8.0f, vp[0].x, vp[0].y), beta1 = fmaf(8.0f, vp[1].x, vp[1].y);
+    uint32_t pb[kNB][2];
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) {
+      pb[nb][0] = transpose8(dev::pack_f16x2(pr[k][nb][0] * f0, pr[k][nb][1] * f0));
+      pb[nb][1] = transpose8(dev::pack_f16x2(pr[k][nb][2] * f1, pr[k][nb][3] * f1));
+      if constexpr (kF == dev::kInt4) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) s.bias[nb][c] = fmaf(pr[k][nb][2 + c], beta1, fmaf(pr[k][nb][c], beta0, s.bias[nb][c]));
+      }
+    }
+    // ---- O^T += V^T W^T
+    const uint32_t token_bytes = at.heads * kRb;
+    const uint32_t base = lds32(t[k] + 16) + (at.head_i + 2 * quad * at.heads) * kRb + g * (kRb / 8);
+    Chunks<kD, kF, kShort> ch;
+#pragma unroll
+    for (int i = 0; i < kD / 64; ++i) {
+      uint32_t lo[8], hi[8];
+      ch.take(base, token_bytes, i, quad, n[k], lo, hi);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb) {
+          mma16816(s.acc[nb][4 * i + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[nb][0], pb[nb][1]);
+        }
+      }
+    }
+  }
+  return true;
+}
+
+// ---- tiles that some row sees in part: one at a time, out of line ------------------------------------
+
+// One tile as a warp sees it.
+struct View {
+  uint32_t t, n, pos;
+};
+// Whether the query row at position `at` sees a tile's token.
+__device__ __forceinline__ bool visible(const Params& p, int32_t at, const View& v, uint32_t tok) {
+  const int32_t d = at - static_cast<int32_t>(v.pos + tok);
+  return tok < v.n && d >= 0 && (p.window == 0 || static_cast<uint32_t>(d) < p.window || v.pos + tok < p.sinks);
+}
+// A query column's position.
+template <int kD, int kNB>
+__device__ __forceinline__ int32_t position(const Place& at, uint32_t col) {
+  return static_cast<int32_t>(lds32(at.rows + kNB * (kD / 32) * 512 + 32 * kNB + col * 4));
+}
+
+// O^T += V^T W^T of such a tile.  Where it holds values that are not finite, or scales far apart, it is taken
+// row by row, so that a row is not touched by what it does not see.
+template <int kD, int kNB, uint32_t kF>
+__device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, const View& v, const Place& at,
+                                            const float (&pr)[kNB][4]) {
+  const uint32_t g = at.lane >> 2, quad = at.lane & 3;
+  constexpr uint32_t kRb = kRow<kD, kF>;
+  float2 vp[2];
+  row_params<kF>(v.t, 20, at, vp);
+  if (g >= v.n) vp[0] = make_float2(0.0f, 0.0f);
+  if (g + 8 >= v.n) vp[1] = make_float2(0.0f, 0.0f);
+  const float u0 = vp[0].x * kValueUnit<kF>, u1 = vp[1].x * kValueUnit<kF>;
+  const uint32_t b0 = __float_as_uint(u0) & 0x7FFFFFFFu, b1 = __float_as_uint(u1) & 0x7FFFFFFFu;
+  const uint32_t fin0 = b0 < 0x7F800000u ? b0 : 0u, fin1 = b1 < 0x7F800000u ? b1 : 0u;
+  const uint32_t high = __reduce_max_sync(0xFFFFFFFFu, max(fin0, fin1));
+  const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, min(g < v.n ? b0 : 0xFFFFFFFFu, g + 8 < v.n ? b1 : 0xFFFFFFFFu));
+  const bool apart = __any_sync(0xFFFFFFFFu, b0 >= 0x7F800000u || b1 >= 0x7F800000u) || high > low + (8u << 23);
+  follow_exponent(s, high);
   const float down = pow2(-s.E), f0 = u0 * down, f1 = u1 * down;
-  const float beta0 = kF == dev::kInt4 ? fmaf(8.0f, vp[0].x, vp[0].y) : vp[0].y;
-  const float beta1 = kF == dev::kInt4 ? fmaf(8.0f, vp[1].x, vp[1].y) : vp[1].y;
+  const float beta0 = fmaf(8.0f, vp[0].x, vp[0].y), beta1 = fmaf(8.0f, vp[1].x, vp[1].y);  // INT4: what (code - 8) / 8 leaves
   uint32_t pb[kNB][2];
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
     float w[4];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const float ref = s.m[nb][c] == -INFINITY ? 0.0f : s.m[nb][c];
-      const float p0 = exp2f(pr[nb][c] - ref), p1 = exp2f(pr[nb][2 + c] - ref);
-      pr[nb][c] = p0;
-      pr[nb][2 + c] = p1;
-      s.l[nb][c] += p0 + p1;
+      const float p0 = pr[nb][c], p1 = pr[nb][2 + c];
       // a hidden token's weight is 0 whatever its parameters hold
       w[c] = p0 == 0.0f ? 0.0f : p0 * f0;
       w[2 + c] = p1 == 0.0f ? 0.0f : p1 * f1;
-      if constexpr (kF != dev::kFp16) {
-        s.bias[nb][c] += (p0 == 0.0f ? 0.0f : p0 * beta0) + (p1 == 0.0f ? 0.0f : p1 * beta1);
+      if constexpr (kF == dev::kInt4) {
+        if (p0 != 0.0f) s.bias[nb][c] = fmaf(p0, beta0, s.bias[nb][c]);
+        if (p1 != 0.0f) s.bias[nb][c] = fmaf(p1, beta1, s.bias[nb][c]);
       }
     }
     pb[nb][0] = transpose8(dev::pack_f16x2(w[0], w[1]));
     pb[nb][1] = transpose8(dev::pack_f16x2(w[2], w[3]));
   }
-  // ---- values; this lane: tokens 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9
-  // In a tile that some row sees in part, a value that is not finite, or a scale far above the others',
-  // must not touch the rows that do not see it: such a tile is taken row by row.
-  bool apart = false;
-  if (!whole && n > 0) {
-    const uint32_t low0 = v0 ? b0 : 0xFFFFFFFFu, low1 = v1 ? b1 : 0xFFFFFFFFu;
-    const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, min(low0, low1));
-    apart = __any_sync(0xFFFFFFFFu, (v0 && b0 >= 0x7F800000u) || (v1 && b1 >= 0x7F800000u)) || top > low + (8u << 23);
-  }
+  const uint32_t token_bytes = at.heads * kRb;
+  const uint32_t base = lds32(v.t + 16) + (at.head_i + 2 * quad * at.heads) * kRb + g * (kRb / 8);
+  Chunks<kD, kF, true> ch;
 #pragma unroll
   for (int i = 0; i < kD / 64; ++i) {
     uint32_t lo[8], hi[8];
-    {
-      uint32_t w[4][kW];
+    ch.take(base, token_bytes, i, quad, v.n, lo, hi);
+    bool bad = false;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t tok = 2 * quad + (t & 1) + (t & 2) * 4;
-        const uint8_t* r = vc + tok * token_bytes + g * (kRow<kD, kF> / 8) + i * kW * 4;
-        if constexpr (kW == 4) *reinterpret_cast<uint4*>(w[t]) = *reinterpret_cast<const uint4*>(r);
-        else if constexpr (kW == 2) *reinterpret_cast<uint2*>(w[t]) = *reinterpret_cast<const uint2*>(r);
-        else w[t][0] = *reinterpret_cast<const uint32_t*>(r);
-        if (tok >= n) {
-#pragma unroll
-          for (int k = 0; k < kW; ++k) w[t][k] = 0u;
-        }
-      }
-      v_pairs<kF>(w[0], w[1], lo);
-      v_pairs<kF>(w[2], w[3], hi);
-    }
-    if (!whole) {
-      bool bad = false;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) bad = bad || has_nonfinite(lo[k]) || has_nonfinite(hi[k]);
-      if (__any_sync(0xFFFFFFFFu, bad) || apart) {
+    for (int k = 0; k < 8; ++k) bad = bad || has_nonfinite(lo[k]) || has_nonfinite(hi[k]);
+    if (__any_sync(0xFFFFFFFFu, bad) || apart) {
 #pragma unroll 1
-        for (int col = 0; col < 8 * kNB; ++col) {
-          // this row's view of the 16 tokens, and the exponent of the scales that it sees
-          const int32_t at = __shfl_sync(0xFFFFFFFFu, kNB == 1 || col < 8 ? ((col & 1) ? s.pos[0][1] : s.pos[0][0])
-                                                                         : ((col & 1) ? s.pos[kNB - 1][1] : s.pos[kNB - 1][0]),
-                                         (col & 7) >> 1);
-          auto sees = [&](uint32_t tok) {
-            const int32_t d = at - static_cast<int32_t>(tile_pos + tok);
-            return tok < n && d >= 0 && (p.window == 0 || static_cast<uint32_t>(d) < p.window || tile_pos + tok < p.sinks);
-          };
-          const uint32_t mine = __reduce_max_sync(0xFFFFFFFFu, max(sees(g) && b0 < 0x7F800000u ? b0 : 0u,
-                                                                  sees(g + 8) && b1 < 0x7F800000u ? b1 : 0u));
-          const int ec = min(max(static_cast<int>(mine >> 23) - 127, -60), 60);
-          const float dc = pow2(-ec), up = exp2f(static_cast<float>(ec - s.E));
-          const int nb = col >> 3;
-          float w[4];
+      for (int col = 0; col < 8 * kNB; ++col) {
+        // this row's view of the 16 tokens, and the exponent of the scales that it sees
+        const int32_t row_at = position<kD, kNB>(at, col);
+        const uint32_t mine = __reduce_max_sync(0xFFFFFFFFu, max(visible(p, row_at, v, g) ? fin0 : 0u,
+                                                                visible(p, row_at, v, g + 8) ? fin1 : 0u));
+        const int ec = min(max(static_cast<int>(mine >> 23) - 127, -60), 60);
+        const float dc = pow2(-ec), up = exp2f(static_cast<float>(ec - s.E));
+        const int nb = col >> 3;
+        float x[4];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float p0 = nb == 0 ? pr[0][c] : pr[kNB - 1][c], p1 = nb == 0 ? pr[0][2 + c] : pr[kNB - 1][2 + c];
-            w[c] = p0 == 0.0f ? 0.0f : p0 * (u0 * dc);
-            w[2 + c] = p1 == 0.0f ? 0.0f : p1 * (u1 * dc);
-          }
-          const uint32_t x0 = transpose8(dev::pack_f16x2(w[0], w[1])), x1 = transpose8(dev::pack_f16x2(w[2], w[3]));
-          const uint32_t keep_lo = (sees(2 * quad) ? 0xFFFFu : 0u) | (sees(2 * quad + 1) ? 0xFFFF0000u : 0u);
-          const uint32_t keep_hi = (sees(2 * quad + 8) ? 0xFFFFu : 0u) | (sees(2 * quad + 9) ? 0xFFFF0000u : 0u);
+        for (int c = 0; c < 2; ++c) {
+          const float p0 = nb == 0 ? pr[0][c] : pr[kNB - 1][c], p1 = nb == 0 ? pr[0][2 + c] : pr[kNB - 1][2 + c];
+          x[c] = p0 == 0.0f ? 0.0f : p0 * (u0 * dc);
+          x[2 + c] = p1 == 0.0f ? 0.0f : p1 * (u1 * dc);
+        }
+        const uint32_t x0 = transpose8(dev::pack_f16x2(x[0], x[1])), x1 = transpose8(dev::pack_f16x2(x[2], x[3]));
+        const uint32_t keep_lo = (visible(p, row_at, v, 2 * quad) ? 0xFFFFu : 0u) | (visible(p, row_at, v, 2 * quad + 1) ? 0xFFFF0000u : 0u);
+        const uint32_t keep_hi = (visible(p, row_at, v, 2 * quad + 8) ? 0xFFFFu : 0u) |
+                                 (visible(p, row_at, v, 2 * quad + 9) ? 0xFFFF0000u : 0u);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma16816(t, lo[2 * k] & keep_lo, lo[2 * k + 1] & keep_lo, hi[2 * k] & keep_hi, hi[2 * k + 1] & keep_hi, x0, x1);
+        for (int k = 0; k < 4; ++k) {
+          float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma16816(t, lo[2 * k] & keep_lo, lo[2 * k + 1] & keep_lo, hi[2 * k] & keep_hi, hi[2 * k + 1] & keep_hi, x0, x1);
 #pragma unroll
-            for (int b = 0; b < kNB; ++b) {
+          for (int b = 0; b < kNB; ++b) {
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                if (static_cast<int>(b * 8 + quad * 2 + c) == col) {
-                  s.acc[b][4 * i + k][c] = fmaf(t[c], up, s.acc[b][4 * i + k][c]);
-                  s.acc[b][4 * i + k][2 + c] = fmaf(t[2 + c], up, s.acc[b][4 * i + k][2 + c]);
-                }
+            for (int c = 0; c < 2; ++c) {
+              if (static_cast<int>(b * 8 + quad * 2 + c) == col) {
+                s.acc[b][4 * i + k][c] = fmaf(t[c], up, s.acc[b][4 * i + k][c]);
+                s.acc[b][4 * i + k][2 + c] = fmaf(t[2 + c], up, s.acc[b][4 * i + k][2 + c]);
               }
             }
           }
         }
-        continue;
       }
-    }
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 4; ++k) {
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) {
-        mma16816(s.acc[nb][4 * i + k], lo[2 * k], lo[2 * k + 1], hi[2 * k], hi[2 * k + 1], pb[nb][0], pb[nb][1]);
+        for (int nb = 0; nb < kNB; ++nb) {
+          mma16816(s.acc[nb][4 * i + k], lo[2 * k], lo[2 * k + 1], hi[2 * k], hi[2 * k + 1], pb[nb][0], pb[nb][1]);
+        }
       }
     }
   }
 }
 
-// ---- the producer warp -------------------------------------------------------------------------
+template <int kD, int kNB, uint32_t kF>
+__device__ __forceinline__ void edge_step(const Params& p, State<kD, kNB>& s, const View& v, const Place& at) {
+  const uint32_t g = at.lane >> 2, quad = at.lane & 3;
+  const uint32_t t[1] = {v.t};
+  float sc[1][kNB][4], top[kNB][2];
+  scores<kD, kNB, kF, 1>(p, t, at, sc);
+  float(&pr)[kNB][4] = sc[0];
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int32_t row_at = position<kD, kNB>(at, nb * 8 + quad * 2 + c);
+      if (!visible(p, row_at, v, g)) pr[nb][c] = -INFINITY;
+      if (!visible(p, row_at, v, g + 8)) pr[nb][2 + c] = -INFINITY;
+      top[nb][c] = fmaxf(pr[nb][c], pr[nb][2 + c]);
+    }
+  }
+  follow_maximum(s, top);
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float ref = s.m[nb][c] == -INFINITY ? 0.0f : s.m[nb][c];  // nothing seen yet
+      pr[nb][c] = ex2(pr[nb][c] - ref);
+      pr[nb][2 + c] = ex2(pr[nb][2 + c] - ref);
+      s.l[nb][c] += pr[nb][c] + pr[nb][2 + c];
+    }
+  }
+  edge_values<kD, kNB, kF>(p, s, v, at, pr);
+}
+
+// Out of line, with the state in memory: these tiles are few, and their code's registers are not the stream's.
+template <int kD, int kNB>
+__device__ __noinline__ void edge_tile(const Params& p, State<kD, kNB>* state, uint32_t t, const Place at) {
+  State<kD, kNB> s = *state;
+  const uint2 a = lds64(t);
+  const View v{t, (a.x >> 8) & 0xFFu, a.y};
+  switch (a.x & 0xFFu) {
+    case dev::kFp16: edge_step<kD, kNB, dev::kFp16>(p, s, v, at); break;
+    case dev::kE4M3: edge_step<kD, kNB, dev::kE4M3>(p, s, v, at); break;
+    case dev::kE5M2: edge_step<kD, kNB, dev::kE5M2>(p, s, v, at); break;
+    default: edge_step<kD, kNB, dev::kInt4>(p, s, v, at); break;
+  }
+  *state = s;
+}
+
+// ---- the producer warps --------------------------------------------------------------------------
+// One fills the ring of the K halves, one that of the V halves; both walk the same stages.  The K warp also
+// writes the stages' descriptions.
 template <int kD, int kNB>
 struct Producer {
   using C = Config<kD, kNB>;
   const Params& p;
   Shared& sh;
   Stage* stages;
-  uint8_t* ring;
-  uint32_t lane;
-  uint32_t st = 0, oldest = 0, head = 0;
+  uint8_t* ring;  // this half's
+  uint32_t ring_at;  // its address
+  uint32_t half, lane;
+  uint32_t st = 0;      // stages emitted
+  uint32_t oldest = 0;  // the first stage whose data is still in use
+  uint32_t head = 0;
   bool ok = true;
 
-  __device__ __forceinline__ bool pop() {
-    ok = ok && mbar_wait(&sh.empty[oldest % kStages], (oldest / kStages) & 1);
+  __device__ __forceinline__ void pop() {
+    ok = ok && mbar_wait(&sh.empty[half][oldest % kStages], (oldest / kStages) & 1);
     ++oldest;
-    return ok;
   }
 
-  // Space for `bytes` (a multiple of 16) in the ring, in stage order.
+  // Space for `bytes` (a multiple of 16) in the ring, in order, and the stage's slot.
   __device__ __forceinline__ uint32_t reserve(uint32_t bytes) {
     if (st - oldest == kStages) pop();
+    // the description is still read with the V half
+    if (half == 0 && st >= kStages) ok = ok && mbar_wait(&sh.empty[1][st % kStages], (st / kStages - 1) & 1);
     uint32_t at = head;
-    if (head + bytes > C::kRing) {
-      at = 0;
-      while (oldest != st && ok) {
-        const uint32_t o = sh.offset[oldest % kStages];
-        if (!(o >= head || o < bytes)) break;
-        pop();
-      }
-    } else {
-      while (oldest != st && ok) {
-        const uint32_t o = sh.offset[oldest % kStages];
-        if (!(o >= at && o < at + bytes)) break;
-        pop();
-      }
+    const bool wrap = head + bytes > C::kRing;
+    if (wrap) at = 0;
+    while (oldest != st && ok) {
+      const uint32_t o = sh.offset[half][oldest % kStages];
+      if (wrap ? !(o >= head || o < bytes) : !(o >= at && o < at + bytes)) break;
+      pop();
     }
     if (oldest == st) at = 0;  // empty: start over
     head = at + bytes;
     return at;
   }
 
-  // One stage: lanes < tiles hold a tile each (payload, its descriptor fields and tokens [t0, t0 + n)).
-  __device__ __forceinline__ void emit(uint32_t tiles, uint32_t flags, uint32_t seq, uint32_t head0, uint32_t heads, uint32_t slot,
-                                       const uint8_t* payload, uint32_t f, uint32_t mode, uint32_t sref, uint32_t t0, uint32_t n,
-                                       uint32_t pos) {
-    const bool mine = lane < tiles;
-    const bool packed = heads == p.H;  // all heads of a token: a tile is one piece of the slot
-    const uint32_t rb = f == dev::kFp16 ? kD * 2 : f == dev::kInt4 ? kD / 2 : kD, pb = f == dev::kInt4 ? 8 : 4;
-    const bool params = mine && f != dev::kFp16 && mode == 0;
-    const uint32_t codes = mine ? n * heads * rb : 0u;
-    uint64_t ka = 0, va = 0;  // byte addresses of the first row's parameters
-    uint32_t kn = 0, vn = 0;  // bytes copied of them
+  // A tile per lane: tokens [t0, t0 + n) of a block at `payload`.
+  struct Source {
+    const uint8_t* payload;
+    uint32_t f, mode, sref, t0, n, pos;
+  };
+  struct Piece {
+    uint32_t seq, head0, heads, slot, direct, single;
+    int32_t pos0;  // of the first new token
+    uint32_t q;    // new tokens
+  };
+
+  // Stages of up to `per` (a power of two) tiles each, from lanes < count; none: one stage without tiles.
+  __device__ __forceinline__ void emit(const Source& x, uint32_t count, uint32_t per, const Piece& pc, uint32_t flags) {
+    const bool packed = pc.heads == p.H;  // all heads of a token: a tile's codes are one piece of the slot
+    const uint32_t rb = x.f == dev::kFp16 ? kD * 2 : x.f == dev::kInt4 ? kD / 2 : kD, pb = x.f == dev::kInt4 ? 8 : 4;
+    const bool live = lane < count, params = live && x.f != dev::kFp16 && x.mode == 0;
+    const uint32_t codes = live ? x.n * pc.heads * rb : 0u;
+    const uint32_t row0 = half ? p.T + x.t0 : x.t0;
+    const uint8_t* src = x.payload + (uint64_t{row0} * p.H + pc.head0) * rb;
+    // The parameters of all heads of the tile's tokens, rounded out to 16 bytes (the slot's end is).
+    uint64_t pa = 0;
+    uint32_t pn = 0;
     if (params) {
-      ka = p.code_bytes[f] + uint64_t{t0 * p.H + head0} * pb;
-      va = ka + uint64_t{p.T} * p.H * pb;
-      if (packed) {
-        const uint32_t len = n * p.H * pb;
-        kn = static_cast<uint32_t>(((ka + len + 15) & ~uint64_t{15}) - (ka & ~uint64_t{15}));
-        vn = static_cast<uint32_t>(((va + len + 15) & ~uint64_t{15}) - (va & ~uint64_t{15}));
-      }
+      pa = p.code_bytes[x.f] + uint64_t{row0} * p.H * pb;
+      pn = static_cast<uint32_t>(((pa + x.n * p.H * pb + 15) & ~uint64_t{15}) - (pa & ~uint64_t{15}));
     }
-    const uint32_t bytes = 2 * codes + kn + vn;
-    uint32_t off = bytes;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, off, o);
-      if (lane >= static_cast<uint32_t>(o)) off += x;
+    const uint8_t* psrc = x.payload + (pa & ~uint64_t{15});
+    const uint32_t bytes = codes + pn, in_stage = lane & (per - 1);
+    uint32_t upto = bytes;  // of the stage's tiles up to this one
+    for (uint32_t o = 1; o < per; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (in_stage >= o) upto += y;
     }
-    const uint32_t total = __shfl_sync(0xFFFFFFFFu, off, 7);  // lanes from `tiles` on add nothing
-    off -= bytes;
-    const uint32_t at = reserve(total);
-    const uint32_t slot_i = st % kStages;
-    Stage& m = stages[slot_i];
-    off += at;
-    if (mine) {
-      Tile t;
-      t.fn = f | n << 8 | mode << 16 | (params && !packed ? 1u << 24 : 0u);
-      t.pos = pos;
-      t.kc = off;
-      t.vc = off + codes;
-      if (packed) {
-        t.kp = off + 2 * codes + static_cast<uint32_t>(ka & 15);
-        t.vp = off + 2 * codes + kn + static_cast<uint32_t>(va & 15);
-      } else {
-        const uint64_t a = reinterpret_cast<uint64_t>(payload) + ka;
-        t.kp = static_cast<uint32_t>(a);
-        t.vp = static_cast<uint32_t>(a >> 32);
-      }
-      const float2 w = mode != 0 ? dev::block_params_value(mode, sref) : make_float2(1.0f, 0.0f);
-      t.ws = w.x;
-      t.wb = w.y;
-      m.tile[lane] = t;
-    }
-    if (lane == 0) {
-      m.tiles = tiles;
-      m.flags = flags;
-      m.seq = seq;
-      m.head0 = head0;
-      m.heads = heads;
-      m.unit_slot = slot;
-      sh.offset[slot_i] = at;
-    }
-    __syncwarp();
-    ++st;
-    if (!ok) return;  // gave up: nothing more is copied, and the consumers give up as well
-    uint64_t* bar = &sh.full[slot_i];
-    if (lane == 0) mbar_arrive_expect(bar, total);
-    __syncwarp();
-    if (packed) {
-      if (mine) {
-        const uint64_t row = uint64_t{t0} * heads * rb;
-        bulk_load(ring + off, payload + row, codes, bar);
-        bulk_load(ring + off + codes, payload + uint64_t{p.T} * heads * rb + row, codes, bar);
-        if (kn) bulk_load(ring + off + 2 * codes, payload + (ka & ~uint64_t{15}), kn, bar);
-        if (vn) bulk_load(ring + off + 2 * codes + kn, payload + (va & ~uint64_t{15}), vn, bar);
-      }
-    } else {
-      for (uint32_t t = 0; t < tiles; ++t) {  // a copy per token and kind: its heads lie together
-        const uint64_t base = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(payload), t);
-        const uint32_t nt = __shfl_sync(0xFFFFFFFFu, n, t), tt = __shfl_sync(0xFFFFFFFFu, t0, t);
-        const uint32_t r = __shfl_sync(0xFFFFFFFFu, rb, t), o = __shfl_sync(0xFFFFFFFFu, off, t);
-        const uint32_t i = lane & 15, kv = lane >> 4;
-        if (i < nt) {
-          bulk_load(ring + o + (kv * nt + i) * heads * r,
-                    reinterpret_cast<const uint8_t*>(base) + (uint64_t{kv * p.T + tt + i} * p.H + head0) * r, heads * r, bar);
+    const float2 w = x.mode != 0 ? dev::block_params_value(x.mode, x.sref) : make_float2(1.0f, 0.0f);
+    // Whether every row sees all the tile's tokens.
+    const int32_t first = static_cast<int32_t>(x.pos), end = first + static_cast<int32_t>(x.n);
+    const bool whole = end <= pc.pos0 + 1 &&
+                       (p.window == 0 || static_cast<uint32_t>(pc.pos0 + static_cast<int32_t>(pc.q) - 1 - first) < p.window ||
+                        x.pos + x.n <= p.sinks);
+    const uint32_t hidden = __ballot_sync(0xFFFFFFFFu, live && !whole), part = __ballot_sync(0xFFFFFFFFu, live && x.n < 16);
+    const uint32_t f0 = __shfl_sync(0xFFFFFFFFu, x.f, lane & ~(per - 1));
+    const uint32_t other = __ballot_sync(0xFFFFFFFFu, live && x.f != f0);
+    const uint32_t n_st = count == 0 ? 1u : (count + per - 1) / per;
+    for (uint32_t k = 0; k < n_st; ++k) {
+      const uint32_t tiles = min(per, count - k * per);  // 0 of 0
+      const uint32_t total = __shfl_sync(0xFFFFFFFFu, upto, k * per + (tiles ? tiles - 1 : 0u));
+      const uint32_t at = reserve(total);
+      if (!ok) return;  // gave up: nothing more is copied, and the consumers give up as well
+      const uint32_t slot_i = st % kStages;
+      const bool mine = live && lane / per == k;
+      const uint32_t off = at + upto - bytes;
+      Stage& m = stages[slot_i];
+      uint64_t* bar = &sh.full[half][slot_i];
+      if (half == 0) {
+        const uint32_t lanes = ((1u << per) - 1u) << (k * per);
+        const bool pairs = per > pc.single && tiles == per && ((hidden | part | other) & lanes) == 0;
+        const uint32_t fl = pc.direct | flags | (flags & kFirstStages && st - first_st < C::kGroups ? kFirst : 0u);
+        if (lane == 0) {
+          *reinterpret_cast<uint4*>(&m.tiles) = make_uint4(tiles, fl, pc.seq, pc.head0);
+          *reinterpret_cast<uint4*>(&m.heads) = make_uint4(pc.heads, pc.slot, pairs, 0u);
         }
       }
+      if (lane == 0) sh.offset[half][slot_i] = at;
+      if (mine) {
+        Tile& d = m.tile[in_stage];
+        const uint32_t where = smem_addr(&d);
+        const uint32_t po = pn ? ring_at + off + codes + static_cast<uint32_t>(pa & 15) + pc.head0 * pb : where + 32;
+        if (half == 0) {
+          *reinterpret_cast<uint4*>(&d) = make_uint4(x.f | x.n << 8 | (whole ? 1u << 16 : 0u), x.pos, ring_at + off, po);
+          *reinterpret_cast<uint2*>(&d.row_step) = pn ? make_uint2(pb, p.H * pb) : make_uint2(0u, 0u);
+          *reinterpret_cast<float2*>(&d.ws) = w;
+        } else {
+          *reinterpret_cast<uint2*>(&d.vc) = make_uint2(ring_at + off, po);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect(bar, total);
+      __syncwarp();
+      if (mine) {
+        if (packed) bulk_load(ring + off, src, codes, bar);
+        if (pn) bulk_load(ring + off + codes, psrc, pn, bar);
+      }
+      if (!packed) {
+        for (uint32_t i = 0; i < tiles; ++i) {  // a copy per token: its heads lie together
+          const uint32_t from = k * per + i;
+          const uint64_t base = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(src), from);
+          const uint32_t nt = __shfl_sync(0xFFFFFFFFu, x.n, from), r = __shfl_sync(0xFFFFFFFFu, rb, from);
+          const uint32_t o = __shfl_sync(0xFFFFFFFFu, off, from);
+          if (lane < nt) {
+            bulk_load(ring + o + lane * pc.heads * r, reinterpret_cast<const uint8_t*>(base) + uint64_t{lane} * p.H * r, pc.heads * r,
+                      bar);
+          }
+        }
+      }
+      ++st;
     }
   }
+  uint32_t first_st = 0;  // of the piece
 
   // First k in [0, count) with cost[k] >= target (count if none).
   __device__ __forceinline__ uint32_t find(const uint32_t* cost, uint32_t count, uint32_t target) {
@@ -595,7 +869,7 @@ struct Producer {
       const uint32_t last = min(k + step, b) - 1;  // lanes past the end repeat the last
       const bool hit = k < b ? __ldg(cost + last) >= target : true;
       const uint32_t first = __ffs(__ballot_sync(0xFFFFFFFFu, hit));
-      if (first == 0) return b;  // no lane: b - a <= 32 step, all below
+      if (first == 0) return b;  // no lane: b - a == 32 step, all below
       const uint32_t lo = a + (first - 1) * step;
       if (lo >= b) return b;
       b = min(lo + step, b);
@@ -621,26 +895,28 @@ struct Producer {
         if (ub >= x1) break;
         const uint32_t lo = x0 > ub ? static_cast<uint32_t>(x0 - ub) : 0u;
         const uint32_t hi = x1 - ub < w ? static_cast<uint32_t>(x1 - ub) : w;
-        piece(i, hg, lo, hi, w, first, count);
+        piece(i, hg, lo, hi, w, first, count, rows.q);
       }
       base += uint64_t{p.head_groups} * w;
     }
-    for (int k = 0; k < C::kGroups && ok; ++k) emit(0, kDone, 0, 0, p.H, 0, nullptr, 0, 0, 0, 0, 0, 0);
+    const Source none{nullptr, 0, 0, 0, 0, 0, 0};
+    const Piece end{0, 0, p.H, 0, 0, 1, 0, 0};
+    for (int k = 0; k < C::kGroups && ok; ++k) emit(none, 0, 1, end, kDone);
   }
 
   // The blocks of unit (i, hg) whose cost begins in [lo, hi).
   __device__ __forceinline__ void piece(uint32_t i, uint32_t hg, uint32_t lo, uint32_t hi, uint32_t w, uint32_t first,
-                                        uint32_t count) {
-    const uint32_t head0 = hg * 8, heads = min(8u, p.H - head0), per_stage = kTiles / heads;
-    const uint32_t slot = blockIdx.x + i * p.head_groups + hg;
-    const uint32_t direct = lo == 0 && hi == w ? kDirect : 0u;
+                                        uint32_t count, uint32_t q) {
+    const uint32_t head0 = hg * 8, heads = min(8u, p.H - head0);
+    const uint32_t single = heads > 4 ? 1u : heads > 2 ? 2u : heads > 1 ? 4u : 8u;  // tiles that occupy a group's warps
+    const Piece pc{i,  head0, heads, blockIdx.x + i * p.head_groups + hg, lo == 0 && hi == w ? kDirect : 0u, single,
+                   static_cast<int32_t>(p.context[i] - q), q};
     const uint32_t* cost = p.block_cost + first;
     uint32_t j0 = lo == 0 ? 0u : find(cost, count, lo) + 1;
     // Stages alternate between the consumer groups.  The first stage of each carries kFirst; at the end
     // every group gets a stage without tiles that carries kLast, after as many empty ones as bring the
     // piece to a multiple of kGroups.
-    const uint32_t flags = kFirst | direct;
-    uint32_t done = 0;
+    first_st = st;
     bool more = true;
     while (more && ok) {
       const uint32_t j = j0 + lane;
@@ -650,54 +926,57 @@ struct Producer {
       bool inside = false;
       if (j < count) {
         const uint32_t start = j > 0 ? __ldg(cost + j - 1) : 0u;
+        b = __ldg(p.blocks + first + j);
         inside = start < hi;
         if (inside) {
-          b = __ldg(p.blocks + first + j);
           f = open_block(p, b, &payload);
           if (f <= 3) v = min((b.y >> 10) & 0x3FFu, p.T);
         }
       }
       more = __all_sync(0xFFFFFFFFu, inside);  // else the piece ends in this batch
-      uint32_t nt = (v + 15) / 16, upto = nt;
+      const uint32_t nt = (v + 15) / 16;
+      // Two tiles of one format share a softmax step, but for FP16: its halves would fill too much of the ring.
+      const uint32_t some = __ballot_sync(0xFFFFFFFFu, nt > 0), f_some = __shfl_sync(0xFFFFFFFFu, f, __ffs(some | 1u << 31) - 1);
+      const uint32_t per = f_some == dev::kFp16 || __any_sync(0xFFFFFFFFu, nt > 0 && f != f_some) ? single : 2 * single;
+      const uint32_t mode = f == dev::kFp16 ? 0u : (b.y >> 4) & 3u;
+      if (__all_sync(0xFFFFFFFFu, inside && nt == 1)) {
+        emit(Source{payload, f, mode, b.z, 0u, v, b.w}, 32, per, pc, kFirstStages);
+      } else {
+        uint32_t upto = nt;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= static_cast<uint32_t>(o)) upto += x;
-      }
-      const uint32_t total = __shfl_sync(0xFFFFFFFFu, upto, 31);
-      const uint32_t ps = static_cast<uint32_t>(reinterpret_cast<uint64_t>(payload)),
-                     pt = static_cast<uint32_t>(reinterpret_cast<uint64_t>(payload) >> 32);
-      for (uint32_t t = 0; t < total && ok; t += per_stage) {
-        // lane k of the stage: tile t + k, in the first block whose running count passes it
-        const uint32_t k = t + lane;
-        const uint32_t tiles = min(per_stage, total - t);
-        uint32_t at = 0;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const uint32_t x = __shfl_sync(0xFFFFFFFFu, upto, at + o - 1);
-          if (x <= k) at += o;
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+          if (lane >= static_cast<uint32_t>(o)) upto += x;
         }
-        at = min(at, 31u);
-        const uint32_t before = __shfl_sync(0xFFFFFFFFu, upto - nt, at);
-        const uint32_t tf = __shfl_sync(0xFFFFFFFFu, f, at), tv = __shfl_sync(0xFFFFFFFFu, v, at);
-        const uint32_t ti = __shfl_sync(0xFFFFFFFFu, b.y, at), tr = __shfl_sync(0xFFFFFFFFu, b.z, at);
-        const uint32_t tw = __shfl_sync(0xFFFFFFFFu, b.w, at);
-        const uint64_t pl = __shfl_sync(0xFFFFFFFFu, ps, at) | uint64_t{__shfl_sync(0xFFFFFFFFu, pt, at)} << 32;
-        const uint32_t t0 = lane < tiles ? (k - before) * 16 : 0u;
-        const uint32_t n = lane < tiles ? min(16u, tv - t0) : 0u;
-        emit(tiles, done < C::kGroups ? flags : direct, i, head0, heads, slot, reinterpret_cast<const uint8_t*>(pl), tf, tf == dev::kFp16 ? 0u : (ti >> 4) & 3u, tr,
-             t0, n, tw + t0);
-        ++done;
+        const uint32_t total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        for (uint32_t t = 0; t < total && ok; t += 32) {
+          // this lane: tile t + lane, in the first block whose running count passes it
+          const uint32_t k = t + lane;
+          uint32_t at = 0;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const uint32_t x = __shfl_sync(0xFFFFFFFFu, upto, at + o - 1);
+            if (x <= k) at += o;
+          }
+          at = min(at, 31u);
+          Source x;
+          x.payload = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(payload), at));
+          x.f = __shfl_sync(0xFFFFFFFFu, f, at);
+          x.mode = __shfl_sync(0xFFFFFFFFu, mode, at);
+          x.sref = __shfl_sync(0xFFFFFFFFu, b.z, at);
+          const uint32_t before = __shfl_sync(0xFFFFFFFFu, upto - nt, at), tv = __shfl_sync(0xFFFFFFFFu, v, at);
+          const uint32_t start = __shfl_sync(0xFFFFFFFFu, b.w, at);
+          x.t0 = k < total ? (k - before) * 16 : 0u;
+          x.n = k < total ? min(16u, tv - x.t0) : 0u;
+          x.pos = start + x.t0;
+          emit(x, min(32u, total - t), per, pc, kFirstStages);
+        }
       }
       j0 += 32;
     }
-    // Closing stages, one per group, without tiles.
-    const uint32_t fill = (C::kGroups - done % C::kGroups) % C::kGroups + C::kGroups;
-    for (uint32_t k = 0; k < fill && ok; ++k) {
-      const uint32_t fl = (done < C::kGroups ? flags : direct) | (k + C::kGroups >= fill ? kLast : 0u);
-      emit(0, fl, i, head0, heads, slot, nullptr, 0, 0, 0, 0, 0, 0);
-      ++done;
-    }
+    const Source none{nullptr, 0, 0, 0, 0, 0, 0};
+    const uint32_t done = st - first_st, fill = (C::kGroups - done % C::kGroups) % C::kGroups + C::kGroups;
+    for (uint32_t k = 0; k < fill && ok; ++k) emit(none, 0, 1, pc, kFirstStages | (k + C::kGroups >= fill ? kLast : 0u));
   }
 };
 
@@ -706,15 +985,17 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
   using C = Config<kD, kNB>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
-  float* merge = reinterpret_cast<float*>(smem + C::kRing);
-  Stage* stages = reinterpret_cast<Stage*>(smem + C::kRing + C::kMergeBytes);
+  float* merge = reinterpret_cast<float*>(smem + 2 * C::kRing);
+  Stage* stages = reinterpret_cast<Stage*>(smem + 2 * C::kRing + C::kMergeBytes);
   __shared__ Shared sh;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kStages; ++i) {
-      mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 8);
+      for (int half = 0; half < 2; ++half) {
+        mbar_init(&sh.full[half][i], 1);
+        mbar_init(&sh.empty[half][i], 8);
+      }
     }
     mbar_init(&sh.merged, C::kWarps);
     mbar_fence_init();
@@ -742,7 +1023,7 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
     }
     __syncthreads();
     uint64_t total = 0;
-    for (uint32_t w = 0; w <= C::kWarps; ++w) {
+    for (uint32_t w = 0; w < C::kThreads / 32; ++w) {
       if (w < warp) upto += sh.warp_sum[w];
       total += sh.warp_sum[w];
     }
@@ -766,19 +1047,23 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
     __syncthreads();
   }
 
-  if (warp == C::kWarps) {
-    Producer<kD, kNB> producer{p, sh, stages, ring, lane};
+  // Registers: 96 (or 168) a thread at launch; the producers' warpgroup hands most of its own over.
+  if (warp >= C::kWarps) {
+    if constexpr (kNB == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const uint32_t half = warp - C::kWarps;
+    if (half > 1) return;
+    Producer<kD, kNB> producer{p, sh, stages, ring + half * C::kRing, smem_addr(ring) + half * C::kRing, half, lane};
     producer.run();
     if (!producer.ok && lane == 0) atomicOr(p.err, dev::kErrInternal);
     return;
   }
 
   // ---- consumers
+  if constexpr (kNB == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
   const uint32_t group = warp / 8, w8 = warp % 8;
+  const uint32_t wr_at = smem_addr(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp * static_cast<uint32_t>(sizeof(WarpRows<kD, kNB>));
+  const uint32_t stages_at = smem_addr(stages);
   State<kD, kNB> s;
-  uint32_t heads = 1, tile_i = 0, head_i = 0, head0 = 0, slot = 0;
-  int32_t pos0 = 0;
-  Rows rows{0, 0};
   uint32_t meets = 0;
   // All consumer warps, with a limit as every wait.
   auto meet = [&]() {
@@ -787,122 +1072,147 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
     return mbar_wait(&sh.merged, meets++ & 1);
   };
   for (uint32_t st = group;; st += C::kGroups) {
-    const uint32_t si = st % kStages;
-    if (!mbar_wait(&sh.full[si], (st / kStages) & 1)) {
+    const uint32_t si = st % kStages, parity = (st / kStages) & 1;
+    if (!mbar_wait(&sh.full[0][si], parity)) {
       if (lane == 0) atomicOr(p.err, dev::kErrInternal);
       break;
     }
-    const Stage& m = stages[si];
-    const uint32_t flags = m.flags;
-    if (flags & kDone) break;
-    if (flags & kFirst) {
-      heads = m.heads;
-      head0 = m.head0;
-      slot = m.unit_slot;
-      tile_i = w8 / heads;
-      head_i = w8 % heads;
-      rows = rows_of(p, m.seq);
-      const uint32_t context = p.context[m.seq];
-      pos0 = static_cast<int32_t>(context - rows.q);
-      begin_piece<kD, kNB>(p, s, rows, context, head0 + head_i, lane);
+    const uint32_t m = stages_at + si * static_cast<uint32_t>(sizeof(Stage));  // address of its description
+    constexpr uint32_t kHead = offsetof(Stage, tiles), kHead2 = offsetof(Stage, heads);
+    if (lds32(m + kHead + 4) & kDone) break;
+    if (lds32(m + kHead + 4) & kFirst) {
+      WarpRows<kD, kNB>* wr = reinterpret_cast<WarpRows<kD, kNB>*>(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp;
+      const uint32_t heads = lds32(m + kHead2), seq = lds32(m + kHead + 8), head0 = lds32(m + kHead + 12);
+      const uint32_t single = heads > 4 ? 1u : heads > 2 ? 2u : heads > 1 ? 4u : 8u;
+      // a group's warps beyond `single` x heads have no tile
+      if (lane == 0) wr->place = make_uint4(heads, w8 % heads, w8 / heads < single ? w8 / heads : 1u << 16, single);
+      begin_piece<kD, kNB>(p, s, wr, rows_of(p, seq), p.context[seq], head0 + w8 % heads, lane);
     }
-    if (tile_i < m.tiles) {
-      const Tile& t = m.tile[tile_i];
-      const uint32_t fn = t.fn, f = fn & 0xFFu, n = (fn >> 8) & 0xFFu, mode = (fn >> 16) & 0xFFu, tile_pos = t.pos;
-      const uint32_t rb = f == dev::kFp16 ? kD * 2 : f == dev::kInt4 ? kD / 2 : kD;
-      const uint32_t token_bytes = heads * rb;
-      const uint8_t* kc = ring + t.kc + head_i * rb;
-      const uint8_t* vc = ring + t.vc + head_i * rb;
-      float2 kp[2], vp[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t tok = (lane >> 2) + 8 * h;
-        kp[h] = vp[h] = make_float2(t.ws, t.wb);
-        if (f != dev::kFp16 && mode == 0 && tok < n) {
-          if (fn >> 24) {
-            const uint8_t* a = reinterpret_cast<const uint8_t*>(uint64_t{t.kp} | uint64_t{t.vp} << 32);
-            const uint64_t row = uint64_t{tok} * p.H + head_i, up = uint64_t{p.T} * p.H;
-            if (f == dev::kInt4) {
-              kp[h] = __ldg(reinterpret_cast<const float2*>(a) + row);
-              vp[h] = __ldg(reinterpret_cast<const float2*>(a) + row + up);
-            } else {
-              kp[h] = make_float2(__ldg(reinterpret_cast<const float*>(a) + row), 0.0f);
-              vp[h] = make_float2(__ldg(reinterpret_cast<const float*>(a) + row + up), 0.0f);
-            }
-          } else {
-            const uint32_t row = tok * heads + head_i;
-            if (f == dev::kInt4) {
-              kp[h] = reinterpret_cast<const float2*>(ring + t.kp)[row];
-              vp[h] = reinterpret_cast<const float2*>(ring + t.vp)[row];
-            } else {
-              kp[h] = make_float2(reinterpret_cast<const float*>(ring + t.kp)[row], 0.0f);
-              vp[h] = make_float2(reinterpret_cast<const float*>(ring + t.vp)[row], 0.0f);
-            }
+    const uint4 place = lds128(wr_at + static_cast<uint32_t>(sizeof(WarpRows<kD, kNB>)) - 16);
+    const Place at{wr_at, place.x, place.y, lane};
+    const uint32_t tile_i = place.z, single = place.w;
+    // This warp's tiles of the stage: tile_i, and every `single`-th behind it.
+    const uint32_t n_tiles = lds32(m + kHead);
+    uint64_t *empty_k = &sh.empty[0][si], *full_v = &sh.full[1][si];
+    bool ok = true;
+    if (tile_i < n_tiles && lds32(m + kHead2 + 8) != 0) {
+      const uint32_t t0 = m + tile_i * static_cast<uint32_t>(sizeof(Tile)), two[2] = {t0, t0 + single * static_cast<uint32_t>(sizeof(Tile))};
+      const uint32_t n[2] = {16, 16};
+      switch (lds32(t0) & 0xFFu) {
+        case dev::kE4M3: ok = step<kD, kNB, dev::kE4M3, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
+        case dev::kE5M2: ok = step<kD, kNB, dev::kE5M2, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
+        default: ok = step<kD, kNB, dev::kInt4, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
+      }
+    } else {
+      uint64_t* give = nullptr;  // the K half's barrier with the last tile's scores, null once it is given back
+#pragma unroll 1
+      for (uint32_t i = tile_i; i < n_tiles && ok; i += single) {
+        const uint32_t one[1] = {m + i * static_cast<uint32_t>(sizeof(Tile))};
+        const uint32_t fn = lds32(one[0]), n[1] = {(fn >> 8) & 0xFFu};
+        give = i + single < n_tiles || !(fn >> 16) ? nullptr : empty_k;
+        if (fn >> 16) {
+          switch (fn & 0xFFFFu) {
+            case dev::kFp16 | 16 << 8: ok = step<kD, kNB, dev::kFp16, 1, false>(p, s, one, n, at, give, full_v, parity); break;
+            case dev::kE4M3 | 16 << 8: ok = step<kD, kNB, dev::kE4M3, 1, false>(p, s, one, n, at, give, full_v, parity); break;
+            case dev::kInt4 | 16 << 8: ok = step<kD, kNB, dev::kInt4, 1, false>(p, s, one, n, at, give, full_v, parity); break;
+            default:
+              switch (fn & 0xFFu) {
+                case dev::kFp16: ok = step<kD, kNB, dev::kFp16, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+                case dev::kE4M3: ok = step<kD, kNB, dev::kE4M3, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+                case dev::kE5M2: ok = step<kD, kNB, dev::kE5M2, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+                default: ok = step<kD, kNB, dev::kInt4, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+              }
           }
+        } else {
+          ok = mbar_wait(full_v, parity);
+          State<kD, kNB> copy = s;
+          if (ok) edge_tile<kD, kNB>(p, &copy, one[0], at);
+          s = copy;
         }
       }
-      const int32_t tp = static_cast<int32_t>(tile_pos), last = pos0 + static_cast<int32_t>(rows.q) - 1;
-      const bool whole = tp + static_cast<int32_t>(n) - 1 <= pos0 &&
-                         (p.window == 0 || static_cast<uint32_t>(last - tp) < p.window || tile_pos + n <= p.sinks);
-      switch (f) {
-        case dev::kFp16: tile_step<kD, kNB, dev::kFp16>(p, s, kc, vc, token_bytes, kp, vp, n, tile_pos, whole, lane); break;
-        case dev::kE4M3: tile_step<kD, kNB, dev::kE4M3>(p, s, kc, vc, token_bytes, kp, vp, n, tile_pos, whole, lane); break;
-        case dev::kE5M2: tile_step<kD, kNB, dev::kE5M2>(p, s, kc, vc, token_bytes, kp, vp, n, tile_pos, whole, lane); break;
-        default: tile_step<kD, kNB, dev::kInt4>(p, s, kc, vc, token_bytes, kp, vp, n, tile_pos, whole, lane); break;
+      if (tile_i >= n_tiles) ok = mbar_wait(full_v, parity);
+      if (give == nullptr) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty_k);
       }
     }
+    if (!ok) {
+      if (lane == 0) atomicOr(p.err, dev::kErrInternal);
+      break;
+    }
+    const uint4 head = lds128(m + kHead);  // tiles, flags, seq, head0
+    const uint32_t slot = lds32(m + kHead2 + 4), flags = head.y;
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.empty[si]);
+    if (lane == 0) mbar_arrive(&sh.empty[1][si]);
 
     if (flags & kLast) {
-      // ---- merge the warps of each head: outputs, max and sum of every row
+      // ---- merge the warps of each head: outputs, max and sum of every row.  The second group leaves its
+      // state in the buffer, the first joins it to its own warp by warp and leaves the sum there.
       const uint32_t g = lane >> 2, quad = lane & 3;
       const float unit = s.E == kNoExponent ? 0.0f : exp2f(static_cast<float>(s.E));
+      float* mine = merge + w8 * 8 * kNB * C::kRowsPad;
+      bool met = true;
+#pragma unroll 1
+      for (int gr = C::kGroups - 1; gr >= 0; --gr) {
+        if (static_cast<int>(group) == gr) {
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) {
+          for (int nb = 0; nb < kNB; ++nb) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float l = s.l[nb][c], b = s.bias[nb][c];
+            for (int c = 0; c < 2; ++c) {
+              float l = s.l[nb][c], b = s.bias[nb][c], m_own = s.m[nb][c], fo = 1.0f, ft = 0.0f;
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-            b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+              for (int o = 4; o < 32; o <<= 1) {
+                l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+                b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+              }
+              float* row = mine + (nb * 8 + quad * 2 + c) * C::kRowsPad;
+              if (gr + 1 < C::kGroups) {
+                const float2 ml = *reinterpret_cast<const float2*>(row + kD);
+                const float M = fmaxf(m_own, ml.x);
+                fo = M == -INFINITY ? 1.0f : exp2f(m_own - M);
+                ft = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
+                l = fmaf(l, fo, ml.y * ft);
+                m_own = M;
+              }
+#pragma unroll
+              for (int mt = 0; mt < kD / 16; ++mt) {
+                float2* at2 = reinterpret_cast<float2*>(row + g * (kD / 8) + 2 * mt);
+                float2 x = make_float2(fmaf(s.acc[nb][mt][c], unit, b), fmaf(s.acc[nb][mt][2 + c], unit, b));
+                if (gr + 1 < C::kGroups) {
+                  const float2 y = *at2;
+                  x = make_float2(fmaf(x.x, fo, y.x * ft), fmaf(x.y, fo, y.y * ft));
+                }
+                *at2 = x;
+              }
+              __syncwarp();  // every lane has read the other group's max and sum
+              if (g == 0) *reinterpret_cast<float2*>(row + kD) = make_float2(m_own, l);
+            }
           }
-          float* row = merge + (warp * 8 * kNB + nb * 8 + quad * 2 + c) * C::kRowsPad;
-#pragma unroll
-          for (int mt = 0; mt < kD / 16; ++mt) {
-            *reinterpret_cast<float2*>(row + g * (kD / 8) + 2 * mt) =
-                make_float2(fmaf(s.acc[nb][mt][c], unit, b), fmaf(s.acc[nb][mt][2 + c], unit, b));
-          }
-          if (g == 0) *reinterpret_cast<float2*>(row + kD) = make_float2(s.m[nb][c], l);
         }
+        met = met && meet();
       }
-      if (!meet()) {
+      if (!met) {
         if (lane == 0) atomicOr(p.err, dev::kErrInternal);
         break;
       }
-      const uint32_t n_rows = rows.q * p.group, n_tiles = kTiles / heads;
+      const uint32_t head0 = head.w;
+      const Rows rows = rows_of(p, head.z);
+      const uint32_t heads = at.heads, n_rows = rows.q * p.group, n_warps = single;
       for (uint32_t i = threadIdx.x; i < heads * n_rows * (kD / 4); i += C::kWarps * 32) {
         const uint32_t e = i % (kD / 4), r = (i / (kD / 4)) % n_rows, h = i / (kD / 4) / n_rows;
         float M = -INFINITY, L = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int gr = 0; gr < C::kGroups; ++gr) {
-          for (uint32_t t = 0; t < n_tiles; ++t) {
-            M = fmaxf(M, merge[((gr * 8 + t * heads + h) * 8 * kNB + r) * C::kRowsPad + kD]);
-          }
-        }
-        for (int gr = 0; gr < C::kGroups; ++gr) {
-          for (uint32_t t = 0; t < n_tiles; ++t) {
-            const float* row = merge + ((gr * 8 + t * heads + h) * 8 * kNB + r) * C::kRowsPad;
-            const float2 ml = *reinterpret_cast<const float2*>(row + kD);
-            const float a = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
-            const float4 x = *reinterpret_cast<const float4*>(row + 4 * e);
-            L = fmaf(ml.y, a, L);
-            o.x = fmaf(x.x, a, o.x);
-            o.y = fmaf(x.y, a, o.y);
-            o.z = fmaf(x.z, a, o.z);
-            o.w = fmaf(x.w, a, o.w);
-          }
+        for (uint32_t t = 0; t < n_warps; ++t) M = fmaxf(M, merge[((t * heads + h) * 8 * kNB + r) * C::kRowsPad + kD]);
+        for (uint32_t t = 0; t < n_warps; ++t) {
+          const float* row = merge + ((t * heads + h) * 8 * kNB + r) * C::kRowsPad;
+          const float2 ml = *reinterpret_cast<const float2*>(row + kD);
+          const float a = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
+          const float4 x = *reinterpret_cast<const float4*>(row + 4 * e);
+          L = fmaf(ml.y, a, L);
+          o.x = fmaf(x.x, a, o.x);
+          o.y = fmaf(x.y, a, o.y);
+          o.z = fmaf(x.z, a, o.z);
+          o.w = fmaf(x.w, a, o.w);
         }
         if (flags & kDirect) {
           if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros

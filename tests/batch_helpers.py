@@ -106,7 +106,7 @@ def plan_oracle(segs, qlens, arena, table, T, layout_id, block_cap, token_cap, m
                 row = tfirst + max(0, q - ctx) + t - from_
                 targets[row] = (r[4], t - r[3])
                 positions[row] = t
-        cost = [(r[5] + 15) // 16 * (14, 7, 7, 4)[r[1] & 15] for r in keep]
+        cost = [(r[5] + 15) // 16 * (14, 7, 7, 7)[r[1] & 15] for r in keep]
         seqs.append({"context": ctx, "q": q, "blocks": [r[:4] for r in keep], "cost": np.cumsum(cost).tolist()})
         bfirst, tfirst = bfirst + n, tfirst + q
     tf.append(min(tfirst, token_cap))
