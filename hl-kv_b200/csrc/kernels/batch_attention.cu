@@ -170,7 +170,7 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
     p.pool[f] = DevPool{static_cast<const uint8_t*>(q.base), q.slot_bytes, q.num_slots};
   }
   const uint64_t rows = uint64_t{plan->token_cap} * q_heads;
-  if (rows > 0x7FFFFFFFull || uint64_t{plan->nseq} * H > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
+  if (rows > 0x7FFFFFFFull || uint64_t{plan->nseq} * H * kStreamRows > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
   p.block_first = plan->d_block_first;
   p.block_count = plan->d_block_count;
   p.token_first = plan->d_token_first;

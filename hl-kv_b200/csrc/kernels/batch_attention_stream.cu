@@ -49,20 +49,42 @@ struct alignas(16) Stage {
   uint32_t pairs;  // two tiles a warp, of one format, 16 tokens each and seen whole
 };
 
-template <int kD, int kNB>
+// What the producers prepare for 32 tiles before they hand them out stage by stage.
+struct alignas(16) Job {
+  uint64_t src, psrc;              // codes and parameters of the tile's half
+  uint32_t codes, pn, upto, delta;  // bytes of each, of the jobs up to this one, from the parameters' copy to the first one
+  uint32_t fn, pos, row_step, token_step;
+  float ws, wb;
+  uint32_t unused[2];
+};
+
+constexpr int kWarps = 16;                   // consumers, two groups of 8
+// And four more, of which two produce and two end at once: with 18 warps a block the same code measured 5 to 10 %
+// slower (decode of 64 x 8192 tokens 232 us against 220 us).
+constexpr int kThreads = (kWarps + 4) * 32;
+
+// kTwo: 9 to 16 query rows.  Each consumer group then takes all stages for 8 of the rows; with up to 8
+// rows the groups take the stages in turn.
+template <int kD, bool kTwo>
 struct Config {
-  static constexpr int kWarps = kNB == 1 ? 16 : 8;  // consumers: 56 to 100 registers a lane hold the state of 8 or 16 rows
-  static constexpr int kGroups = kWarps / 8;
-  static constexpr int kThreads = (kWarps + 4) * 32;  // and a warpgroup of which one warp produces
-  static constexpr int kRowsPad = kD + 4;  // floats of a row in the merge buffer: outputs, max, sum
-  static constexpr uint32_t kMergeBytes = 8 * 8 * kNB * kRowsPad * 4;  // one consumer group's state
-  static constexpr uint32_t kQueryBytes = kWarps * (kNB * (kD / 32) * 512 + kNB * 64 + 16);  // WarpRows
-  static constexpr uint32_t kOther = kMergeBytes + static_cast<uint32_t>(sizeof(Stage)) * kStages + kQueryBytes;
+  static constexpr uint32_t kStep = kTwo ? 1 : 2;      // a group's stages are every kStep-th
+  static constexpr uint32_t kReaders = kTwo ? 16 : 8;  // warps that read a stage
+  static constexpr int kRowsPad = kD + 4;              // floats of a row in the merge buffer: outputs, max, sum
+  static constexpr uint32_t kMergeBytes = 8 * 8 * kRowsPad * 4;  // one consumer group's state
+  static constexpr uint32_t kQueryBytes = kWarps * ((kD / 32) * 512 + 64 + 16);  // WarpRows
+  static constexpr uint32_t kOther = kMergeBytes + static_cast<uint32_t>(sizeof(Stage)) * kStages + kQueryBytes + 2 * 32 * sizeof(Job);
   static constexpr uint32_t kRing = (226u * 1024u - kOther) / 256u * 128u;  // of each half
   static constexpr uint32_t kSmem = 2 * kRing + kOther;
 };
 
+// The piece of a unit that a producer is handing out.
+struct Piece {
+  uint32_t seq, head0, heads, slot, direct, single, q;
+  int32_t pos0;  // of the first new token
+};
+
 struct Shared {
+  Piece pieces[2];
   uint64_t full[2][kStages], empty[2][kStages], merged;  // of a stage's K half and its V half
   uint32_t offset[2][kStages];  // ring offsets of the halves' data
   uint64_t warp_sum[20];
@@ -222,6 +244,13 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ void sts64(uint32_t a, uint2 v) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(v.x), "r"(v.y) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ float2 lds_f2(uint32_t a) {
   const uint2 v = lds64(a);
   return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
@@ -255,11 +284,11 @@ struct Place {
 
 template <int kD, int kNB>
 __device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, WarpRows<kD, kNB>* wr, Rows rows, uint32_t context,
-                                            uint32_t head, uint32_t lane) {
+                                            uint32_t head, uint32_t row0, uint32_t lane) {
   const uint32_t g = lane >> 2, quad = lane & 3;
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
-    const uint32_t r = nb * 8 + g, tok = r / p.group, in_group = r % p.group;
+    const uint32_t r = row0 + nb * 8 + g, tok = r / p.group, in_group = r % p.group;
     const bool live = r < rows.q * p.group;
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (rows.first + (live ? tok : 0u)) * p.q_stride +
                                                       uint64_t{head * p.group + (live ? in_group : 0u)} * kD) +
@@ -281,8 +310,8 @@ __device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, 
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
     if (quad == 0) {
-      wr->qsum[r] = sum * p.qscale;
-      wr->pos[r] = static_cast<int32_t>(context - rows.q + tok);
+      wr->qsum[nb * 8 + g] = sum * p.qscale;
+      wr->pos[nb * 8 + g] = static_cast<int32_t>(context - rows.q + tok);
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -725,18 +754,19 @@ __device__ __noinline__ void edge_tile(const Params& p, State<kD, kNB>* state, u
 // ---- the producer warps --------------------------------------------------------------------------
 // One fills the ring of the K halves, one that of the V halves; both walk the same stages.  The K warp also
 // writes the stages' descriptions.
-template <int kD, int kNB>
+template <int kD, bool kTwo>
 struct Producer {
-  using C = Config<kD, kNB>;
+  using C = Config<kD, kTwo>;
   const Params& p;
   Shared& sh;
-  Stage* stages;
-  uint8_t* ring;  // this half's
-  uint32_t ring_at;  // its address
+  uint32_t stages;  // address of the stages' descriptions
+  uint32_t jobs;    // of this warp's 32 jobs
+  uint32_t ring;    // of this half's ring
   uint32_t half, lane;
   uint32_t st = 0;      // stages emitted
   uint32_t oldest = 0;  // the first stage whose data is still in use
   uint32_t head = 0;
+  uint32_t first_st = 0;  // of the piece
   bool ok = true;
 
   __device__ __forceinline__ void pop() {
@@ -762,104 +792,132 @@ struct Producer {
     return at;
   }
 
-  // A tile per lane: tokens [t0, t0 + n) of a block at `payload`.
-  struct Source {
-    const uint8_t* payload;
-    uint32_t f, mode, sref, t0, n, pos;
-  };
-  struct Piece {
-    uint32_t seq, head0, heads, slot, direct, single;
-    int32_t pos0;  // of the first new token
-    uint32_t q;    // new tokens
-  };
-
-  // Stages of up to `per` (a power of two) tiles each, from lanes < count; none: one stage without tiles.
-  __device__ __forceinline__ void emit(const Source& x, uint32_t count, uint32_t per, const Piece& pc, uint32_t flags) {
-    const bool packed = pc.heads == p.H;  // all heads of a token: a tile's codes are one piece of the slot
-    const uint32_t rb = x.f == dev::kFp16 ? kD * 2 : x.f == dev::kInt4 ? kD / 2 : kD, pb = x.f == dev::kInt4 ? 8 : 4;
-    const bool live = lane < count, params = live && x.f != dev::kFp16 && x.mode == 0;
-    const uint32_t codes = live ? x.n * pc.heads * rb : 0u;
-    const uint32_t row0 = half ? p.T + x.t0 : x.t0;
-    const uint8_t* src = x.payload + (uint64_t{row0} * p.H + pc.head0) * rb;
-    // The parameters of all heads of the tile's tokens, rounded out to 16 bytes (the slot's end is).
-    uint64_t pa = 0;
-    uint32_t pn = 0;
-    if (params) {
-      pa = p.code_bytes[x.f] + uint64_t{row0} * p.H * pb;
-      pn = static_cast<uint32_t>(((pa + x.n * p.H * pb + 15) & ~uint64_t{15}) - (pa & ~uint64_t{15}));
-    }
-    const uint8_t* psrc = x.payload + (pa & ~uint64_t{15});
-    const uint32_t bytes = codes + pn, in_stage = lane & (per - 1);
-    uint32_t upto = bytes;  // of the stage's tiles up to this one
-    for (uint32_t o = 1; o < per; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-      if (in_stage >= o) upto += y;
-    }
-    const float2 w = x.mode != 0 ? dev::block_params_value(x.mode, x.sref) : make_float2(1.0f, 0.0f);
-    // Whether every row sees all the tile's tokens.
-    const int32_t first = static_cast<int32_t>(x.pos), end = first + static_cast<int32_t>(x.n);
-    const bool whole = end <= pc.pos0 + 1 &&
-                       (p.window == 0 || static_cast<uint32_t>(pc.pos0 + static_cast<int32_t>(pc.q) - 1 - first) < p.window ||
-                        x.pos + x.n <= p.sinks);
-    const uint32_t hidden = __ballot_sync(0xFFFFFFFFu, live && !whole), part = __ballot_sync(0xFFFFFFFFu, live && x.n < 16);
-    const uint32_t f0 = __shfl_sync(0xFFFFFFFFu, x.f, lane & ~(per - 1));
-    const uint32_t other = __ballot_sync(0xFFFFFFFFu, live && x.f != f0);
-    const uint32_t n_st = count == 0 ? 1u : (count + per - 1) / per;
-    for (uint32_t k = 0; k < n_st; ++k) {
-      const uint32_t tiles = min(per, count - k * per);  // 0 of 0
-      const uint32_t total = __shfl_sync(0xFFFFFFFFu, upto, k * per + (tiles ? tiles - 1 : 0u));
-      const uint32_t at = reserve(total);
-      if (!ok) return;  // gave up: nothing more is copied, and the consumers give up as well
-      const uint32_t slot_i = st % kStages;
-      const bool mine = live && lane / per == k;
-      const uint32_t off = at + upto - bytes;
-      Stage& m = stages[slot_i];
-      uint64_t* bar = &sh.full[half][slot_i];
+  // The next stage: `tiles` jobs from job `from` on (none: only its description).
+  __device__ __forceinline__ void emit(uint32_t from, uint32_t tiles, bool pairs, uint32_t flags) {
+    const uint32_t job = jobs + (from + lane) * static_cast<uint32_t>(sizeof(Job));
+    uint4 size = make_uint4(0u, 0u, 0u, 0u);  // codes, pn, upto, delta
+    if (lane < tiles) size = lds128(job + 16);
+    size.z -= __shfl_sync(0xFFFFFFFFu, size.z - size.x - size.y, 0);  // counted from the stage's first tile
+    const uint32_t total = tiles ? __shfl_sync(0xFFFFFFFFu, size.z, tiles - 1) : 0u;
+    const uint32_t at = reserve(total);
+    if (!ok) return;  // gave up: nothing more is copied, and the consumers give up as well
+    const uint32_t slot = st % kStages, m = stages + slot * static_cast<uint32_t>(sizeof(Stage));
+    const uint32_t off = ring + at + size.z - size.x - size.y, where = m + lane * static_cast<uint32_t>(sizeof(Tile));
+    const bool packed = sh.pieces[half].heads == p.H;  // all heads of a token: a tile's codes are one piece of the slot
+    if (lane == 0) {
+      sh.offset[half][slot] = at;
       if (half == 0) {
-        const uint32_t lanes = ((1u << per) - 1u) << (k * per);
-        const bool pairs = per > pc.single && tiles == per && ((hidden | part | other) & lanes) == 0;
-        const uint32_t fl = pc.direct | flags | (flags & kFirstStages && st - first_st < C::kGroups ? kFirst : 0u);
-        if (lane == 0) {
-          *reinterpret_cast<uint4*>(&m.tiles) = make_uint4(tiles, fl, pc.seq, pc.head0);
-          *reinterpret_cast<uint4*>(&m.heads) = make_uint4(pc.heads, pc.slot, pairs, 0u);
+        constexpr uint32_t kHead = offsetof(Stage, tiles), kHead2 = offsetof(Stage, heads);
+        const uint32_t fl = sh.pieces[half].direct | flags | (flags & kFirstStages && st - first_st < C::kStep ? kFirst : 0u);
+        sts128(m + kHead, make_uint4(tiles, fl, sh.pieces[half].seq, sh.pieces[half].head0));
+        sts128(m + kHead2, make_uint4(sh.pieces[half].heads, sh.pieces[half].slot, pairs, 0u));
+      }
+    }
+    if (lane < tiles) {
+      const uint32_t po = size.y ? off + size.x + size.w : where + offsetof(Tile, ws);
+      if (half == 0) {
+        const uint4 d = lds128(job + 32);  // fn, pos, row_step, token_step
+        const uint2 w = lds64(job + 48);
+        sts128(where, make_uint4(d.x, d.y, off, po));
+        sts64(where + 24, make_uint2(d.z, d.w));
+        sts64(where + 32, w);
+      } else {
+        sts64(where + 16, make_uint2(off, po));
+      }
+    }
+    __syncwarp();
+    uint64_t* bar = &sh.full[half][slot];
+    if (lane == 0) mbar_arrive_expect(bar, total);
+    __syncwarp();
+    if (lane < tiles) {
+      const uint4 a = lds128(job);
+      if (packed) bulk_load(off, uint64_t{a.x} | uint64_t{a.y} << 32, size.x, bar);
+      if (size.y) bulk_load(off + size.x, uint64_t{a.z} | uint64_t{a.w} << 32, size.y, bar);
+    }
+    if (!packed) {
+      for (uint32_t i = 0; i < tiles; ++i) {  // a copy per token: its heads lie together
+        const uint32_t j = jobs + (from + i) * static_cast<uint32_t>(sizeof(Job));
+        const uint2 a = lds64(j);
+        const uint32_t fn = lds32(j + 32), f = fn & 0xFFu, rb = f == dev::kFp16 ? kD * 2 : f == dev::kInt4 ? kD / 2 : kD;
+        const uint32_t to = __shfl_sync(0xFFFFFFFFu, off, i);
+        if (lane < ((fn >> 8) & 0xFFu)) {
+          bulk_load(to + lane * sh.pieces[half].heads * rb, (uint64_t{a.x} | uint64_t{a.y} << 32) + uint64_t{lane} * p.H * rb,
+                    sh.pieces[half].heads * rb, bar);
         }
       }
-      if (lane == 0) sh.offset[half][slot_i] = at;
-      if (mine) {
-        Tile& d = m.tile[in_stage];
-        const uint32_t where = smem_addr(&d);
-        const uint32_t po = pn ? ring_at + off + codes + static_cast<uint32_t>(pa & 15) + pc.head0 * pb : where + 32;
-        if (half == 0) {
-          *reinterpret_cast<uint4*>(&d) = make_uint4(x.f | x.n << 8 | (whole ? 1u << 16 : 0u), x.pos, ring_at + off, po);
-          *reinterpret_cast<uint2*>(&d.row_step) = pn ? make_uint2(pb, p.H * pb) : make_uint2(0u, 0u);
-          *reinterpret_cast<float2*>(&d.ws) = w;
-        } else {
-          *reinterpret_cast<uint2*>(&d.vc) = make_uint2(ring_at + off, po);
-        }
+    }
+    ++st;
+  }
+
+  // Tiles of lanes < count: tokens [t0, t0 + n) of a block at `payload`.  They go out sorted by format (their order
+  // does not matter to the sum), so that two tiles of one format share a softmax step: all but FP16 ones, whose
+  // halves would fill too much of the ring, and those that some row sees in part.
+  __device__ __forceinline__ void hand_out(uint32_t count, const uint8_t* payload, uint32_t f, uint32_t mode, uint32_t sref, uint32_t t0,
+                                           uint32_t n, uint32_t pos) {
+    const bool live = lane < count;
+    __syncwarp();  // the jobs before have been read
+    {
+      // Whether every row sees all the tile's tokens.
+      const int32_t pos0 = sh.pieces[half].pos0, first = static_cast<int32_t>(pos), end = first + static_cast<int32_t>(n);
+      const bool whole =
+          end <= pos0 + 1 && (p.window == 0 || static_cast<uint32_t>(pos0 + static_cast<int32_t>(sh.pieces[half].q) - 1 - first) < p.window ||
+                              pos + n <= p.sinks);
+      const uint32_t key = whole && n == 16 ? f : 4u;
+      uint32_t rank = 0;
+#pragma unroll
+      for (uint32_t k = 0; k <= 4; ++k) {
+        const uint32_t of_k = __ballot_sync(0xFFFFFFFFu, live && key == k);
+        if (key > k) rank += __popc(of_k);
+        else if (key == k) rank += __popc(of_k & ((1u << lane) - 1u));
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect(bar, total);
-      __syncwarp();
-      if (mine) {
-        if (packed) bulk_load(ring + off, src, codes, bar);
-        if (pn) bulk_load(ring + off + codes, psrc, pn, bar);
+      const uint32_t heads = sh.pieces[half].heads, head0 = sh.pieces[half].head0;
+      const uint32_t rb = f == dev::kFp16 ? kD * 2 : f == dev::kInt4 ? kD / 2 : kD, pb = f == dev::kInt4 ? 8 : 4;
+      const uint32_t row0 = half ? p.T + t0 : t0;
+      // The parameters of all heads of the tile's tokens, rounded out to 16 bytes (the slot's end is).
+      uint64_t pa = 0;
+      uint32_t pn = 0;
+      if (f != dev::kFp16 && mode == 0) {
+        pa = p.code_bytes[f] + uint64_t{row0} * p.H * pb;
+        pn = static_cast<uint32_t>(((pa + n * p.H * pb + 15) & ~uint64_t{15}) - (pa & ~uint64_t{15}));
       }
-      if (!packed) {
-        for (uint32_t i = 0; i < tiles; ++i) {  // a copy per token: its heads lie together
-          const uint32_t from = k * per + i;
-          const uint64_t base = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(src), from);
-          const uint32_t nt = __shfl_sync(0xFFFFFFFFu, x.n, from), r = __shfl_sync(0xFFFFFFFFu, rb, from);
-          const uint32_t o = __shfl_sync(0xFFFFFFFFu, off, from);
-          if (lane < nt) {
-            bulk_load(ring + o + lane * pc.heads * r, reinterpret_cast<const uint8_t*>(base) + uint64_t{lane} * p.H * r, pc.heads * r,
-                      bar);
-          }
-        }
+      const uint64_t src = reinterpret_cast<uint64_t>(payload) + (uint64_t{row0} * p.H + head0) * rb;
+      const uint64_t psrc = reinterpret_cast<uint64_t>(payload) + (pa & ~uint64_t{15});
+      if (live) {
+        const uint32_t job = jobs + rank * static_cast<uint32_t>(sizeof(Job));
+        sts128(job, make_uint4(static_cast<uint32_t>(src), static_cast<uint32_t>(src >> 32), static_cast<uint32_t>(psrc),
+                               static_cast<uint32_t>(psrc >> 32)));
+        sts128(job + 16, make_uint4(n * heads * rb, pn, 0u, static_cast<uint32_t>(pa & 15) + head0 * pb));
+        sts128(job + 32, make_uint4(f | n << 8 | (whole ? 1u << 16 : 0u), pos, pn ? pb : 0u, pn ? p.H * pb : 0u));
+        const float2 w = mode != 0 ? dev::block_params_value(mode, sref) : make_float2(1.0f, 0.0f);
+        sts64(job + 48, make_uint2(__float_as_uint(w.x), __float_as_uint(w.y)));
       }
-      ++st;
+    }
+    __syncwarp();
+    const uint32_t mine = jobs + lane * static_cast<uint32_t>(sizeof(Job));
+    uint32_t upto = 0, fn = 0;
+    if (live) {
+      const uint2 size = lds64(mine + 16);
+      upto = size.x + size.y;
+      fn = lds32(mine + 32);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= static_cast<uint32_t>(o)) upto += y;
+    }
+    if (live) sts32(mine + 24, upto);
+    const uint32_t next = __shfl_down_sync(0xFFFFFFFFu, fn, 1);
+    // bit k: jobs k and k + 1 are alike and may share a step
+    const uint32_t alike = __ballot_sync(0xFFFFFFFFu, lane + 1 < count && fn == next && fn >> 8 == (1u << 8 | 16u) && (fn & 0xFFu) != dev::kFp16);
+    __syncwarp();
+    const uint32_t single = sh.pieces[half].single;
+    for (uint32_t from = 0, tiles; from < count && ok; from += tiles) {
+      const uint32_t links = (1u << (2 * single - 1)) - 1u;
+      const bool pairs = ((alike >> from) & links) == links;
+      tiles = pairs ? 2 * single : min(single, count - from);
+      emit(from, tiles, pairs, kFirstStages);
     }
   }
-  uint32_t first_st = 0;  // of the piece
 
   // First k in [0, count) with cost[k] >= target (count if none).
   __device__ __forceinline__ uint32_t find(const uint32_t* cost, uint32_t count, uint32_t target) {
@@ -880,42 +938,51 @@ struct Producer {
   }
 
   __device__ __forceinline__ void run() {
-    const uint64_t W = sh.total, x0 = blockIdx.x * W / gridDim.x, x1 = (uint64_t{blockIdx.x} + 1) * W / gridDim.x;
     uint64_t base = sh.base;  // of sequence i's units
-    for (uint32_t i = sh.seq; i < p.nseq && base < x1 && ok; ++i) {
+    for (uint32_t i = sh.seq; i < p.nseq && ok; ++i) {
+      const uint64_t W = sh.total, x0 = blockIdx.x * W / gridDim.x, x1 = (uint64_t{blockIdx.x} + 1) * W / gridDim.x;
+      if (base >= x1) break;
       const Rows rows = rows_of(p, i);
       uint32_t w = p.cost[i];
       if (rows.q == 0 || uint64_t{rows.q} * p.group > kStreamRows) w = 0;
       if (w == 0) continue;
-      uint32_t first;
-      const uint32_t count = count_of(p, i, &first);
       uint32_t hg = x0 > base ? static_cast<uint32_t>((x0 - base) / w) : 0u;
       for (; hg < p.head_groups && ok; ++hg) {
         const uint64_t ub = base + uint64_t{hg} * w;
         if (ub >= x1) break;
         const uint32_t lo = x0 > ub ? static_cast<uint32_t>(x0 - ub) : 0u;
         const uint32_t hi = x1 - ub < w ? static_cast<uint32_t>(x1 - ub) : w;
-        piece(i, hg, lo, hi, w, first, count, rows.q);
+        // Both producers describe the piece, in the same words, each before it goes on to it; a producer
+        // that is ahead of the other has the description of its own half.
+        const uint32_t heads = min(8u, p.H - hg * 8);
+        __syncwarp();
+        if (lane == 0) {
+          Piece& pc = sh.pieces[half];
+          pc.seq = i;
+          pc.head0 = hg * 8;
+          pc.heads = heads;
+          pc.slot = blockIdx.x + i * p.head_groups + hg;
+          pc.direct = lo == 0 && hi == w ? kDirect : 0u;
+          pc.single = heads > 4 ? 1u : heads > 2 ? 2u : heads > 1 ? 4u : 8u;  // tiles that occupy a group's warps
+          pc.q = rows.q;
+          pc.pos0 = static_cast<int32_t>(p.context[i] - rows.q);
+        }
+        __syncwarp();
+        uint32_t first;
+        const uint32_t count = count_of(p, i, &first);
+        piece(first, count, lo, hi);
       }
       base += uint64_t{p.head_groups} * w;
     }
-    const Source none{nullptr, 0, 0, 0, 0, 0, 0};
-    const Piece end{0, 0, p.H, 0, 0, 1, 0, 0};
-    for (int k = 0; k < C::kGroups && ok; ++k) emit(none, 0, 1, end, kDone);
+    for (uint32_t k = 0; k < C::kStep && ok; ++k) emit(0, 0, false, kDone);
   }
 
-  // The blocks of unit (i, hg) whose cost begins in [lo, hi).
-  __device__ __forceinline__ void piece(uint32_t i, uint32_t hg, uint32_t lo, uint32_t hi, uint32_t w, uint32_t first,
-                                        uint32_t count, uint32_t q) {
-    const uint32_t head0 = hg * 8, heads = min(8u, p.H - head0);
-    const uint32_t single = heads > 4 ? 1u : heads > 2 ? 2u : heads > 1 ? 4u : 8u;  // tiles that occupy a group's warps
-    const Piece pc{i,  head0, heads, blockIdx.x + i * p.head_groups + hg, lo == 0 && hi == w ? kDirect : 0u, single,
-                   static_cast<int32_t>(p.context[i] - q), q};
+  // The blocks of a unit whose cost begins in [lo, hi).
+  __device__ __forceinline__ void piece(uint32_t first, uint32_t count, uint32_t lo, uint32_t hi) {
     const uint32_t* cost = p.block_cost + first;
     uint32_t j0 = lo == 0 ? 0u : find(cost, count, lo) + 1;
-    // Stages alternate between the consumer groups.  The first stage of each carries kFirst; at the end
-    // every group gets a stage without tiles that carries kLast, after as many empty ones as bring the
-    // piece to a multiple of kGroups.
+    // The first stage of each consumer group carries kFirst; at the end every group gets a stage without tiles
+    // that carries kLast, after as many empty ones as bring the piece to a multiple of kStep.
     first_st = st;
     bool more = true;
     while (more && ok) {
@@ -935,12 +1002,9 @@ struct Producer {
       }
       more = __all_sync(0xFFFFFFFFu, inside);  // else the piece ends in this batch
       const uint32_t nt = (v + 15) / 16;
-      // Two tiles of one format share a softmax step, but for FP16: its halves would fill too much of the ring.
-      const uint32_t some = __ballot_sync(0xFFFFFFFFu, nt > 0), f_some = __shfl_sync(0xFFFFFFFFu, f, __ffs(some | 1u << 31) - 1);
-      const uint32_t per = f_some == dev::kFp16 || __any_sync(0xFFFFFFFFu, nt > 0 && f != f_some) ? single : 2 * single;
       const uint32_t mode = f == dev::kFp16 ? 0u : (b.y >> 4) & 3u;
-      if (__all_sync(0xFFFFFFFFu, inside && nt == 1)) {
-        emit(Source{payload, f, mode, b.z, 0u, v, b.w}, 32, per, pc, kFirstStages);
+      if (__all_sync(0xFFFFFFFFu, nt == 1 || (nt == 0 && !inside))) {
+        hand_out(__popc(__ballot_sync(0xFFFFFFFFu, nt > 0)), payload, f, mode, b.z, 0u, v, b.w);  // a tile for every block, from lane 0 on
       } else {
         uint32_t upto = nt;
 #pragma unroll
@@ -959,50 +1023,46 @@ struct Producer {
             if (x <= k) at += o;
           }
           at = min(at, 31u);
-          Source x;
-          x.payload = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(payload), at));
-          x.f = __shfl_sync(0xFFFFFFFFu, f, at);
-          x.mode = __shfl_sync(0xFFFFFFFFu, mode, at);
-          x.sref = __shfl_sync(0xFFFFFFFFu, b.z, at);
           const uint32_t before = __shfl_sync(0xFFFFFFFFu, upto - nt, at), tv = __shfl_sync(0xFFFFFFFFu, v, at);
-          const uint32_t start = __shfl_sync(0xFFFFFFFFu, b.w, at);
-          x.t0 = k < total ? (k - before) * 16 : 0u;
-          x.n = k < total ? min(16u, tv - x.t0) : 0u;
-          x.pos = start + x.t0;
-          emit(x, min(32u, total - t), per, pc, kFirstStages);
+          const uint32_t t0 = k < total ? (k - before) * 16 : 0u;
+          hand_out(min(32u, total - t),
+                   reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(payload), at)),
+                   __shfl_sync(0xFFFFFFFFu, f, at), __shfl_sync(0xFFFFFFFFu, mode, at), __shfl_sync(0xFFFFFFFFu, b.z, at), t0,
+                   k < total ? min(16u, tv - t0) : 0u, __shfl_sync(0xFFFFFFFFu, b.w, at) + t0);
         }
       }
       j0 += 32;
     }
-    const Source none{nullptr, 0, 0, 0, 0, 0, 0};
-    const uint32_t done = st - first_st, fill = (C::kGroups - done % C::kGroups) % C::kGroups + C::kGroups;
-    for (uint32_t k = 0; k < fill && ok; ++k) emit(none, 0, 1, pc, kFirstStages | (k + C::kGroups >= fill ? kLast : 0u));
+    const uint32_t done = st - first_st, fill = (C::kStep - done % C::kStep) % C::kStep + C::kStep;
+    for (uint32_t k = 0; k < fill && ok; ++k) emit(0, 0, false, kFirstStages | (k + C::kStep >= fill ? kLast : 0u));
   }
 };
 
-template <int kD, int kNB>
-__global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(const __grid_constant__ Params p) {
-  using C = Config<kD, kNB>;
+template <int kD, bool kTwo>
+__global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_constant__ Params p) {
+  using C = Config<kD, kTwo>;
+  constexpr int kNB = 1;  // column blocks of a warp
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
   float* merge = reinterpret_cast<float*>(smem + 2 * C::kRing);
   Stage* stages = reinterpret_cast<Stage*>(smem + 2 * C::kRing + C::kMergeBytes);
   __shared__ Shared sh;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  dev::allow_dependents_to_launch();  // the merge, which waits for this kernel's end
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kStages; ++i) {
       for (int half = 0; half < 2; ++half) {
         mbar_init(&sh.full[half][i], 1);
-        mbar_init(&sh.empty[half][i], 8);
+        mbar_init(&sh.empty[half][i], C::kReaders);
       }
     }
-    mbar_init(&sh.merged, C::kWarps);
+    mbar_init(&sh.merged, kWarps);
     mbar_fence_init();
   }
   // ---- where this CTA's share begins: the costs of the sequences, added up in chunks of consecutive ones
   {
-    const uint32_t chunk = (p.nseq + C::kThreads - 1) / C::kThreads;
+    const uint32_t chunk = (p.nseq + kThreads - 1) / kThreads;
     const uint32_t a = min(threadIdx.x * chunk, p.nseq), b = min(a + chunk, p.nseq);
     auto cost_of = [&](uint32_t i) -> uint64_t {
       const Rows rows = rows_of(p, i);
@@ -1023,7 +1083,7 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
     }
     __syncthreads();
     uint64_t total = 0;
-    for (uint32_t w = 0; w < C::kThreads / 32; ++w) {
+    for (uint32_t w = 0; w < kThreads / 32; ++w) {
       if (w < warp) upto += sh.warp_sum[w];
       total += sh.warp_sum[w];
     }
@@ -1047,19 +1107,18 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
     __syncthreads();
   }
 
-  // Registers: 96 (or 168) a thread at launch; the producers' warpgroup hands most of its own over.
-  if (warp >= C::kWarps) {
-    if constexpr (kNB == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    const uint32_t half = warp - C::kWarps;
+  if (warp >= kWarps) {
+    const uint32_t half = warp - kWarps;
     if (half > 1) return;
-    Producer<kD, kNB> producer{p, sh, stages, ring + half * C::kRing, smem_addr(ring) + half * C::kRing, half, lane};
+    const uint32_t base = smem_addr(ring);
+    Producer<kD, kTwo> producer{p, sh, smem_addr(stages), base + C::kSmem - (2 - half) * 32 * static_cast<uint32_t>(sizeof(Job)),
+                                base + half * C::kRing, half, lane};
     producer.run();
     if (!producer.ok && lane == 0) atomicOr(p.err, dev::kErrInternal);
     return;
   }
 
   // ---- consumers
-  if constexpr (kNB == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
   const uint32_t group = warp / 8, w8 = warp % 8;
   const uint32_t wr_at = smem_addr(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp * static_cast<uint32_t>(sizeof(WarpRows<kD, kNB>));
   const uint32_t stages_at = smem_addr(stages);
@@ -1071,7 +1130,7 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
     if (lane == 0) mbar_arrive(&sh.merged);
     return mbar_wait(&sh.merged, meets++ & 1);
   };
-  for (uint32_t st = group;; st += C::kGroups) {
+  for (uint32_t st = kTwo ? 0u : group;; st += C::kStep) {
     const uint32_t si = st % kStages, parity = (st / kStages) & 1;
     if (!mbar_wait(&sh.full[0][si], parity)) {
       if (lane == 0) atomicOr(p.err, dev::kErrInternal);
@@ -1086,7 +1145,7 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
       const uint32_t single = heads > 4 ? 1u : heads > 2 ? 2u : heads > 1 ? 4u : 8u;
       // a group's warps beyond `single` x heads have no tile
       if (lane == 0) wr->place = make_uint4(heads, w8 % heads, w8 / heads < single ? w8 / heads : 1u << 16, single);
-      begin_piece<kD, kNB>(p, s, wr, rows_of(p, seq), p.context[seq], head0 + w8 % heads, lane);
+      begin_piece<kD, kNB>(p, s, wr, rows_of(p, seq), p.context[seq], head0 + w8 % heads, kTwo ? group * 8 : 0u, lane);
     }
     const uint4 place = lds128(wr_at + static_cast<uint32_t>(sizeof(WarpRows<kD, kNB>)) - 16);
     const Place at{wr_at, place.x, place.y, lane};
@@ -1146,157 +1205,183 @@ __global__ void __launch_bounds__(Config<kD, kNB>::kThreads, 1) stream_kernel(co
     if (lane == 0) mbar_arrive(&sh.empty[1][si]);
 
     if (flags & kLast) {
-      // ---- merge the warps of each head: outputs, max and sum of every row.  The second group leaves its
-      // state in the buffer, the first joins it to its own warp by warp and leaves the sum there.
+      // ---- merge the warps of each head: outputs, max and sum of every row.  Groups that took the stages in
+      // turn: the second leaves its state in the buffer, the first joins it to its own warp by warp and
+      // leaves the sum there.  Groups of different rows use the buffer one after the other.
       const uint32_t g = lane >> 2, quad = lane & 3;
       const float unit = s.E == kNoExponent ? 0.0f : exp2f(static_cast<float>(s.E));
-      float* mine = merge + w8 * 8 * kNB * C::kRowsPad;
+      float* mine = merge + w8 * 8 * C::kRowsPad;
+      const Rows rows = rows_of(p, head.z);
+      const uint32_t head0 = head.w, heads = at.heads, n_rows = rows.q * p.group;
       bool met = true;
 #pragma unroll 1
-      for (int gr = C::kGroups - 1; gr >= 0; --gr) {
-        if (static_cast<int>(group) == gr) {
+      for (uint32_t turn = 0; turn < 2; ++turn) {
+        if (group == 1 - turn) {
+          const bool join = !kTwo && turn == 1;
 #pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) {
+          for (int c = 0; c < 2; ++c) {
+            float l = s.l[0][c], b = s.bias[0][c], m_own = s.m[0][c], fo = 1.0f, ft = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float l = s.l[nb][c], b = s.bias[nb][c], m_own = s.m[nb][c], fo = 1.0f, ft = 0.0f;
-#pragma unroll
-              for (int o = 4; o < 32; o <<= 1) {
-                l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-                b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
-              }
-              float* row = mine + (nb * 8 + quad * 2 + c) * C::kRowsPad;
-              if (gr + 1 < C::kGroups) {
-                const float2 ml = *reinterpret_cast<const float2*>(row + kD);
-                const float M = fmaxf(m_own, ml.x);
-                fo = M == -INFINITY ? 1.0f : exp2f(m_own - M);
-                ft = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
-                l = fmaf(l, fo, ml.y * ft);
-                m_own = M;
-              }
-#pragma unroll
-              for (int mt = 0; mt < kD / 16; ++mt) {
-                float2* at2 = reinterpret_cast<float2*>(row + g * (kD / 8) + 2 * mt);
-                float2 x = make_float2(fmaf(s.acc[nb][mt][c], unit, b), fmaf(s.acc[nb][mt][2 + c], unit, b));
-                if (gr + 1 < C::kGroups) {
-                  const float2 y = *at2;
-                  x = make_float2(fmaf(x.x, fo, y.x * ft), fmaf(x.y, fo, y.y * ft));
-                }
-                *at2 = x;
-              }
-              __syncwarp();  // every lane has read the other group's max and sum
-              if (g == 0) *reinterpret_cast<float2*>(row + kD) = make_float2(m_own, l);
+            for (int o = 4; o < 32; o <<= 1) {
+              l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+              b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
             }
+            float* row = mine + (quad * 2 + c) * C::kRowsPad;
+            if (join) {
+              const float2 ml = *reinterpret_cast<const float2*>(row + kD);
+              const float M = fmaxf(m_own, ml.x);
+              fo = M == -INFINITY ? 1.0f : exp2f(m_own - M);
+              ft = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
+              l = fmaf(l, fo, ml.y * ft);
+              m_own = M;
+            }
+#pragma unroll
+            for (int mt = 0; mt < kD / 16; ++mt) {
+              float2* at2 = reinterpret_cast<float2*>(row + g * (kD / 8) + 2 * mt);
+              float2 x = make_float2(fmaf(s.acc[0][mt][c], unit, b), fmaf(s.acc[0][mt][2 + c], unit, b));
+              if (join) {
+                const float2 y = *at2;
+                x = make_float2(fmaf(x.x, fo, y.x * ft), fmaf(x.y, fo, y.y * ft));
+              }
+              *at2 = x;
+            }
+            __syncwarp();  // every lane has read the other group's max and sum
+            if (g == 0) *reinterpret_cast<float2*>(row + kD) = make_float2(m_own, l);
           }
         }
         met = met && meet();
+        if (!met) break;
+        if (!kTwo && turn == 0) continue;
+        const uint32_t row0 = kTwo ? (1 - turn) * 8 : 0u, rows_here = n_rows > row0 ? min(8u, n_rows - row0) : 0u;
+        for (uint32_t i = threadIdx.x; i < heads * rows_here * (kD / 4); i += kWarps * 32) {
+          const uint32_t e = i % (kD / 4), r = (i / (kD / 4)) % rows_here, h = i / (kD / 4) / rows_here;
+          float M = -INFINITY, L = 0.0f;
+          float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (uint32_t t = 0; t < single; ++t) M = fmaxf(M, merge[((t * heads + h) * 8 + r) * C::kRowsPad + kD]);
+          for (uint32_t t = 0; t < single; ++t) {
+            const float* row = merge + ((t * heads + h) * 8 + r) * C::kRowsPad;
+            const float2 ml = *reinterpret_cast<const float2*>(row + kD);
+            const float a = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
+            const float4 x = *reinterpret_cast<const float4*>(row + 4 * e);
+            L = fmaf(ml.y, a, L);
+            o.x = fmaf(x.x, a, o.x);
+            o.y = fmaf(x.y, a, o.y);
+            o.z = fmaf(x.z, a, o.z);
+            o.w = fmaf(x.w, a, o.w);
+          }
+          if (flags & kDirect) {
+            if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros
+            const uint32_t tok = (row0 + r) / p.group, gi = (row0 + r) % p.group;
+            *reinterpret_cast<uint2*>(p.out + (rows.first + tok) * p.out_stride + uint64_t{(head0 + h) * p.group + gi} * kD + 4 * e) =
+                make_uint2(dev::pack_f16x2(o.x / L, o.y / L), dev::pack_f16x2(o.z / L, o.w / L));
+          } else {
+            float* dst = p.partial + ((uint64_t{slot} * 8 + h) * p.slot_rows + row0 + r) * C::kRowsPad;
+            *reinterpret_cast<float4*>(dst + 4 * e) = o;
+            if (e == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(M, L);
+          }
+        }
+        met = met && meet();  // the buffer is written again
+        if (!met) break;
       }
       if (!met) {
         if (lane == 0) atomicOr(p.err, dev::kErrInternal);
         break;
       }
-      const uint32_t head0 = head.w;
-      const Rows rows = rows_of(p, head.z);
-      const uint32_t heads = at.heads, n_rows = rows.q * p.group, n_warps = single;
-      for (uint32_t i = threadIdx.x; i < heads * n_rows * (kD / 4); i += C::kWarps * 32) {
-        const uint32_t e = i % (kD / 4), r = (i / (kD / 4)) % n_rows, h = i / (kD / 4) / n_rows;
-        float M = -INFINITY, L = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t t = 0; t < n_warps; ++t) M = fmaxf(M, merge[((t * heads + h) * 8 * kNB + r) * C::kRowsPad + kD]);
-        for (uint32_t t = 0; t < n_warps; ++t) {
-          const float* row = merge + ((t * heads + h) * 8 * kNB + r) * C::kRowsPad;
-          const float2 ml = *reinterpret_cast<const float2*>(row + kD);
-          const float a = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
-          const float4 x = *reinterpret_cast<const float4*>(row + 4 * e);
-          L = fmaf(ml.y, a, L);
-          o.x = fmaf(x.x, a, o.x);
-          o.y = fmaf(x.y, a, o.y);
-          o.z = fmaf(x.z, a, o.z);
-          o.w = fmaf(x.w, a, o.w);
-        }
-        if (flags & kDirect) {
-          if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros
-          const uint32_t tok = r / p.group, gi = r % p.group;
-          *reinterpret_cast<uint2*>(p.out + (rows.first + tok) * p.out_stride + uint64_t{(head0 + h) * p.group + gi} * kD + 4 * e) =
-              make_uint2(dev::pack_f16x2(o.x / L, o.y / L), dev::pack_f16x2(o.z / L, o.w / L));
-        } else {
-          float* dst = p.partial + ((uint64_t{slot} * 8 + h) * p.slot_rows + r) * C::kRowsPad;
-          *reinterpret_cast<float4*>(dst + 4 * e) = o;
-          if (e == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(M, L);
-        }
-      }
-      if (!meet()) {  // the buffer is written again
-        if (lane == 0) atomicOr(p.err, dev::kErrInternal);
-        break;
-      }
     }
   }
 }
 
-// Joins the partial results of the units that several CTAs took: one CTA of kD / 4 threads x rows per
-// (sequence, head).  Also writes the zeros of rows whose sequence lists no block.
+// Joins the partial results of the units that several CTAs took: one CTA per (sequence, head, row), its warps
+// taking the partials in turn, each with its own running maximum.  Also writes the zeros of rows whose sequence
+// lists no block.
+constexpr int kMergeWarps = 8;
 template <int kD>
-__global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ Params p) {
-  constexpr int kPad = kD + 4, kLanes = kD / 4, kRows = 128 / kLanes;
-  const uint32_t i = blockIdx.x / p.H, head = blockIdx.x % p.H, hg = head / 8, h = head % 8;
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Params p) {
+  constexpr int kPad = kD + 4, kPer = kD / 32;  // floats of a row; elements of a lane
+  __shared__ float s_o[kMergeWarps][kD];
+  __shared__ float2 s_ml[kMergeWarps];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t r = blockIdx.x % p.slot_rows, unit_head = blockIdx.x / p.slot_rows;
+  const uint32_t i = unit_head / p.H, head = unit_head % p.H, hg = head / 8, h = head % 8;
+  dev::wait_for_prerequisites();
   const Rows rows = rows_of(p, i);
   const uint32_t n_rows = rows.q * p.group;
-  if (n_rows == 0 || uint64_t{rows.q} * p.group > kStreamRows) return;
-  const uint32_t e = threadIdx.x % kLanes;
-  const uint64_t W = p.prefix[p.nseq] * p.head_groups, w = p.prefix[i + 1] - p.prefix[i];
+  if (r >= n_rows || uint64_t{rows.q} * p.group > kStreamRows) return;
+  const uint64_t W = p.prefix[p.nseq] * p.head_groups, before = p.prefix[i], w = p.prefix[i + 1] - before;
   uint32_t c0 = 0, c1 = 0;
   if (w > 0) {
-    const uint64_t a = p.prefix[i] * p.head_groups + hg * w, b = a + w - 1;
+    const uint64_t a = before * p.head_groups + hg * w, b = a + w - 1;
     // CTA c takes [c W / G, (c + 1) W / G): the one that holds x is the largest c with c W / G <= x
     c0 = static_cast<uint32_t>(((a + 1) * p.ctas - 1) / W);
     c1 = static_cast<uint32_t>(((b + 1) * p.ctas - 1) / W);
     if (c0 == c1) return;  // one CTA had it all and wrote the rows
   }
-  const uint64_t unit = uint64_t{i} * p.head_groups + hg;
-  for (uint32_t r = threadIdx.x / kLanes; r < n_rows; r += kRows) {
-    float M = -INFINITY, L = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (w > 0) {
-      const float* base = p.partial + ((c0 + unit) * 8 + h) * p.slot_rows * kPad + uint64_t{r} * kPad;
-      const uint64_t step = uint64_t{8} * p.slot_rows * kPad;
-      // a CTA whose range is empty (more CTAs than cost) took nothing and wrote nothing
-      auto empty = [&](uint32_t c) { return p.ctas > W && c * W / p.ctas == (uint64_t{c} + 1) * W / p.ctas; };
-#pragma unroll 4
-      for (uint32_t c = c0; c <= c1; ++c) {
-        if (!empty(c)) M = fmaxf(M, base[(c - c0) * step + kD]);
-      }
-#pragma unroll 4
-      for (uint32_t c = c0; c <= c1; ++c) {
-        if (empty(c)) continue;
-        const float* s = base + (c - c0) * step;
-        const float2 ml = *reinterpret_cast<const float2*>(s + kD);
-        const float4 x = *reinterpret_cast<const float4*>(s + 4 * e);
-        const float a = M == -INFINITY ? 1.0f : exp2f(ml.x - M);
-        L = fmaf(ml.y, a, L);
-        o.x = fmaf(x.x, a, o.x);
-        o.y = fmaf(x.y, a, o.y);
-        o.z = fmaf(x.z, a, o.z);
-        o.w = fmaf(x.w, a, o.w);
-      }
+  float M = -INFINITY, L = 0.0f, o[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) o[k] = 0.0f;
+  if (w > 0) {
+    const uint64_t step = uint64_t{8} * p.slot_rows * kPad;
+    const float* base = p.partial + (c0 + uint64_t{i} * p.head_groups + hg) * step + (uint64_t{h} * p.slot_rows + r) * kPad;
+    // a CTA whose range is empty (more CTAs than cost) took nothing and may have written nothing
+    auto empty = [&](uint32_t c) { return p.ctas > W && c * W / p.ctas == (uint64_t{c} + 1) * W / p.ctas; };
+#pragma unroll 2
+    for (uint32_t c = c0 + warp; c <= c1; c += kMergeWarps) {
+      if (empty(c)) continue;
+      const float* s = base + (c - c0) * step;
+      const float2 ml = *reinterpret_cast<const float2*>(s + kD);
+      float x[kPer];
+      if constexpr (kPer == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(s + 4 * lane);
+      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(s + 2 * lane);
+      const float m = fmaxf(M, ml.x);
+      const float fo = m == -INFINITY ? 1.0f : exp2f(M - m), ft = m == -INFINITY ? 1.0f : exp2f(ml.x - m);
+      M = m;
+      L = fmaf(L, fo, ml.y * ft);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) o[k] = fmaf(o[k], fo, x[k] * ft);
     }
-    if (L == 0.0f && M == -INFINITY) L = 1.0f;
-    const uint32_t tok = r / p.group, gi = r % p.group;
-    *reinterpret_cast<uint2*>(p.out + (rows.first + tok) * p.out_stride + uint64_t{head * p.group + gi} * kD + 4 * e) =
-        make_uint2(dev::pack_f16x2(o.x / L, o.y / L), dev::pack_f16x2(o.z / L, o.w / L));
   }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) s_o[warp][lane * kPer + k] = o[k];
+  if (lane == 0) s_ml[warp] = make_float2(M, L);
+  __syncthreads();
+  const uint32_t e = threadIdx.x;
+  if (e >= kD) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kMergeWarps; ++k) M = fmaxf(M, s_ml[k].x);
+  float sum = 0.0f;
+  L = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kMergeWarps; ++k) {
+    const float a = M == -INFINITY ? 1.0f : exp2f(s_ml[k].x - M);
+    L = fmaf(s_ml[k].y, a, L);
+    sum = fmaf(s_o[k][e], a, sum);
+  }
+  if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros
+  const uint32_t tok = r / p.group, gi = r % p.group;
+  p.out[(rows.first + tok) * p.out_stride + uint64_t{head * p.group + gi} * kD + e] = __half_as_ushort(__float2half_rn(sum / L));
 }
 
-template <int kD, int kNB>
+template <int kD, bool kTwo>
 cudaError_t launch(const Params& p, cudaStream_t s) {
-  using C = Config<kD, kNB>;
-  const cudaError_t e = cudaFuncSetAttribute(stream_kernel<kD, kNB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  using C = Config<kD, kTwo>;
+  const cudaError_t e = cudaFuncSetAttribute(stream_kernel<kD, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              static_cast<int>(C::kSmem));
   if (e != cudaSuccess) return e;
-  stream_kernel<kD, kNB><<<p.ctas, C::kThreads, C::kSmem, s>>>(p);
+  stream_kernel<kD, kTwo><<<p.ctas, kThreads, C::kSmem, s>>>(p);
   const cudaError_t e2 = cudaGetLastError();
   if (e2 != cudaSuccess) return e2;
-  merge_kernel<kD><<<p.nseq * p.H, 128, 0, s>>>(p);
-  return cudaGetLastError();
+  // The merge's CTAs start while the stream's last ones run, and wait for them.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.nseq * p.H * p.slot_rows);
+  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, merge_kernel<kD>, p);
 }
 
 uint64_t prefix_bytes(uint32_t nseq) { return ((uint64_t{nseq} + 1) * 8 + 15) / 16 * 16; }
@@ -1316,8 +1401,8 @@ void stream_layout(Params* p, void* ws) {
 }
 
 cudaError_t launch_stream(uint32_t head_dim, const Params& p, cudaStream_t s) {
-  if (p.slot_rows <= 8) return head_dim == 64 ? launch<64, 1>(p, s) : launch<128, 1>(p, s);
-  return head_dim == 64 ? launch<64, 2>(p, s) : launch<128, 2>(p, s);
+  if (p.slot_rows <= 8) return head_dim == 64 ? launch<64, false>(p, s) : launch<128, false>(p, s);
+  return head_dim == 64 ? launch<64, true>(p, s) : launch<128, true>(p, s);
 }
 
 }  // namespace battn
