@@ -14,107 +14,6 @@ namespace hlkv {
 namespace battn {
 namespace {
 
-// kN consecutive elements of a row from element e, and the row's {scale, bias}: the codes' values
-// without the parameters.
-template <int kN>
-__device__ __forceinline__ void load_codes(uint32_t f, const uint8_t* payload, uint64_t elem, float (&x)[kN]) {
-  static_assert(kN == 2 || kN == 4);
-  if (f == dev::kFp16) {
-#pragma unroll
-    for (int i = 0; i < kN; i += 2) {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(payload + (elem + i) * 2));
-      x[i] = v.x;
-      x[i + 1] = v.y;
-    }
-  } else if (f == dev::kInt4) {
-#pragma unroll
-    for (int i = 0; i < kN; i += 2) {
-      const uint32_t w = payload[(elem + i) >> 1];
-      x[i] = static_cast<float>(w & 15u);
-      x[i + 1] = static_cast<float>(w >> 4);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kN; i += 2) {
-      const uint32_t w = *reinterpret_cast<const uint16_t*>(payload + elem + i);
-      const float2 v = f == dev::kE4M3 ? dev::fp8x2_exact<dev::kE4M3>(w) : dev::fp8x2_exact<dev::kE5M2>(w);
-      x[i] = v.x;
-      x[i + 1] = v.y;
-    }
-  }
-}
-
-__device__ __forceinline__ float2 row_params(uint32_t f, uint32_t info, uint32_t sref, const uint8_t* params, uint32_t row) {
-  if (f == dev::kFp16) return make_float2(1.0f, 0.0f);
-  const uint32_t mode = (info >> 4) & 3u;
-  if (mode != 0) return dev::block_params_value(mode, sref);
-  if (f == dev::kInt4) return __ldg(reinterpret_cast<const float2*>(params) + row);
-  return make_float2(__ldg(reinterpret_cast<const float*>(params) + row), 0.0f);
-}
-
-constexpr int kRowThreads = 128;
-
-// One warp per (new token, query head); lane l holds elements [l kN, (l + 1) kN) of the head.
-template <int kD>
-__global__ void __launch_bounds__(kRowThreads) batch_attention_rows(const Params p) {
-  constexpr int kN = kD / 32;
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t id = uint64_t{blockIdx.x} * (kRowThreads / 32) + (threadIdx.x >> 5);
-  const uint32_t token = static_cast<uint32_t>(id / p.q_heads), qh = static_cast<uint32_t>(id % p.q_heads), h = qh / p.group;
-  if (token >= p.token_first[p.nseq]) return;
-  uint32_t lo = 0, hi = p.nseq;  // the sequence with token_first[lo] <= token < token_first[lo + 1]
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (p.token_first[mid] <= token) lo = mid; else hi = mid;
-  }
-  const uint32_t q_len = p.token_first[lo + 1] - p.token_first[lo], ctx = p.context[lo];
-  if (uint64_t{q_len} * p.group <= kStreamRows) return;  // the stream kernel's
-  const int64_t pos = int64_t{ctx} - q_len + (token - p.token_first[lo]);
-
-  float q[kN], acc[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    q[i] = __half2float(__ushort_as_half(p.q[token * p.q_stride + uint64_t{qh} * kD + lane * kN + i])) * p.qscale;
-    acc[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  uint32_t first;
-  const uint32_t count = count_of(p, lo, &first);
-  for (uint32_t j = 0; j < count; ++j) {
-    const uint4 b = __ldg(p.blocks + first + j);
-    const uint32_t vt = min((b.y >> 10) & 0x3FFu, p.T);
-    const uint8_t* payload;
-    const uint32_t f = open_block(p, b, &payload);
-    if (f > 3) continue;
-    for (uint32_t i = 0; i < vt; ++i) {
-      const int64_t t = int64_t{b.w} + i;
-      if (t > pos || (p.window != 0 && pos - t >= p.window && t >= p.sinks)) continue;
-      float k[kN], v[kN];
-      const uint32_t krow = i * p.H + h, vrow = krow + p.T * p.H;
-      load_codes<kN>(f, payload, uint64_t{krow} * kD + lane * kN, k);
-      load_codes<kN>(f, payload, uint64_t{vrow} * kD + lane * kN, v);
-      const float2 kp = row_params(f, b.y, b.z, payload + p.code_bytes[f], krow);
-      const float2 vp = row_params(f, b.y, b.z, payload + p.code_bytes[f], vrow);
-      float x = 0.0f;
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x = fmaf(q[e], fmaf(k[e], kp.x, kp.y), x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-      const float mn = fmaxf(m, x);
-      const float a = mn == -INFINITY ? 1.0f : exp2f(m - mn), w = x == -INFINITY ? 0.0f : exp2f(x - mn);
-      l = fmaf(l, a, w);
-#pragma unroll
-      for (int e = 0; e < kN; ++e) acc[e] = fmaf(acc[e], a, w * fmaf(v[e], vp.x, vp.y));
-      m = mn;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < kN; ++e) {
-    const float r = m == -INFINITY && l == 0.0f ? 0.0f : acc[e] / l;
-    p.out[token * p.out_stride + uint64_t{qh} * kD + lane * kN + e] = __half_as_ushort(__float2half_rn(r));
-  }
-}
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
@@ -200,8 +99,5 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const cudaError_t e = launch_stream(layout->head_dim, p, s);
   if (e != cudaSuccess || p.max_rows <= kStreamRows) return cuda_status(e);
-  const unsigned grid = static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32));
-  if (D == 64) batch_attention_rows<64><<<grid, kRowThreads, 0, s>>>(p);
-  else batch_attention_rows<128><<<grid, kRowThreads, 0, s>>>(p);
-  return cuda_status(cudaGetLastError());
+  return cuda_status(launch_tiles(layout->head_dim, p, s));
 }

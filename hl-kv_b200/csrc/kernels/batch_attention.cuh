@@ -74,6 +74,69 @@ __device__ __forceinline__ uint32_t open_block(const Params& p, uint4 b, const u
   return f;
 }
 
+// ---- codes as binary16 ------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two FP8 codes in the low (or high) half of w -> their values as binary16.
+template <uint32_t kF>
+__device__ __forceinline__ uint32_t fp8_lo(uint32_t w) {
+  uint32_t h;
+  if constexpr (kF == dev::kE4M3) {
+    asm("{.reg .b16 l, u; mov.b32 {l, u}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(h) : "r"(w));
+  } else {
+    h = __byte_perm(w, 0u, 0x1404);  // an E5M2 code is the upper byte of its binary16 value
+  }
+  return h;
+}
+template <uint32_t kF>
+__device__ __forceinline__ uint32_t fp8_hi(uint32_t w) {
+  uint32_t h;
+  if constexpr (kF == dev::kE4M3) {
+    asm("{.reg .b16 l, u; mov.b32 {l, u}, %1; cvt.rn.f16x2.e4m3x2 %0, u;}" : "=r"(h) : "r"(w));
+  } else {
+    h = __byte_perm(w, 0u, 0x3424);
+  }
+  return h;
+}
+__device__ __forceinline__ bool has_nonfinite(uint32_t h2) {
+  return (h2 & 0x7C00u) == 0x7C00u || (h2 & 0x7C000000u) == 0x7C000000u;
+}
+
+// 1024 + c and 1024 + 16 c from masks -> (c - 8) / 8 by (1024 + c) / 8 - 129 and (1024 + 16 c) / 128 - 9: exact.
+// One logic operation holds one immediate, the mask; the other constant comes in a register.
+__device__ __forceinline__ uint32_t magic1024() {
+  uint32_t m;
+  asm("mov.b32 %0, 0x64006400;" : "=r"(m));
+  return m;
+}
+__device__ __forceinline__ uint32_t nibble_lo(uint32_t x, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(magic));
+  return hfma2(r, 0x30003000u, 0xD808D808u);
+}
+__device__ __forceinline__ uint32_t nibble_hi(uint32_t x, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(magic));
+  return hfma2(r, 0x20002000u, 0xC880C880u);
+}
+
+// 2^x by the hardware's approximation (2^-22 of the result; subnormal results are 0).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
 // ---- barriers in shared memory and bulk copies ------------------------------------------------
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -108,10 +171,100 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, uint64_t src, uint32_t b
                : "memory");
 }
 
+// ---- one row by one warp --------------------------------------------------------------------------
+// kN consecutive elements of a row from element e, and the row's {scale, bias}: the codes' values
+// without the parameters.
+template <int kN>
+__device__ __forceinline__ void load_codes(uint32_t f, const uint8_t* payload, uint64_t elem, float (&x)[kN]) {
+  static_assert(kN == 2 || kN == 4);
+  if (f == dev::kFp16) {
+#pragma unroll
+    for (int i = 0; i < kN; i += 2) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(payload + (elem + i) * 2));
+      x[i] = v.x;
+      x[i + 1] = v.y;
+    }
+  } else if (f == dev::kInt4) {
+#pragma unroll
+    for (int i = 0; i < kN; i += 2) {
+      const uint32_t w = payload[(elem + i) >> 1];
+      x[i] = static_cast<float>(w & 15u);
+      x[i + 1] = static_cast<float>(w >> 4);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN; i += 2) {
+      const uint32_t w = *reinterpret_cast<const uint16_t*>(payload + elem + i);
+      const float2 v = f == dev::kE4M3 ? dev::fp8x2_exact<dev::kE4M3>(w) : dev::fp8x2_exact<dev::kE5M2>(w);
+      x[i] = v.x;
+      x[i + 1] = v.y;
+    }
+  }
+}
+
+__device__ __forceinline__ float2 params_of_row(uint32_t f, uint32_t info, uint32_t sref, const uint8_t* params, uint32_t row) {
+  if (f == dev::kFp16) return make_float2(1.0f, 0.0f);
+  const uint32_t mode = (info >> 4) & 3u;
+  if (mode != 0) return dev::block_params_value(mode, sref);
+  if (f == dev::kInt4) return __ldg(reinterpret_cast<const float2*>(params) + row);
+  return make_float2(__ldg(reinterpret_cast<const float*>(params) + row), 0.0f);
+}
+
+// One row (new token of sequence i at position pos, query head qh) by one warp, token by token: lane l holds
+// elements [l kN, (l + 1) kN) of the head.
+template <int kD>
+__device__ __noinline__ void attend_row(const Params& p, uint32_t i, uint32_t token, int64_t pos, uint32_t qh) {
+  constexpr int kN = kD / 32;
+  const uint32_t lane = threadIdx.x & 31, h = qh / p.group;
+  float q[kN], acc[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    q[i] = __half2float(__ushort_as_half(p.q[token * p.q_stride + uint64_t{qh} * kD + lane * kN + i])) * p.qscale;
+    acc[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  uint32_t first;
+  const uint32_t count = count_of(p, i, &first);
+  for (uint32_t j = 0; j < count; ++j) {
+    const uint4 b = __ldg(p.blocks + first + j);
+    const uint32_t vt = min((b.y >> 10) & 0x3FFu, p.T);
+    const uint8_t* payload;
+    const uint32_t f = open_block(p, b, &payload);
+    if (f > 3) continue;
+    for (uint32_t k_tok = 0; k_tok < vt; ++k_tok) {
+      const int64_t t = int64_t{b.w} + k_tok;
+      if (t > pos || (p.window != 0 && pos - t >= p.window && t >= p.sinks)) continue;
+      float k[kN], v[kN];
+      const uint32_t krow = k_tok * p.H + h, vrow = krow + p.T * p.H;
+      load_codes<kN>(f, payload, uint64_t{krow} * kD + lane * kN, k);
+      load_codes<kN>(f, payload, uint64_t{vrow} * kD + lane * kN, v);
+      const float2 kp = params_of_row(f, b.y, b.z, payload + p.code_bytes[f], krow);
+      const float2 vp = params_of_row(f, b.y, b.z, payload + p.code_bytes[f], vrow);
+      float x = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x = fmaf(q[e], fmaf(k[e], kp.x, kp.y), x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+      const float mn = fmaxf(m, x);
+      const float a = mn == -INFINITY ? 1.0f : exp2f(m - mn), w = x == -INFINITY ? 0.0f : exp2f(x - mn);
+      l = fmaf(l, a, w);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) acc[e] = fmaf(acc[e], a, w * fmaf(v[e], vp.x, vp.y));
+      m = mn;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kN; ++e) {
+    const float r = m == -INFINITY && l == 0.0f ? 0.0f : acc[e] / l;
+    p.out[token * p.out_stride + uint64_t{qh} * kD + lane * kN + e] = __half_as_ushort(__float2half_rn(r));
+  }
+}
+
 // Launches of the kernels (their translation units).
 cudaError_t launch_stream(uint32_t head_dim, const Params& p, cudaStream_t s);
 size_t stream_workspace(uint32_t nseq, uint32_t H, uint32_t head_dim, uint32_t max_rows, uint32_t ctas);
 void stream_layout(Params* p, void* ws);
+cudaError_t launch_tiles(uint32_t head_dim, const Params& p, cudaStream_t s);
 
 }  // namespace battn
 }  // namespace hlkv

@@ -105,62 +105,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// Two FP8 codes in the low (or high) half of w -> their values as binary16.
-template <uint32_t kF>
-__device__ __forceinline__ uint32_t fp8_lo(uint32_t w) {
-  uint32_t h;
-  if constexpr (kF == dev::kE4M3) {
-    asm("{.reg .b16 l, u; mov.b32 {l, u}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(h) : "r"(w));
-  } else {
-    h = __byte_perm(w, 0u, 0x1404);  // an E5M2 code is the upper byte of its binary16 value
-  }
-  return h;
-}
-template <uint32_t kF>
-__device__ __forceinline__ uint32_t fp8_hi(uint32_t w) {
-  uint32_t h;
-  if constexpr (kF == dev::kE4M3) {
-    asm("{.reg .b16 l, u; mov.b32 {l, u}, %1; cvt.rn.f16x2.e4m3x2 %0, u;}" : "=r"(h) : "r"(w));
-  } else {
-    h = __byte_perm(w, 0u, 0x3424);
-  }
-  return h;
-}
-__device__ __forceinline__ bool has_nonfinite(uint32_t h2) {
-  return (h2 & 0x7C00u) == 0x7C00u || (h2 & 0x7C000000u) == 0x7C000000u;
-}
-
 // Row bytes of a format.
 template <int kD, uint32_t kF>
 constexpr uint32_t kRow = kF == dev::kFp16 ? kD * 2 : kF == dev::kInt4 ? kD / 2 : kD;
-
-// 1024 + c and 1024 + 16 c from masks -> (c - 8) / 8 by (1024 + c) / 8 - 129 and (1024 + 16 c) / 128 - 9: exact.
-// One logic operation holds one immediate, the mask; the other constant comes in a register.
-__device__ __forceinline__ uint32_t magic1024() {
-  uint32_t m;
-  asm("mov.b32 %0, 0x64006400;" : "=r"(m));
-  return m;
-}
-__device__ __forceinline__ uint32_t nibble_lo(uint32_t x, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(magic));
-  return hfma2(r, 0x30003000u, 0xD808D808u);
-}
-__device__ __forceinline__ uint32_t nibble_hi(uint32_t x, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(x), "r"(magic));
-  return hfma2(r, 0x20002000u, 0xC880C880u);
-}
 
 // Four pairs (j, j + 4) of the 8 elements at `w`, as binary16 (INT4: the code times 2^-24, binary16's
 // smallest step, so that masking a code is its conversion).
@@ -225,8 +172,6 @@ template <uint32_t kF>
 constexpr float kKeyUnit = kF == dev::kInt4 ? 0x1p24f : 1.0f;
 template <uint32_t kF>
 constexpr float kValueUnit = kF == dev::kFp16 ? 1.0f : kF == dev::kE4M3 ? 0x1p8f : kF == dev::kE5M2 ? 0x1p15f : 8.0f;
-
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // Loads by shared-memory address: 32 bits of address where a generic pointer takes 64.
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
@@ -323,13 +268,6 @@ __device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, 
   }
   s.E = kNoExponent;
   __syncwarp();
-}
-
-// 2^x by the hardware's approximation (2^-22 of the result; subnormal results are 0).
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
 }
 
 // {scale, bias} of the rows of tokens g and g + 8; `at` names the parameters' address in the description.

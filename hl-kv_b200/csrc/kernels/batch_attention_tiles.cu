@@ -1,0 +1,658 @@
+// Batch attention for many query rows (prompts and chunks of prompts): tiles on the fifth-generation tensor
+// cores.
+//
+// A row is a (new token, query head) pair of one (sequence, KV head); 4 D operations for each token it sees, so
+// the bound is the matrix rate, and next to it the exponentials (16 a clock and SM) and the conversion of codes.
+// A CTA takes 256 rows as two accumulator tiles of 128 and walks the sequence's visible tokens in tiles of
+// 128:
+//   S = Q K^T (tcgen05.mma, both operands in shared memory), a running softmax by one thread per row,
+//   O += P V (P from tensor memory, V from shared memory).
+// Eight warps convert the blocks' codes to binary16 in the 128-byte-swizzled layout, one tile ahead, once for both
+// accumulator tiles; the two tiles' softmax warpgroups alternate with the tensor cores: while one exponentiates,
+// the other's products run.  Tensor memory: S0, S1, O0, O1; P overwrites S.
+// As in the stream kernel a code's binary16 value is exact and its parameters stay outside: the K row's scale and
+// bias in the score, the V row's scale in the weight, its bias in a sum of its own, all in binary32.  A weight is
+// rounded once, to binary16, in units of 2^E that follow the exponents of the value scales (one for 16 tokens).
+// Codes are laid in the order (0, 4, 1, 5, 2, 6, 3, 7) of each 8, where the formats' words hold them: Q's elements
+// lie the same way, and the outputs are put back in order at the end.
+#include <cmath>
+
+#include "batch_attention.cuh"
+
+namespace hlkv {
+namespace battn {
+namespace {
+
+constexpr int kSoftmaxWarps = 8, kStageWarps = 8;
+constexpr int kThreads = (kSoftmaxWarps + kStageWarps + 4) * 32;  // and one that issues the products
+constexpr uint32_t kTile = 128;                                  // tokens of a tile
+constexpr uint32_t kRowsCta = 256;
+
+template <int kD>
+struct Config {
+  static constexpr uint32_t kPanels = kD / 64;               // 64 elements of a row make 128 bytes
+  static constexpr uint32_t kPanel = kTile * 128;            // bytes
+  static constexpr uint32_t kOperand = kPanels * kPanel;     // 128 rows of kD binary16 values
+  static constexpr uint32_t kQ = 0, kK = 2 * kOperand, kV = kK + 2 * kOperand, kEnd = kV + 2 * kOperand;
+  static constexpr uint32_t kSmem = kEnd + 1024;  // the operands start on 1024 bytes
+};
+
+struct Shared {
+  uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];  // of the two stages
+  uint64_t s_full[2], p_full[2], o_done[2];               // of the two accumulator tiles
+  // Of the tokens of the last four tiles: a K half may be written again while the softmax of the tile two before
+  // still reads these.
+  float ks[4][kTile], kb[4][kTile], vs[4][kTile], vb[4][kTile];
+  int exponent[4][kStageWarps];
+  uint32_t kind[4][kStageWarps];  // of 16 tokens: 1 a scale, 2 a bias, 4 some token does not exist
+  uint32_t exists[4][kStageWarps];
+  uint32_t tmem, redo;
+};
+
+// ---- tcgen05 ---------------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  // start address, leading and stride byte offsets in units of 16 bytes, version 1, 128-byte swizzle
+  return uint64_t{(addr >> 4) & 0x3FFFu} | uint64_t{lbo >> 4} << 16 | uint64_t{sbo >> 4} << 32 | uint64_t{1} << 46 | uint64_t{2} << 61;
+}
+// binary16 operands, binary32 accumulator, M = 128.
+constexpr uint32_t instruction(uint32_t n, bool b_transposed) {
+  return 1u << 4 | (b_transposed ? 1u << 16 : 0u) | n / 8 << 17 | 128u / 16 << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+               "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+               : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns of this warp's 32 rows: one row a lane.
+__device__ __forceinline__ void tmem_load32(uint32_t a, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+        "=r"(r[30]), "=r"(r[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t a, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t a, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Eight elements in one of the formats -> binary16 in the order (0, 4, 1, 5, 2, 6, 3, 7).  FP16 as it is; a K row's
+// FP8 codes as they are, a V row's E4M3 times 2^-8 and E5M2 times 2^-15; INT4 (code - 8) / 8.
+template <bool kValue>
+__device__ __forceinline__ uint4 convert(uint32_t f, uint4 raw) {
+  uint32_t a0, a1, a2, a3;
+  if (f == dev::kFp16) {
+    a0 = __byte_perm(raw.x, raw.z, 0x5410);
+    a1 = __byte_perm(raw.x, raw.z, 0x7632);
+    a2 = __byte_perm(raw.y, raw.w, 0x5410);
+    a3 = __byte_perm(raw.y, raw.w, 0x7632);
+  } else if (f == dev::kInt4) {
+    const uint32_t magic = magic1024(), y = raw.x >> 8;
+    a0 = nibble_lo(raw.x, magic);
+    a1 = nibble_hi(raw.x, magic);
+    a2 = nibble_lo(y, magic);
+    a3 = nibble_hi(y, magic);
+  } else {
+    const uint32_t x = __byte_perm(raw.x, raw.y, 0x5140), y = __byte_perm(raw.x, raw.y, 0x7362);
+    if (f == dev::kE4M3) {
+      a0 = fp8_lo<dev::kE4M3>(x);
+      a1 = fp8_hi<dev::kE4M3>(x);
+      a2 = fp8_lo<dev::kE4M3>(y);
+      a3 = fp8_hi<dev::kE4M3>(y);
+    } else {
+      a0 = fp8_lo<dev::kE5M2>(x);
+      a1 = fp8_hi<dev::kE5M2>(x);
+      a2 = fp8_lo<dev::kE5M2>(y);
+      a3 = fp8_hi<dev::kE5M2>(y);
+    }
+    if constexpr (kValue) {
+      const uint32_t down = f == dev::kE4M3 ? 0x1C001C00u : 0x02000200u;
+      a0 = hmul2(a0, down);
+      a1 = hmul2(a1, down);
+      a2 = hmul2(a2, down);
+      a3 = hmul2(a3, down);
+    }
+  }
+  return make_uint4(a0, a1, a2, a3);
+}
+
+// Shared-memory address of 16-byte chunk c (of kD / 8) of row r in an operand: panels of 64 elements, the chunk
+// index of a row's 128 bytes XORed with the row's place in its 8.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t base, uint32_t r, uint32_t c) {
+  return base + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// The tokens that a CTA's rows see, as positions: [0, a) and [b0, b1), walked in tiles of 128.
+struct Walk {
+  uint32_t a, b0, b1;
+  __device__ __forceinline__ uint32_t first_tiles() const { return (a + kTile - 1) / kTile; }
+  __device__ __forceinline__ uint32_t tiles() const { return first_tiles() + (b1 - b0 + kTile - 1) / kTile; }
+  __device__ __forceinline__ void tile(uint32_t j, uint32_t* pos, uint32_t* n) const {
+    const uint32_t fa = first_tiles();
+    if (j < fa) {
+      *pos = j * kTile;
+      *n = min(kTile, a - *pos);
+    } else {
+      *pos = b0 + (j - fa) * kTile;
+      *n = min(kTile, b1 - *pos);
+    }
+  }
+};
+
+template <int kD>
+__global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ Params p) {
+  using C = Config<kD>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared sh;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+
+  // ---- the CTA's rows: tiles of the longest contexts first
+  const uint32_t units = p.nseq * p.H, tiles_max = gridDim.x / units;
+  const uint32_t unit = blockIdx.x % units, seq = unit / p.H, h = unit % p.H;
+  const Rows rows = rows_of(p, seq);
+  const uint32_t n_rows = rows.q * p.group, row_tiles = (n_rows + kRowsCta - 1) / kRowsCta;
+  const uint32_t order = blockIdx.x / units;
+  if (n_rows <= kStreamRows || order >= row_tiles || tiles_max == 0) return;
+  const uint32_t row0 = (row_tiles - 1 - order) * kRowsCta, rows_here = min(kRowsCta, n_rows - row0);
+  const uint32_t n_acc = rows_here > 128 ? 2 : 1;
+  const uint32_t ctx = p.context[seq];
+  const int32_t pos_base = static_cast<int32_t>(ctx) - static_cast<int32_t>(rows.q);  // of the first new token
+  const int32_t p_lo = pos_base + static_cast<int32_t>(row0 / p.group), p_hi = pos_base + static_cast<int32_t>((row0 + rows_here - 1) / p.group);
+  Walk walk{0, 0, 0};
+  uint32_t first_block;
+  const uint32_t n_blocks = count_of(p, seq, &first_block);
+  if (p_hi >= 0 && n_blocks > 0) {
+    const uint32_t end = static_cast<uint32_t>(p_hi) + 1;
+    const int64_t low = p.window == 0 ? 0 : int64_t{p_lo} - p.window + 1;
+    if (low <= int64_t{p.sinks}) {
+      walk = Walk{0, 0, end};
+    } else {
+      walk = Walk{min(p.sinks, end), static_cast<uint32_t>(low), end};
+    }
+  }
+  const uint32_t n_tiles = walk.tiles();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.k_full[i], kStageWarps);
+      mbar_init(&sh.v_full[i], kStageWarps);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_done[i], 1);
+    }
+    sh.redo = 0;
+    mbar_fence_init();
+  }
+  if (warp == kSoftmaxWarps + kStageWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // ---- Q into its two operands, rows behind the last one zeros
+  for (uint32_t i = threadIdx.x; i < n_acc * 128 * (kD / 8); i += kThreads) {
+    const uint32_t c = i % (kD / 8), r = i / (kD / 8), row = row0 + r;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (r < rows_here) {
+      v = __ldg(reinterpret_cast<const uint4*>(p.q + (rows.first + row / p.group) * p.q_stride + uint64_t{h * p.group + row % p.group} * kD) + c);
+    }
+    v = convert<false>(dev::kFp16, v);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(base + C::kQ + (r >> 7) * C::kOperand, r & 127, c)), "r"(v.x), "r"(v.y),
+                 "r"(v.z), "r"(v.w)
+                 : "memory");
+  }
+  dev::fence_proxy_async_smem();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tmem;
+  bool ok = true;
+
+  if (warp < kSoftmaxWarps) {
+    // ================= softmax: one row a thread =================
+    const uint32_t acc = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = ((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + acc * 128, t_o = tmem + lanes + 256 + acc * kD;
+    const uint32_t row = row0 + acc * 128 + r;
+    const bool live = acc * 128 + r < rows_here;
+    const uint32_t tok = row / p.group, head = h * p.group + row % p.group;
+    const int32_t pos = pos_base + static_cast<int32_t>(tok);
+    // the first token of the window
+  const int32_t low = p.window == 0 ? -1 : static_cast<int32_t>(max(int64_t{pos} - p.window + 1, int64_t{-1}));
+    float qsum = 0.0f;
+    if (live) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (rows.first + tok) * p.q_stride + uint64_t{head} * kD);
+      for (int i = 0; i < kD / 8; ++i) {
+        const uint4 w = __ldg(src + i);
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[k]));
+          qsum += f.x + f.y;
+        }
+      }
+    }
+    qsum *= p.qscale;
+    float m = -INFINITY, l = 0.0f, bias = 0.0f;
+    int E = 0;
+    if (acc < n_acc) {
+      for (uint32_t j = 0; j < n_tiles; ++j) {
+        const uint32_t info = j & 3;
+        uint32_t tp, n;
+        walk.tile(j, &tp, &n);
+        ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&sh.s_full[acc], j & 1));
+        if (!ok) break;
+        fence_after();
+        // Whether all 128 rows see all 128 tokens.
+        const int32_t t0 = static_cast<int32_t>(tp), acc_lo = pos_base + static_cast<int32_t>((row0 + acc * 128) / p.group);
+        uint32_t any_kind = 0;
+        int e_tile = -1000;
+#pragma unroll
+        for (int g = 0; g < kStageWarps; ++g) {
+          any_kind |= sh.kind[info][g];
+          e_tile = max(e_tile, sh.exponent[info][g]);
+        }
+        const bool masked = n < kTile || (any_kind & 4u) != 0 || t0 + 127 > acc_lo ||
+                            (p.window != 0 && t0 + 128 > static_cast<int32_t>(min(p.sinks, 0x7FFFFF00u)) &&
+                             p_hi - t0 >= static_cast<int32_t>(min(p.window, 0x7FFFFFFFu)));
+        // ---- scores of 32 tokens from tensor memory
+        auto scores = [&](uint32_t c, float (&x)[32]) {
+          uint32_t raw[32];
+          tmem_load32(t_s + c * 32, raw);
+          wait_ld();
+          const uint32_t kind = sh.kind[info][2 * c] | sh.kind[info][2 * c + 1];
+          if (kind & 3u) {
+            const float4* ks = reinterpret_cast<const float4*>(&sh.ks[info][c * 32]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 k = ks[i];
+              x[4 * i] = __uint_as_float(raw[4 * i]) * k.x;
+              x[4 * i + 1] = __uint_as_float(raw[4 * i + 1]) * k.y;
+              x[4 * i + 2] = __uint_as_float(raw[4 * i + 2]) * k.z;
+              x[4 * i + 3] = __uint_as_float(raw[4 * i + 3]) * k.w;
+            }
+            if (kind & 2u) {
+              const float4* kb = reinterpret_cast<const float4*>(&sh.kb[info][c * 32]);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 k = kb[i];
+                x[4 * i] = fmaf(k.x, qsum, x[4 * i]);
+                x[4 * i + 1] = fmaf(k.y, qsum, x[4 * i + 1]);
+                x[4 * i + 2] = fmaf(k.z, qsum, x[4 * i + 2]);
+                x[4 * i + 3] = fmaf(k.w, qsum, x[4 * i + 3]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(raw[i]) * p.qscale;
+          }
+          if (masked) {
+            const uint32_t exists = sh.exists[info][2 * c] | sh.exists[info][2 * c + 1] << 16;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int32_t t = t0 + static_cast<int32_t>(c) * 32 + i;
+              const bool see = t <= pos && (t >= low || static_cast<uint32_t>(t) < p.sinks) && (exists >> i & 1u);
+              x[i] = see ? x[i] : -INFINITY;
+            }
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (uint32_t c = 0; c < 4; ++c) {
+          float x[32];
+          scores(c, x);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
+        }
+        // ---- the reference maximum and the accumulator's unit
+        const int e_new = min(max(e_tile, -60), 60);
+        const bool shift = j == 0 || (e_tile != -1000 && (e_new > E + 6 || e_new < E - 6));
+        const bool grow = top > m + 8.0f;
+        if (__any_sync(0xFFFFFFFFu, grow) || shift) {
+          const float mn = grow ? fmaxf(m, top) : m;
+          const float a = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+          m = mn;
+          l *= a;
+          bias *= a;
+          const int e_to = shift ? (e_tile == -1000 ? 0 : e_new) : E;
+          if (j > 0) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh.o_done[acc], (j - 1) & 1));
+            if (!ok) break;
+            fence_after();
+            const float f = a * exp2f(static_cast<float>(E - e_to));
+#pragma unroll 1
+            for (uint32_t c = 0; c < kD / 32; ++c) {
+              uint32_t o[32];
+              tmem_load32(t_o + c * 32, o);
+              wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_store32(t_o + c * 32, o);
+            }
+          }
+          E = e_to;
+        }
+        // ---- weights
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+        for (uint32_t c = 0; c < 4; ++c) {
+          float x[32];
+          scores(c, x);
+          uint32_t w[16];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t g = 2 * c + half, kind = sh.kind[info][g];
+            // the group's weights are in units of 2^(its exponent), the sums in their own
+            const int de = min(max(sh.exponent[info][g], -60), 60) - E;
+            const float from = ref - static_cast<float>(kind & 3u ? de : -E), back = exp2f(static_cast<float>(kind & 3u ? -de : E));
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              x[16 * half + i] = ex2(x[16 * half + i] - from);
+              sum += x[16 * half + i];
+            }
+            l = fmaf(sum, back, l);
+            if (kind & 2u) {
+              const float4* vb = reinterpret_cast<const float4*>(&sh.vb[info][g * 16]);
+              float b = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float4 v = vb[i];
+                b = fmaf(x[16 * half + 4 * i], v.x, b);
+                b = fmaf(x[16 * half + 4 * i + 1], v.y, b);
+                b = fmaf(x[16 * half + 4 * i + 2], v.z, b);
+                b = fmaf(x[16 * half + 4 * i + 3], v.w, b);
+              }
+              bias = fmaf(b, back, bias);
+            }
+            if (kind & 3u) {
+              const float4* vs = reinterpret_cast<const float4*>(&sh.vs[info][g * 16]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float4 v = vs[i];
+                w[8 * half + 2 * i] = dev::pack_f16x2(x[16 * half + 4 * i] * v.x, x[16 * half + 4 * i + 1] * v.y);
+                w[8 * half + 2 * i + 1] = dev::pack_f16x2(x[16 * half + 4 * i + 2] * v.z, x[16 * half + 4 * i + 3] * v.w);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[8 * half + i] = dev::pack_f16x2(x[16 * half + 2 * i], x[16 * half + 2 * i + 1]);
+            }
+          }
+          tmem_store16(t_s + c * 16, w);
+        }
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[acc]);
+      }
+      // ---- the rows' results
+      if (ok && n_tiles > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh.o_done[acc], (n_tiles - 1) & 1));
+      if (ok) {
+        fence_after();
+        const float unit = exp2f(static_cast<float>(E));
+        const bool none = m == -INFINITY && l == 0.0f;
+#pragma unroll 1
+        for (uint32_t c = 0; c < kD / 32; ++c) {
+          uint32_t o[32];
+          if (n_tiles > 0) {
+            tmem_load32(t_o + c * 32, o);
+            wait_ld();
+          }
+          __syncwarp();
+          uint4* dst = reinterpret_cast<uint4*>(p.out + (rows.first + tok) * p.out_stride + uint64_t{head} * kD + c * 32);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              // elements 2 i and 2 i + 1 of the 8 lie at 0 4 1 5 2 6 3 7
+              const int e0 = 8 * k + (i < 2 ? 4 * i : 4 * (i - 2) + 1), e1 = e0 + 2;
+              const float a = none ? 0.0f : fmaf(__uint_as_float(o[e0]), unit, bias) / l, b = none ? 0.0f : fmaf(__uint_as_float(o[e1]), unit, bias) / l;
+              y[i] = dev::pack_f16x2(a, b);
+            }
+            if (live) dst[k] = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+      }
+      fence_before();
+    }
+  } else if (warp < kSoftmaxWarps + kStageWarps) {
+    // ================= conversion: 16 tokens of a tile per warp =================
+    const uint32_t sw = warp - kSoftmaxWarps;
+    const uint4* blocks = p.blocks + first_block;
+    uint32_t cur = 0, cur_start = 0;  // the block of this warp's first token in the tile before, and its first position
+    bool searched = false;
+    for (uint32_t j = 0; j < n_tiles; ++j) {
+      const uint32_t stage = j & 1;
+      uint32_t tp, n;
+      walk.tile(j, &tp, &n);
+      // ---- this lane's token (lanes 16 to 31 repeat 0 to 15): its block, by the listed starts
+      const uint32_t i = sw * 16 + (lane & 15);
+      const uint32_t t = tp + i, mine0 = tp + sw * 16;
+      if (!searched || j == walk.first_tiles()) {
+        // the last block that starts at or before mine0 (or block 0)
+        uint32_t a = 0, b = n_blocks;
+        while (b - a > 1) {
+          const uint32_t step = (b - a + 31) / 32, k = a + lane * step;
+          const bool hit = k < b && __ldg(&blocks[k].w) <= mine0;
+          const uint32_t hits = __popc(__ballot_sync(0xFFFFFFFFu, hit));  // lane 0 counts as one
+          const uint32_t at = a + (hits > 0 ? hits - 1 : 0u) * step;
+          b = min(at + step, b);
+          a = at;
+        }
+        cur = a;
+        cur_start = n_blocks ? __ldg(&blocks[a].w) : 0u;
+        searched = true;
+      }
+      uint32_t f = 4, info = 0, sref = 0, r = 0;
+      const uint8_t* payload = nullptr;
+      if (i < n) {
+        // a block holds at most T tokens, so the token's is at least this far on
+        uint32_t k = cur + (t > cur_start ? (t - cur_start) / p.T : 0u);
+        for (; k < n_blocks; ++k) {
+          const uint4 blk = __ldg(blocks + k);
+          const uint32_t v = min((blk.y >> 10) & 0x3FFu, p.T);
+          if (t < blk.w) break;  // not listed
+          if (t - blk.w < v) {
+            f = open_block(p, blk, &payload);
+            info = blk.y;
+            sref = blk.z;
+            r = t - blk.w;
+            break;
+          }
+        }
+        if ((lane & 15) == 0 && k < n_blocks) {
+          cur = k;
+          cur_start = __ldg(&blocks[k].w);
+        }
+      }
+      cur = __shfl_sync(0xFFFFFFFFu, cur, 0);
+      cur_start = __shfl_sync(0xFFFFFFFFu, cur_start, 0);
+      const uint32_t krow = r * p.H + h, vrow = krow + p.T * p.H;
+      float2 kp = make_float2(1.0f, 0.0f), vp = make_float2(1.0f, 0.0f);
+      if (f <= 3) {
+        kp = params_of_row(f, info, sref, payload + p.code_bytes[f], krow);
+        vp = params_of_row(f, info, sref, payload + p.code_bytes[f], vrow);
+      }
+      const uint32_t kinds = __reduce_or_sync(0xFFFFFFFFu, f > 3 ? 4u : f == dev::kInt4 ? 3u : f == dev::kFp16 ? 0u : 1u);
+      const bool scaled = (kinds & 3u) != 0;
+      const uint32_t exists = __ballot_sync(0xFFFFFFFFu, f <= 3) & 0xFFFFu;
+      const float unit = f == dev::kFp16 ? 1.0f : f == dev::kE4M3 ? 0x1p8f : f == dev::kE5M2 ? 0x1p15f : 8.0f;
+      const float u = f > 3 ? 0.0f : vp.x * unit;
+      const uint32_t ub = __float_as_uint(u) & 0x7FFFFFFFu;
+      const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, ub < 0x7F800000u ? ub : 0u);
+      const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, f > 3 ? 0xFFFFFFFFu : ub);
+      const int e = min(max(static_cast<int>(top >> 23) - 127, -60), 60);
+      // A tile that some row sees in part: values that are not finite, or scales far apart, would touch rows that
+      // do not see them.  Such a CTA's rows are done over, one by one.
+      const int32_t t0 = static_cast<int32_t>(tp);
+      const bool part = n < kTile || t0 + 127 > p_lo ||
+                        (p.window != 0 && t0 + 128 > static_cast<int32_t>(min(p.sinks, 0x7FFFFF00u)) &&
+                         p_hi - t0 >= static_cast<int32_t>(min(p.window, 0x7FFFFFFFu)));
+      bool bad = part && f <= 3 && (ub >= 0x7F800000u || (low != 0xFFFFFFFFu && top > low + (10u << 23)) || !dev::finite_f32(vp.y));
+
+      // ---- K, then V
+#pragma unroll 1
+      for (uint32_t half = 0; half < 2; ++half) {
+        if (j >= 2) {
+          ok = ok && mbar_wait(half ? &sh.v_empty[stage] : &sh.k_empty[stage], (j / 2 - 1) & 1);
+          if (!ok) break;
+        }
+        if (lane < 16) {
+          if (half == 0) {
+            const uint32_t info_i = j & 3;
+            sh.ks[info_i][i] = f > 3 ? 0.0f : kp.x * (p.qscale * (f == dev::kInt4 ? 8.0f : 1.0f));
+            sh.kb[info_i][i] = f == dev::kInt4 ? fmaf(8.0f, kp.x, kp.y) : 0.0f;
+            sh.vs[info_i][i] = scaled ? u * pow2(-e) : 1.0f;
+            sh.vb[info_i][i] = f == dev::kInt4 ? fmaf(8.0f, vp.x, vp.y) : 0.0f;
+            if (lane == 0) {
+              sh.kind[info_i][sw] = kinds;
+              sh.exists[info_i][sw] = exists;
+              sh.exponent[info_i][sw] = scaled ? (top ? e : -1000) : 0;
+            }
+          }
+        }
+        const uint32_t row = half ? vrow : krow;
+        const uint64_t src = reinterpret_cast<uint64_t>(payload) + uint64_t{row} * (f == dev::kFp16 ? kD * 2 : f == dev::kInt4 ? kD / 2 : kD);
+        constexpr uint32_t kChunks = kD / 8, kRowsIter = 32 / kChunks, kIters = 16 / kRowsIter;  // 16 or 8 chunks a row
+        const uint32_t c = lane % kChunks, sub = lane / kChunks;
+        const uint32_t operand = base + (half ? C::kV : C::kK) + stage * C::kOperand;
+        constexpr uint32_t kBatch = kIters < 4 ? kIters : 4;
+#pragma unroll 1
+        for (uint32_t it0 = 0; it0 < kIters; it0 += kBatch) {
+          uint4 raw[kBatch];
+          uint32_t fr[kBatch];
+#pragma unroll
+          for (uint32_t it = 0; it < kBatch; ++it) {
+            const uint32_t from = (it0 + it) * kRowsIter + sub;
+            const uint64_t a = __shfl_sync(0xFFFFFFFFu, src, from);
+            fr[it] = __shfl_sync(0xFFFFFFFFu, f, from);
+            raw[it] = make_uint4(0u, 0u, 0u, 0u);
+            if (fr[it] == dev::kFp16) raw[it] = __ldg(reinterpret_cast<const uint4*>(a) + c);
+            else if (fr[it] == dev::kInt4) raw[it].x = __ldg(reinterpret_cast<const uint32_t*>(a) + c);
+            else if (fr[it] < 4) {
+              const uint2 w = __ldg(reinterpret_cast<const uint2*>(a) + c);
+              raw[it].x = w.x;
+              raw[it].y = w.y;
+            }
+          }
+#pragma unroll
+          for (uint32_t it = 0; it < kBatch; ++it) {
+            const uint32_t to = sw * 16 + (it0 + it) * kRowsIter + sub;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (fr[it] < 4) v = half ? convert<true>(fr[it], raw[it]) : convert<false>(fr[it], raw[it]);
+            if (half && part) bad = bad || has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(operand, to, c)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                         : "memory");
+          }
+        }
+        dev::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(half ? &sh.v_full[stage] : &sh.k_full[stage]);
+      }
+      if (bad) sh.redo = 1;
+      if (!ok) break;
+    }
+  } else if (warp == kSoftmaxWarps + kStageWarps) {
+    // ================= products: one thread =================
+    if (lane == 0 && n_tiles > 0) {
+      constexpr uint32_t kIdS = instruction(kTile, false), kIdO = instruction(kD, true);
+      auto scores = [&](uint32_t acc, uint32_t j) {
+        const uint32_t q = base + C::kQ + acc * C::kOperand, k = base + C::kK + (j & 1) * C::kOperand;
+#pragma unroll
+        for (uint32_t s = 0; s < kD / 16; ++s) {
+          const uint32_t at = (s / 4) * C::kPanel + (s % 4) * 32;
+          mma_ss(tmem + acc * 128, desc(q + at, 16, 1024), desc(k + at, 16, 1024), kIdS, s > 0);
+        }
+        commit(&sh.s_full[acc]);
+      };
+      ok = mbar_wait(&sh.k_full[0], 0);
+      fence_after();
+      for (uint32_t acc = 0; acc < n_acc && ok; ++acc) scores(acc, 0);
+      if (ok) commit(&sh.k_empty[0]);
+      for (uint32_t j = 0; j < n_tiles && ok; ++j) {
+        for (uint32_t acc = 0; acc < n_acc && ok; ++acc) {
+          ok = mbar_wait(&sh.p_full[acc], j & 1) && (acc > 0 || mbar_wait(&sh.v_full[j & 1], (j >> 1) & 1));
+          if (!ok) break;
+          fence_after();
+          const uint32_t v = base + C::kV + (j & 1) * C::kOperand;
+#pragma unroll
+          for (uint32_t s = 0; s < kTile / 16; ++s) {
+            mma_ts(tmem + 256 + acc * kD, tmem + acc * 128 + s * 8, desc(v + s * 2048, C::kPanel, 1024), kIdO, j > 0 || s > 0);
+          }
+          commit(&sh.o_done[acc]);
+          if (j + 1 < n_tiles) {
+            if (acc == 0) ok = mbar_wait(&sh.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
+            if (!ok) break;
+            fence_after();
+            scores(acc, j + 1);
+          }
+        }
+        if (!ok) break;
+        commit(&sh.v_empty[j & 1]);
+        if (j + 1 < n_tiles) commit(&sh.k_empty[(j + 1) & 1]);
+      }
+    }
+    __syncwarp();
+  }
+  if (!ok && lane == 0) atomicOr(p.err, dev::kErrInternal);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == kSoftmaxWarps + kStageWarps) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+  if (sh.redo) {
+    for (uint32_t r = warp; r < rows_here; r += kThreads / 32) {
+      const uint32_t row = row0 + r, tok = row / p.group;
+      attend_row<kD>(p, seq, rows.first + tok, int64_t{pos_base} + tok, h * p.group + row % p.group);
+    }
+  }
+}
+
+template <int kD>
+cudaError_t launch(const Params& p, cudaStream_t s) {
+  const cudaError_t e = cudaFuncSetAttribute(tile_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Config<kD>::kSmem));
+  if (e != cudaSuccess) return e;
+  const uint64_t grid = uint64_t{p.nseq} * p.H * ((uint64_t{p.max_rows} + kRowsCta - 1) / kRowsCta);
+  if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+  tile_kernel<kD><<<static_cast<unsigned>(grid), kThreads, Config<kD>::kSmem, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_tiles(uint32_t head_dim, const Params& p, cudaStream_t s) {
+  return head_dim == 64 ? launch<64>(p, s) : launch<128>(p, s);
+}
+
+}  // namespace battn
+}  // namespace hlkv
