@@ -103,6 +103,41 @@ __device__ __forceinline__ void tmem_store32(uint32_t a, const uint32_t (&r)[32]
       : "memory");
 }
 
+// Two binary32 operations in one instruction.
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ Pair pair(uint32_t x, uint32_t y) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "r"(x), "r"(y));
+  return r;
+}
+__device__ __forceinline__ float2 split(Pair a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 // Eight elements in one of the formats -> binary16 in the order (0, 4, 1, 5, 2, 6, 3, 7).  FP16 as it is; a K row's
 // FP8 codes as they are, a V row's E4M3 times 2^-8 and E5M2 times 2^-15; INT4 (code - 8) / 8.
 template <bool kValue>
@@ -283,54 +318,54 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         const bool masked = n < kTile || (any_kind & 4u) != 0 || t0 + 127 > acc_lo ||
                             (p.window != 0 && t0 + 128 > static_cast<int32_t>(min(p.sinks, 0x7FFFFF00u)) &&
                              p_hi - t0 >= static_cast<int32_t>(min(p.window, 0x7FFFFFFFu)));
-        // ---- scores of 32 tokens from tensor memory
-        auto scores = [&](uint32_t c, float (&x)[32]) {
+        // ---- scores of 32 tokens from tensor memory, in pairs: S ks (+ kb sum(q)) + add
+        const Pair q2 = pair(qsum, qsum), scale2 = pair(p.qscale, p.qscale);
+        auto scores = [&](uint32_t c, Pair add0, Pair add1, Pair (&x)[16]) {
           uint32_t raw[32];
           tmem_load32(t_s + c * 32, raw);
           wait_ld();
           const uint32_t kind = sh.kind[info][2 * c] | sh.kind[info][2 * c + 1];
           if (kind & 3u) {
-            const float4* ks = reinterpret_cast<const float4*>(&sh.ks[info][c * 32]);
+            const float4 *ks = reinterpret_cast<const float4*>(&sh.ks[info][c * 32]), *kb = reinterpret_cast<const float4*>(&sh.kb[info][c * 32]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float4 k = ks[i];
-              x[4 * i] = __uint_as_float(raw[4 * i]) * k.x;
-              x[4 * i + 1] = __uint_as_float(raw[4 * i + 1]) * k.y;
-              x[4 * i + 2] = __uint_as_float(raw[4 * i + 2]) * k.z;
-              x[4 * i + 3] = __uint_as_float(raw[4 * i + 3]) * k.w;
-            }
-            if (kind & 2u) {
-              const float4* kb = reinterpret_cast<const float4*>(&sh.kb[info][c * 32]);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 k = kb[i];
-                x[4 * i] = fmaf(k.x, qsum, x[4 * i]);
-                x[4 * i + 1] = fmaf(k.y, qsum, x[4 * i + 1]);
-                x[4 * i + 2] = fmaf(k.z, qsum, x[4 * i + 2]);
-                x[4 * i + 3] = fmaf(k.w, qsum, x[4 * i + 3]);
+              Pair a0 = i < 4 ? add0 : add1, a1 = a0;
+              if (kind & 2u) {
+                const float4 b = kb[i];
+                a0 = fma2(pair(b.x, b.y), q2, a0);
+                a1 = fma2(pair(b.z, b.w), q2, a1);
               }
+              const float4 k = ks[i];
+              x[2 * i] = fma2(pair(raw[4 * i], raw[4 * i + 1]), pair(k.x, k.y), a0);
+              x[2 * i + 1] = fma2(pair(raw[4 * i + 2], raw[4 * i + 3]), pair(k.z, k.w), a1);
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(raw[i]) * p.qscale;
+            for (int i = 0; i < 16; ++i) x[i] = fma2(pair(raw[2 * i], raw[2 * i + 1]), scale2, i < 8 ? add0 : add1);
           }
           if (masked) {
             const uint32_t exists = sh.exists[info][2 * c] | sh.exists[info][2 * c + 1] << 16;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int32_t t = t0 + static_cast<int32_t>(c) * 32 + i;
-              const bool see = t <= pos && (t >= low || static_cast<uint32_t>(t) < p.sinks) && (exists >> i & 1u);
-              x[i] = see ? x[i] : -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+              const int32_t t = t0 + static_cast<int32_t>(c) * 32 + 2 * i;
+              const bool see0 = t <= pos && (t >= low || static_cast<uint32_t>(t) < p.sinks) && (exists >> (2 * i) & 1u);
+              const bool see1 = t + 1 <= pos && (t + 1 >= low || static_cast<uint32_t>(t) + 1 < p.sinks) && (exists >> (2 * i + 1) & 1u);
+              const float2 v = split(x[i]);
+              x[i] = pair(see0 ? v.x : -INFINITY, see1 ? v.y : -INFINITY);
             }
           }
         };
+        const Pair zero = pair(0.0f, 0.0f);
         float top = -INFINITY;
 #pragma unroll 1
         for (uint32_t c = 0; c < 4; ++c) {
-          float x[32];
-          scores(c, x);
+          Pair x[16];
+          scores(c, zero, zero, x);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
+          for (int i = 0; i < 16; ++i) {
+            const float2 v = split(x[i]);
+            top = fmaxf(top, fmaxf(v.x, v.y));
+          }
         }
         // ---- the reference maximum and the accumulator's unit
         const int e_new = min(max(e_tile, -60), 60);
@@ -364,47 +399,53 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
         for (uint32_t c = 0; c < 4; ++c) {
-          float x[32];
-          scores(c, x);
+          // a group's weights are in units of 2^(its exponent), the sums in their own
+          const uint32_t kind0 = sh.kind[info][2 * c], kind1 = sh.kind[info][2 * c + 1];
+          const int d0 = (kind0 & 3u ? min(max(sh.exponent[info][2 * c], -60), 60) : 0) - E;
+          const int d1 = (kind1 & 3u ? min(max(sh.exponent[info][2 * c + 1], -60), 60) : 0) - E;
+          const float add0 = static_cast<float>(d0) - ref, add1 = static_cast<float>(d1) - ref;
+          Pair x[16];
+          scores(c, pair(add0, add0), pair(add1, add1), x);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 v = split(x[i]);
+            x[i] = pair(ex2(v.x), ex2(v.y));
+          }
+          Pair s0 = x[0], s1 = x[8];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) {
+            s0 = add2(s0, x[i]);
+            s1 = add2(s1, x[8 + i]);
+          }
+          const float2 l0 = split(s0), l1 = split(s1);
+          const float back0 = pow2(-d0), back1 = pow2(-d1);
+          l = fmaf(l0.x + l0.y, back0, fmaf(l1.x + l1.y, back1, l));
+          if ((kind0 | kind1) & 2u) {
+            const float4* vb = reinterpret_cast<const float4*>(&sh.vb[info][c * 32]);
+            Pair b0 = zero, b1 = zero;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 u = vb[i], v = vb[4 + i];
+              b0 = fma2(x[2 * i + 1], pair(u.z, u.w), fma2(x[2 * i], pair(u.x, u.y), b0));
+              b1 = fma2(x[2 * i + 9], pair(v.z, v.w), fma2(x[2 * i + 8], pair(v.x, v.y), b1));
+            }
+            const float2 y0 = split(b0), y1 = split(b1);
+            bias = fmaf(y0.x + y0.y, back0, fmaf(y1.x + y1.y, back1, bias));
+          }
           uint32_t w[16];
+          if ((kind0 | kind1) & 3u) {
+            const float4* vs = reinterpret_cast<const float4*>(&sh.vs[info][c * 32]);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t g = 2 * c + half, kind = sh.kind[info][g];
-            // the group's weights are in units of 2^(its exponent), the sums in their own
-            const int de = min(max(sh.exponent[info][g], -60), 60) - E;
-            const float from = ref - static_cast<float>(kind & 3u ? de : -E), back = exp2f(static_cast<float>(kind & 3u ? -de : E));
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              x[16 * half + i] = ex2(x[16 * half + i] - from);
-              sum += x[16 * half + i];
+            for (int i = 0; i < 8; ++i) {
+              const float4 v = vs[i];
+              x[2 * i] = mul2(x[2 * i], pair(v.x, v.y));
+              x[2 * i + 1] = mul2(x[2 * i + 1], pair(v.z, v.w));
             }
-            l = fmaf(sum, back, l);
-            if (kind & 2u) {
-              const float4* vb = reinterpret_cast<const float4*>(&sh.vb[info][g * 16]);
-              float b = 0.0f;
+          }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float4 v = vb[i];
-                b = fmaf(x[16 * half + 4 * i], v.x, b);
-                b = fmaf(x[16 * half + 4 * i + 1], v.y, b);
-                b = fmaf(x[16 * half + 4 * i + 2], v.z, b);
-                b = fmaf(x[16 * half + 4 * i + 3], v.w, b);
-              }
-              bias = fmaf(b, back, bias);
-            }
-            if (kind & 3u) {
-              const float4* vs = reinterpret_cast<const float4*>(&sh.vs[info][g * 16]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float4 v = vs[i];
-                w[8 * half + 2 * i] = dev::pack_f16x2(x[16 * half + 4 * i] * v.x, x[16 * half + 4 * i + 1] * v.y);
-                w[8 * half + 2 * i + 1] = dev::pack_f16x2(x[16 * half + 4 * i + 2] * v.z, x[16 * half + 4 * i + 3] * v.w);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) w[8 * half + i] = dev::pack_f16x2(x[16 * half + 2 * i], x[16 * half + 2 * i + 1]);
-            }
+          for (int i = 0; i < 16; ++i) {
+            const float2 v = split(x[i]);
+            w[i] = dev::pack_f16x2(v.x, v.y);
           }
           tmem_store16(t_s + c * 16, w);
         }
@@ -446,67 +487,132 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     }
   } else if (warp < kSoftmaxWarps + kStageWarps) {
     // ================= conversion: 16 tokens of a tile per warp =================
+    // A pipeline of batches of rows: the loads of a batch are issued before the one before it is converted, and the
+    // next tile's blocks are looked up while this one's rows are.
     const uint32_t sw = warp - kSoftmaxWarps;
     const uint4* blocks = p.blocks + first_block;
-    uint32_t cur = 0, cur_start = 0;  // the block of this warp's first token in the tile before, and its first position
-    bool searched = false;
-    for (uint32_t j = 0; j < n_tiles; ++j) {
-      const uint32_t stage = j & 1;
+    constexpr uint32_t kChunks = kD / 8, kRowsIter = 32 / kChunks, kIters = 16 / kRowsIter;  // 16-byte pieces of an operand's row
+    constexpr uint32_t kBatch = 4, kBatches = kIters / kBatch;                               // of a half: 2 or 1
+    const uint32_t chunk = lane % kChunks, sub = lane / kChunks;
+
+    // A lane's token of a tile (lanes 16 to 31 repeat 0 to 15).
+    struct Token {
+      uint64_t k;     // address of its K row
+      uint32_t f;     // 4: it does not exist
+      float2 kp, vp;  // its rows' {scale, bias}
+    };
+    uint32_t cur = 0, cur_start = 0;  // a block at or before this warp's next first token, and its first position
+    uint32_t at_k = 0;                // the block that `entry` is
+    uint4 entry = make_uint4(0u, 0u, 0u, 0u);
+    auto position = [&](uint32_t j, uint32_t* t) {
       uint32_t tp, n;
       walk.tile(j, &tp, &n);
-      // ---- this lane's token (lanes 16 to 31 repeat 0 to 15): its block, by the listed starts
       const uint32_t i = sw * 16 + (lane & 15);
-      const uint32_t t = tp + i, mine0 = tp + sw * 16;
-      if (!searched || j == walk.first_tiles()) {
-        // the last block that starts at or before mine0 (or block 0)
+      *t = tp + i;
+      return i < n;
+    };
+    // First half of the lookup for tile j: the block that holds the token if those since `cur` are full.
+    auto look = [&](uint32_t j) {
+      uint32_t t;
+      const bool in = position(j, &t);
+      if (j == 0 || j == walk.first_tiles()) {  // a run begins: the last block that starts at or before the first token
+        const uint32_t first = __shfl_sync(0xFFFFFFFFu, t, 0);
         uint32_t a = 0, b = n_blocks;
         while (b - a > 1) {
           const uint32_t step = (b - a + 31) / 32, k = a + lane * step;
-          const bool hit = k < b && __ldg(&blocks[k].w) <= mine0;
-          const uint32_t hits = __popc(__ballot_sync(0xFFFFFFFFu, hit));  // lane 0 counts as one
+          const uint32_t hits = __popc(__ballot_sync(0xFFFFFFFFu, k < b && __ldg(&blocks[k].w) <= first));
           const uint32_t at = a + (hits > 0 ? hits - 1 : 0u) * step;
           b = min(at + step, b);
           a = at;
         }
         cur = a;
-        cur_start = n_blocks ? __ldg(&blocks[a].w) : 0u;
-        searched = true;
+        cur_start = __ldg(&blocks[a].w);
       }
-      uint32_t f = 4, info = 0, sref = 0, r = 0;
-      const uint8_t* payload = nullptr;
-      if (i < n) {
-        // a block holds at most T tokens, so the token's is at least this far on
-        uint32_t k = cur + (t > cur_start ? (t - cur_start) / p.T : 0u);
-        for (; k < n_blocks; ++k) {
-          const uint4 blk = __ldg(blocks + k);
-          const uint32_t v = min((blk.y >> 10) & 0x3FFu, p.T);
-          if (t < blk.w) break;  // not listed
-          if (t - blk.w < v) {
-            f = open_block(p, blk, &payload);
-            info = blk.y;
-            sref = blk.z;
-            r = t - blk.w;
-            break;
+      at_k = cur + (t > cur_start ? (t - cur_start) / p.T : 0u);
+      if (in && at_k < n_blocks) entry = __ldg(blocks + at_k);
+    };
+    // Second half: partly filled blocks put the token further on.
+    auto find = [&](uint32_t j) {
+      uint32_t t;
+      Token tok;
+      tok.f = 4;
+      tok.k = 0;
+      tok.kp = tok.vp = make_float2(1.0f, 0.0f);
+      if (position(j, &t)) {
+        while (at_k < n_blocks && t >= entry.w && t - entry.w >= min((entry.y >> 10) & 0x3FFu, p.T)) {
+          if (++at_k < n_blocks) entry = __ldg(blocks + at_k);
+        }
+        if (at_k < n_blocks && t >= entry.w) {  // else not listed
+          const uint8_t* payload = nullptr;
+          tok.f = open_block(p, entry, &payload);
+          if (tok.f <= 3) {
+            const uint32_t row = (t - entry.w) * p.H + h;
+            tok.k = reinterpret_cast<uint64_t>(payload) + uint64_t{row} * (tok.f == dev::kFp16 ? kD * 2 : tok.f == dev::kInt4 ? kD / 2 : kD);
+            tok.kp = params_of_row(tok.f, entry.y, entry.z, payload + p.code_bytes[tok.f], row);
+            tok.vp = params_of_row(tok.f, entry.y, entry.z, payload + p.code_bytes[tok.f], row + p.T * p.H);
           }
         }
-        if ((lane & 15) == 0 && k < n_blocks) {
-          cur = k;
-          cur_start = __ldg(&blocks[k].w);
+      }
+      const uint32_t k0 = __shfl_sync(0xFFFFFFFFu, at_k, 0), w0 = __shfl_sync(0xFFFFFFFFu, entry.w, 0);
+      if (k0 < n_blocks) {
+        cur = k0;
+        cur_start = w0;
+      }
+      return tok;
+    };
+    uint4 raw[2][kBatch];
+    uint32_t fr[2][kBatch];
+    // Batch b of a tile: of its K half, then of its V half.
+    auto load = [&](const Token& tok, uint32_t b, uint4 (&r)[kBatch], uint32_t (&fs)[kBatch]) {
+      const uint32_t half = b / kBatches, it0 = b % kBatches * kBatch;
+      const uint64_t row_bytes = tok.f == dev::kFp16 ? kD * 2 : tok.f == dev::kInt4 ? kD / 2 : kD;
+      const uint64_t src = tok.k + (half ? row_bytes * p.T * p.H : 0u);
+#pragma unroll
+      for (uint32_t it = 0; it < kBatch; ++it) {
+        const uint32_t from = (it0 + it) * kRowsIter + sub;
+        const uint64_t a = __shfl_sync(0xFFFFFFFFu, src, from);
+        fs[it] = __shfl_sync(0xFFFFFFFFu, tok.f, from);
+        r[it] = make_uint4(0u, 0u, 0u, 0u);
+        if (fs[it] == dev::kFp16) r[it] = __ldg(reinterpret_cast<const uint4*>(a) + chunk);
+        else if (fs[it] == dev::kInt4) r[it].x = __ldg(reinterpret_cast<const uint32_t*>(a) + chunk);
+        else if (fs[it] < 4) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(a) + chunk);
+          r[it].x = w.x;
+          r[it].y = w.y;
         }
       }
-      cur = __shfl_sync(0xFFFFFFFFu, cur, 0);
-      cur_start = __shfl_sync(0xFFFFFFFFu, cur_start, 0);
-      const uint32_t krow = r * p.H + h, vrow = krow + p.T * p.H;
-      float2 kp = make_float2(1.0f, 0.0f), vp = make_float2(1.0f, 0.0f);
-      if (f <= 3) {
-        kp = params_of_row(f, info, sref, payload + p.code_bytes[f], krow);
-        vp = params_of_row(f, info, sref, payload + p.code_bytes[f], vrow);
+    };
+    bool bad = false, part = false;
+    auto store = [&](uint32_t j, uint32_t b, const uint4 (&r)[kBatch], const uint32_t (&fs)[kBatch]) {
+      const uint32_t half = b / kBatches, it0 = b % kBatches * kBatch;
+      const uint32_t operand = base + (half ? C::kV : C::kK) + (j & 1) * C::kOperand;
+#pragma unroll
+      for (uint32_t it = 0; it < kBatch; ++it) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (fs[it] < 4) v = half ? convert<true>(fs[it], r[it]) : convert<false>(fs[it], r[it]);
+        if (half && part) bad = bad || has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(operand, sw * 16 + (it0 + it) * kRowsIter + sub, chunk)), "r"(v.x),
+                     "r"(v.y), "r"(v.z), "r"(v.w)
+                     : "memory");
       }
+    };
+    Token tok;
+    if (n_tiles > 0) {
+      look(0);
+      tok = find(0);
+      load(tok, 0, raw[0], fr[0]);
+    }
+    for (uint32_t j = 0; j < n_tiles; ++j) {
+      Token next = tok;
+      // ---- what the softmax needs of the tokens
+      uint32_t tp, n;
+      walk.tile(j, &tp, &n);
+      const uint32_t i = sw * 16 + (lane & 15), f = tok.f;
       const uint32_t kinds = __reduce_or_sync(0xFFFFFFFFu, f > 3 ? 4u : f == dev::kInt4 ? 3u : f == dev::kFp16 ? 0u : 1u);
-      const bool scaled = (kinds & 3u) != 0;
       const uint32_t exists = __ballot_sync(0xFFFFFFFFu, f <= 3) & 0xFFFFu;
+      const bool scaled = (kinds & 3u) != 0;
       const float unit = f == dev::kFp16 ? 1.0f : f == dev::kE4M3 ? 0x1p8f : f == dev::kE5M2 ? 0x1p15f : 8.0f;
-      const float u = f > 3 ? 0.0f : vp.x * unit;
+      const float u = f > 3 ? 0.0f : tok.vp.x * unit;
       const uint32_t ub = __float_as_uint(u) & 0x7FFFFFFFu;
       const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, ub < 0x7F800000u ? ub : 0u);
       const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, f > 3 ? 0xFFFFFFFFu : ub);
@@ -514,73 +620,49 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       // A tile that some row sees in part: values that are not finite, or scales far apart, would touch rows that
       // do not see them.  Such a CTA's rows are done over, one by one.
       const int32_t t0 = static_cast<int32_t>(tp);
-      const bool part = n < kTile || t0 + 127 > p_lo ||
-                        (p.window != 0 && t0 + 128 > static_cast<int32_t>(min(p.sinks, 0x7FFFFF00u)) &&
-                         p_hi - t0 >= static_cast<int32_t>(min(p.window, 0x7FFFFFFFu)));
-      bool bad = part && f <= 3 && (ub >= 0x7F800000u || (low != 0xFFFFFFFFu && top > low + (10u << 23)) || !dev::finite_f32(vp.y));
-
-      // ---- K, then V
-#pragma unroll 1
-      for (uint32_t half = 0; half < 2; ++half) {
-        if (j >= 2) {
-          ok = ok && mbar_wait(half ? &sh.v_empty[stage] : &sh.k_empty[stage], (j / 2 - 1) & 1);
+      part = n < kTile || t0 + 127 > p_lo ||
+             (p.window != 0 && t0 + 128 > static_cast<int32_t>(min(p.sinks, 0x7FFFFF00u)) &&
+              p_hi - t0 >= static_cast<int32_t>(min(p.window, 0x7FFFFFFFu)));
+      bad = bad || (part && f <= 3 && (ub >= 0x7F800000u || (low != 0xFFFFFFFFu && top > low + (10u << 23)) || !dev::finite_f32(tok.vp.y)));
+      const bool more = j + 1 < n_tiles;
+      if (more) look(j + 1);
+#pragma unroll
+      for (uint32_t b = 0; b < 2 * kBatches; ++b) {
+        const uint32_t half = b / kBatches;
+        // the next batch's loads
+        if (b + 1 < 2 * kBatches) {
+          load(tok, b + 1, raw[(b + 1) & 1], fr[(b + 1) & 1]);
+        } else if (more) {
+          next = find(j + 1);
+          load(next, 0, raw[(b + 1) & 1], fr[(b + 1) & 1]);
+        }
+        if (b % kBatches == 0) {
+          if (j >= 2) ok = ok && mbar_wait(half ? &sh.v_empty[j & 1] : &sh.k_empty[j & 1], (j / 2 - 1) & 1);
           if (!ok) break;
-        }
-        if (lane < 16) {
-          if (half == 0) {
-            const uint32_t info_i = j & 3;
-            sh.ks[info_i][i] = f > 3 ? 0.0f : kp.x * (p.qscale * (f == dev::kInt4 ? 8.0f : 1.0f));
-            sh.kb[info_i][i] = f == dev::kInt4 ? fmaf(8.0f, kp.x, kp.y) : 0.0f;
-            sh.vs[info_i][i] = scaled ? u * pow2(-e) : 1.0f;
-            sh.vb[info_i][i] = f == dev::kInt4 ? fmaf(8.0f, vp.x, vp.y) : 0.0f;
+          if (half == 0 && lane < 16) {
+            const uint32_t info = j & 3;
+            sh.ks[info][i] = f > 3 ? 0.0f : tok.kp.x * (p.qscale * (f == dev::kInt4 ? 8.0f : 1.0f));
+            sh.kb[info][i] = f == dev::kInt4 ? fmaf(8.0f, tok.kp.x, tok.kp.y) : 0.0f;
+            sh.vs[info][i] = scaled ? u * pow2(-e) : 1.0f;
+            sh.vb[info][i] = f == dev::kInt4 ? fmaf(8.0f, tok.vp.x, tok.vp.y) : 0.0f;
             if (lane == 0) {
-              sh.kind[info_i][sw] = kinds;
-              sh.exists[info_i][sw] = exists;
-              sh.exponent[info_i][sw] = scaled ? (top ? e : -1000) : 0;
+              sh.kind[info][sw] = kinds;
+              sh.exists[info][sw] = exists;
+              sh.exponent[info][sw] = scaled ? (top ? e : -1000) : 0;
             }
           }
         }
-        const uint32_t row = half ? vrow : krow;
-        const uint64_t src = reinterpret_cast<uint64_t>(payload) + uint64_t{row} * (f == dev::kFp16 ? kD * 2 : f == dev::kInt4 ? kD / 2 : kD);
-        constexpr uint32_t kChunks = kD / 8, kRowsIter = 32 / kChunks, kIters = 16 / kRowsIter;  // 16 or 8 chunks a row
-        const uint32_t c = lane % kChunks, sub = lane / kChunks;
-        const uint32_t operand = base + (half ? C::kV : C::kK) + stage * C::kOperand;
-        constexpr uint32_t kBatch = kIters < 4 ? kIters : 4;
-#pragma unroll 1
-        for (uint32_t it0 = 0; it0 < kIters; it0 += kBatch) {
-          uint4 raw[kBatch];
-          uint32_t fr[kBatch];
-#pragma unroll
-          for (uint32_t it = 0; it < kBatch; ++it) {
-            const uint32_t from = (it0 + it) * kRowsIter + sub;
-            const uint64_t a = __shfl_sync(0xFFFFFFFFu, src, from);
-            fr[it] = __shfl_sync(0xFFFFFFFFu, f, from);
-            raw[it] = make_uint4(0u, 0u, 0u, 0u);
-            if (fr[it] == dev::kFp16) raw[it] = __ldg(reinterpret_cast<const uint4*>(a) + c);
-            else if (fr[it] == dev::kInt4) raw[it].x = __ldg(reinterpret_cast<const uint32_t*>(a) + c);
-            else if (fr[it] < 4) {
-              const uint2 w = __ldg(reinterpret_cast<const uint2*>(a) + c);
-              raw[it].x = w.x;
-              raw[it].y = w.y;
-            }
-          }
-#pragma unroll
-          for (uint32_t it = 0; it < kBatch; ++it) {
-            const uint32_t to = sw * 16 + (it0 + it) * kRowsIter + sub;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (fr[it] < 4) v = half ? convert<true>(fr[it], raw[it]) : convert<false>(fr[it], raw[it]);
-            if (half && part) bad = bad || has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(operand, to, c)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                         : "memory");
-          }
+        store(j, b, raw[b & 1], fr[b & 1]);
+        if (b % kBatches == kBatches - 1) {
+          dev::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(half ? &sh.v_full[j & 1] : &sh.k_full[j & 1]);
         }
-        dev::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(half ? &sh.v_full[stage] : &sh.k_full[stage]);
       }
-      if (bad) sh.redo = 1;
+      tok = next;
       if (!ok) break;
     }
+    if (bad) sh.redo = 1;
   } else if (warp == kSoftmaxWarps + kStageWarps) {
     // ================= products: one thread =================
     if (lane == 0 && n_tiles > 0) {
