@@ -86,6 +86,13 @@ __device__ __forceinline__ void tmem_load32(uint32_t a, uint32_t (&r)[32]) {
         "=r"(r[30]), "=r"(r[31])
       : "r"(a));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t a, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(a));
+}
 __device__ __forceinline__ void tmem_store16(uint32_t a, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(a),
@@ -177,6 +184,11 @@ __device__ __forceinline__ uint4 convert(uint32_t f, uint4 raw) {
   }
   return make_uint4(a0, a1, a2, a3);
 }
+
+template <uint32_t kF>
+struct Format {
+  static constexpr uint32_t value = kF;
+};
 
 // Shared-memory address of 16-byte chunk c (of kD / 8) of row r in an operand: panels of 64 elements, the chunk
 // index of a row's 128 bytes XORed with the row's place in its 8.
@@ -306,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&sh.s_full[acc], j & 1));
         if (!ok) break;
         fence_after();
+        __syncwarp();
         // Whether all 128 rows see all 128 tokens.
         const int32_t t0 = static_cast<int32_t>(tp), acc_lo = pos_base + static_cast<int32_t>((row0 + acc * 128) / p.group);
         uint32_t any_kind = 0;
@@ -356,56 +369,75 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
         };
         const Pair zero = pair(0.0f, 0.0f);
-        float top = -INFINITY;
+        // ---- the accumulator's unit
+        auto rescale = [&](float f) {  // O of this tile's row, once the products before have been added to it
+          if (j == 0) return true;
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh.o_done[acc], (j - 1) & 1))) return false;
+          fence_after();
 #pragma unroll 1
-        for (uint32_t c = 0; c < 4; ++c) {
-          Pair x[16];
-          scores(c, zero, zero, x);
+          for (uint32_t c = 0; c < kD / 32; ++c) {
+            uint32_t o[32];
+            tmem_load32(t_o + c * 32, o);
+            wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 v = split(x[i]);
-            top = fmaxf(top, fmaxf(v.x, v.y));
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_store32(t_o + c * 32, o);
           }
-        }
-        // ---- the reference maximum and the accumulator's unit
+          wait_st();
+          return true;
+        };
         const int e_new = min(max(e_tile, -60), 60);
-        const bool shift = j == 0 || (e_tile != -1000 && (e_new > E + 6 || e_new < E - 6));
-        const bool grow = top > m + 8.0f;
-        if (__any_sync(0xFFFFFFFFu, grow) || shift) {
-          const float mn = grow ? fmaxf(m, top) : m;
-          const float a = mn == -INFINITY ? 1.0f : exp2f(m - mn);
-          m = mn;
-          l *= a;
-          bias *= a;
-          const int e_to = shift ? (e_tile == -1000 ? 0 : e_new) : E;
-          if (j > 0) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh.o_done[acc], (j - 1) & 1));
-            if (!ok) break;
-            fence_after();
-            const float f = a * exp2f(static_cast<float>(E - e_to));
-#pragma unroll 1
-            for (uint32_t c = 0; c < kD / 32; ++c) {
-              uint32_t o[32];
-              tmem_load32(t_o + c * 32, o);
-              wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_store32(t_o + c * 32, o);
-            }
-          }
-          E = e_to;
+        if (j == 0) {
+          E = e_tile == -1000 ? 0 : e_new;
+        } else if (e_tile != -1000 && (e_new > E + 6 || e_new < E - 6)) {
+          ok = rescale(exp2f(static_cast<float>(E - e_new)));
+          if (!ok) break;
+          E = e_new;
         }
-        // ---- weights
-        const float ref = m == -INFINITY ? 0.0f : m;
+        // ---- weights, in one pass: 32 tokens at a time, against the reference maximum so far.  Where a score passes
+        // it by more than 8 (weights reach 2^8 at most), the maximum moves, and what was made with the old one
+        // (O, the sums, this tile's weights so far) is scaled.
 #pragma unroll 1
         for (uint32_t c = 0; c < 4; ++c) {
           // a group's weights are in units of 2^(its exponent), the sums in their own
           const uint32_t kind0 = sh.kind[info][2 * c], kind1 = sh.kind[info][2 * c + 1];
           const int d0 = (kind0 & 3u ? min(max(sh.exponent[info][2 * c], -60), 60) : 0) - E;
           const int d1 = (kind1 & 3u ? min(max(sh.exponent[info][2 * c + 1], -60), 60) : 0) - E;
+          const float ref = m == -INFINITY ? 0.0f : m;
           const float add0 = static_cast<float>(d0) - ref, add1 = static_cast<float>(d1) - ref;
           Pair x[16];
           scores(c, pair(add0, add0), pair(add1, add1), x);
+          float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 u = split(x[i]), v = split(x[8 + i]);
+            top0 = fmaxf(top0, fmaxf(u.x, u.y));
+            top1 = fmaxf(top1, fmaxf(v.x, v.y));
+          }
+          const float top = fmaxf(top0 - static_cast<float>(d0), top1 - static_cast<float>(d1));  // above the reference
+          const bool grow = top > (m == -INFINITY ? -INFINITY : 8.0f);
+          if (__any_sync(0xFFFFFFFFu, grow)) {
+            const float up = grow ? top : 0.0f;  // the maximum moves to ref + up
+            const float a = m == -INFINITY ? (grow ? 0.0f : 1.0f) : exp2f(-up);
+            ok = rescale(a);
+            if (!ok) break;
+            if (grow) m = ref + top;
+            l *= a;
+            bias *= a;
+            const uint32_t a2 = dev::pack_f16x2(a, a);
+#pragma unroll 1
+            for (uint32_t k = 0; k < c; ++k) {
+              uint32_t w[16];
+              tmem_load16(t_s + k * 16, w);
+              wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = hmul2(w[i], a2);
+              tmem_store16(t_s + k * 16, w);
+            }
+            const Pair down = pair(-up, -up);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = add2(x[i], down);
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 v = split(x[i]);
@@ -449,6 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
           tmem_store16(t_s + c * 16, w);
         }
+        if (!ok) break;
         wait_st();
         fence_before();
         __syncwarp();
@@ -500,6 +533,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       uint64_t k;     // address of its K row
       uint32_t f;     // 4: it does not exist
       float2 kp, vp;  // its rows' {scale, bias}
+      uint64_t first;  // all 16 in one block: address of the first one's K row,
+      uint32_t step;   // and bytes from a token's row to the next one's (0: they are not)
     };
     uint32_t cur = 0, cur_start = 0;  // a block at or before this warp's next first token, and its first position
     uint32_t at_k = 0;                // the block that `entry` is
@@ -553,7 +588,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
         }
       }
+      const uint32_t rb = tok.f == dev::kFp16 ? kD * 2 : tok.f == dev::kInt4 ? kD / 2 : kD;
+      tok.first = __shfl_sync(0xFFFFFFFFu, tok.k, 0);
       const uint32_t k0 = __shfl_sync(0xFFFFFFFFu, at_k, 0), w0 = __shfl_sync(0xFFFFFFFFu, entry.w, 0);
+      tok.step = __all_sync(0xFFFFFFFFu, tok.f <= 3 && at_k == k0) ? p.H * rb : 0u;
       if (k0 < n_blocks) {
         cur = k0;
         cur_start = w0;
@@ -565,6 +603,25 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     // Batch b of a tile: of its K half, then of its V half.
     auto load = [&](const Token& tok, uint32_t b, uint4 (&r)[kBatch], uint32_t (&fs)[kBatch]) {
       const uint32_t half = b / kBatches, it0 = b % kBatches * kBatch;
+      if (tok.step != 0) {  // 16 rows of one block: equally far apart
+        const uint64_t a = tok.first + (half ? uint64_t{tok.step} * p.T : 0u) + uint64_t{it0 * kRowsIter + sub} * tok.step;
+        const uint32_t step = kRowsIter * tok.step;
+        if (tok.f == dev::kFp16) {
+#pragma unroll
+          for (uint32_t it = 0; it < kBatch; ++it) r[it] = __ldg(reinterpret_cast<const uint4*>(a + it * step) + chunk);
+        } else if (tok.f == dev::kInt4) {
+#pragma unroll
+          for (uint32_t it = 0; it < kBatch; ++it) r[it].x = __ldg(reinterpret_cast<const uint32_t*>(a + it * step) + chunk);
+        } else {
+#pragma unroll
+          for (uint32_t it = 0; it < kBatch; ++it) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(a + it * step) + chunk);
+            r[it].x = w.x;
+            r[it].y = w.y;
+          }
+        }
+        return;
+      }
       const uint64_t row_bytes = tok.f == dev::kFp16 ? kD * 2 : tok.f == dev::kInt4 ? kD / 2 : kD;
       const uint64_t src = tok.k + (half ? row_bytes * p.T * p.H : 0u);
 #pragma unroll
@@ -583,13 +640,31 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       }
     };
     bool bad = false, part = false;
-    auto store = [&](uint32_t j, uint32_t b, const uint4 (&r)[kBatch], const uint32_t (&fs)[kBatch]) {
+    auto store = [&](uint32_t j, uint32_t b, bool even, uint32_t f, const uint4 (&r)[kBatch], const uint32_t (&fs)[kBatch]) {
       const uint32_t half = b / kBatches, it0 = b % kBatches * kBatch;
       const uint32_t operand = base + (half ? C::kV : C::kK) + (j & 1) * C::kOperand;
+      if (even && !(half && part)) {
+        auto all = [&](auto format) {
+          constexpr uint32_t kF = decltype(format)::value;
+#pragma unroll
+          for (uint32_t it = 0; it < kBatch; ++it) {
+            const uint4 v = half ? convert<true>(kF, r[it]) : convert<false>(kF, r[it]);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(operand, sw * 16 + (it0 + it) * kRowsIter + sub, chunk)),
+                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                         : "memory");
+          }
+        };
+        if (f == dev::kFp16) all(Format<dev::kFp16>{});
+        else if (f == dev::kE4M3) all(Format<dev::kE4M3>{});
+        else if (f == dev::kE5M2) all(Format<dev::kE5M2>{});
+        else all(Format<dev::kInt4>{});
+        return;
+      }
 #pragma unroll
       for (uint32_t it = 0; it < kBatch; ++it) {
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (fs[it] < 4) v = half ? convert<true>(fs[it], r[it]) : convert<false>(fs[it], r[it]);
+        const uint32_t ft = even ? f : fs[it];
+        if (ft < 4) v = half ? convert<true>(ft, r[it]) : convert<false>(ft, r[it]);
         if (half && part) bad = bad || has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w);
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(operand, sw * 16 + (it0 + it) * kRowsIter + sub, chunk)), "r"(v.x),
                      "r"(v.y), "r"(v.z), "r"(v.w)
@@ -652,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             }
           }
         }
-        store(j, b, raw[b & 1], fr[b & 1]);
+        store(j, b, tok.step != 0, tok.f, raw[b & 1], fr[b & 1]);
         if (b % kBatches == kBatches - 1) {
           dev::fence_proxy_async_smem();
           __syncwarp();
