@@ -24,7 +24,7 @@ namespace battn {
 namespace {
 
 constexpr int kSoftmaxWarps = 8, kStageWarps = 8;
-constexpr int kThreads = (kSoftmaxWarps + kStageWarps + 4) * 32;  // and one that issues the products
+constexpr int kThreads = (kSoftmaxWarps + kStageWarps + 1) * 32;  // and one that issues the products
 constexpr uint32_t kTile = 128;                                  // tokens of a tile
 constexpr uint32_t kRowsCta = 256;
 
@@ -357,14 +357,15 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             for (int i = 0; i < 16; ++i) x[i] = fma2(pair(raw[2 * i], raw[2 * i + 1]), scale2, i < 8 ? add0 : add1);
           }
           if (masked) {
-            const uint32_t exists = sh.exists[info][2 * c] | sh.exists[info][2 * c + 1] << 16;
+            // a bit per token: up to the row's own, and from the window's first one on or among the sinks
+            const int32_t tc = t0 + static_cast<int32_t>(c) * 32;
+            auto below = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+            const uint32_t see = below(pos - tc + 1) & (~below(low - tc) | below(static_cast<int32_t>(min(p.sinks, 0x7FFFFFFFu)) - tc)) &
+                                 (sh.exists[info][2 * c] | sh.exists[info][2 * c + 1] << 16);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int32_t t = t0 + static_cast<int32_t>(c) * 32 + 2 * i;
-              const bool see0 = t <= pos && (t >= low || static_cast<uint32_t>(t) < p.sinks) && (exists >> (2 * i) & 1u);
-              const bool see1 = t + 1 <= pos && (t + 1 >= low || static_cast<uint32_t>(t) + 1 < p.sinks) && (exists >> (2 * i + 1) & 1u);
               const float2 v = split(x[i]);
-              x[i] = pair(see0 ? v.x : -INFINITY, see1 ? v.y : -INFINITY);
+              x[i] = pair(see & 1u << (2 * i) ? v.x : -INFINITY, see & 2u << (2 * i) ? v.y : -INFINITY);
             }
           }
         };
