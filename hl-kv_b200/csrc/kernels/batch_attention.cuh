@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "codec.cuh"
@@ -259,6 +260,21 @@ __device__ __noinline__ void attend_row(const Params& p, uint32_t i, uint32_t to
     p.out[token * p.out_stride + uint64_t{qh} * kD + lane * kN + e] = __half_as_ushort(__float2half_rn(r));
   }
 }
+
+// A kernel's permission for large shared memory, asked for once per device (a microsecond of each call).
+struct SharedMemoryOnce {
+  std::atomic<uint64_t> done{0};
+  cudaError_t allow(const void* kernel, uint32_t bytes) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? uint64_t{1} << device : 0u;
+    if ((done.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+  }
+};
 
 // Launches of the kernels (their translation units).
 cudaError_t launch_stream(uint32_t head_dim, const Params& p, cudaStream_t s);

@@ -1303,8 +1303,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
 template <int kD, bool kTwo>
 cudaError_t launch(const Params& p, cudaStream_t s) {
   using C = Config<kD, kTwo>;
-  const cudaError_t e = cudaFuncSetAttribute(stream_kernel<kD, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(C::kSmem));
+  static SharedMemoryOnce once;
+  const cudaError_t e = once.allow(reinterpret_cast<const void*>(stream_kernel<kD, kTwo>), C::kSmem);
   if (e != cudaSuccess) return e;
   stream_kernel<kD, kTwo><<<p.ctas, kThreads, C::kSmem, s>>>(p);
   const cudaError_t e2 = cudaGetLastError();

@@ -798,7 +798,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 
 template <int kD>
 cudaError_t launch(const Params& p, cudaStream_t s) {
-  const cudaError_t e = cudaFuncSetAttribute(tile_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Config<kD>::kSmem));
+  static SharedMemoryOnce once;
+  const cudaError_t e = once.allow(reinterpret_cast<const void*>(tile_kernel<kD>), Config<kD>::kSmem);
   if (e != cudaSuccess) return e;
   const uint64_t grid = uint64_t{p.nseq} * p.H * ((uint64_t{p.max_rows} + kRowsCta - 1) / kRowsCta);
   if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;

@@ -422,7 +422,7 @@ extern "C" int hlkv_batch_plan(const HlkvBatchPlan* plan, const HlkvLayout* layo
   const uint64_t average = plan->block_cap / plan->nseq;
   unsigned ctas = 1;
   while (ctas < kMaxCluster && uint64_t{ctas} * kRound < average &&
-         uint64_t{plan->nseq} * ctas * 2 <= static_cast<uint64_t>(sm_count()) * 2) {
+         uint64_t{plan->nseq} * ctas * 2 <= static_cast<uint64_t>(sm_count()) * 4) {
     ctas *= 2;
   }
   cudaLaunchConfig_t cfg{};

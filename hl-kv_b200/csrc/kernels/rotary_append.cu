@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunks = 2;
+constexpr uint32_t kMaxTokens = 8;  // of a CTA
 
 enum : int { kHalves = 0, kHalvesPartial = 1, kAdjacent = 2 };  // how pairs lie in a head
 
@@ -140,10 +141,22 @@ __device__ __forceinline__ uint32_t encode_row_f32(uint32_t f, const float (&x)[
     const float scale = __fmul_rn(range, 1.0f / 15.0f);
     uint32_t word[2] = {0u, 0u};
     if (scale > 0.0f) {
+      const float y = __frcp_rn(scale), ylo = __fmul_rn(y, dev::kBracketLo), yhi = __fmul_rn(y, dev::kBracketHi);
+      uint32_t diff = 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const uint32_t q = dev::rint_u(__fdiv_rn(__fsub_rn(x[i], mn), scale));
-        word[i / 8] |= min(q, 15u) << (4 * (i % 8));
+        const float d = __fsub_rn(x[i], mn);
+        const uint32_t qa = dev::rint_u(__fmul_rn(d, ylo)), qb = dev::rint_u(__fmul_rn(d, yhi));
+        diff |= qa ^ qb;
+        word[i / 8] |= min(qa, 15u) << (4 * (i % 8));
+      }
+      if (diff != 0) {  // near the middle of two codes: the divisions themselves
+        word[0] = word[1] = 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t q = dev::rint_u(__fdiv_rn(__fsub_rn(x[i], mn), scale));
+          word[i / 8] |= min(q, 15u) << (4 * (i % 8));
+        }
       }
     }
 #pragma unroll
@@ -162,35 +175,101 @@ __device__ __forceinline__ uint32_t encode_row_f32(uint32_t f, const float (&x)[
   if (m >= 0x7F800000u) return dev::kErrNonFinite;
   float scale = 1.0f;
   if (m > 0) scale = fmaxf(__fmul_rn(__uint_as_float(m), f == dev::kE4M3 ? 1.0f / 448.0f : 1.0f / 57344.0f), 1.17549435e-38f);
+  const float y = __frcp_rn(scale), ylo = __fmul_rn(y, dev::kBracketLo), yhi = __fmul_rn(y, dev::kBracketHi);
+  uint32_t r[8], diff = 0;
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    uint32_t r[4];
+  for (int i = 0; i < 8; ++i) {
+    const float a0 = __fmul_rn(x[2 * i], ylo), a1 = __fmul_rn(x[2 * i + 1], ylo);
+    const float b0 = __fmul_rn(x[2 * i], yhi), b1 = __fmul_rn(x[2 * i + 1], yhi);
+    r[i] = f == dev::kE4M3 ? dev::cvt_e4m3x2(a0, a1) : dev::cvt_e5m2x2(a0, a1);
+    diff |= r[i] ^ (f == dev::kE4M3 ? dev::cvt_e4m3x2(b0, b1) : dev::cvt_e5m2x2(b0, b1));
+  }
+  if (diff != 0) {  // near the middle of two codes: the divisions themselves
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = __fdiv_rn(x[8 * c + 2 * i], scale), b = __fdiv_rn(x[8 * c + 2 * i + 1], scale);
+    for (int i = 0; i < 8; ++i) {
+      const float a = __fdiv_rn(x[2 * i], scale), b = __fdiv_rn(x[2 * i + 1], scale);
       r[i] = f == dev::kE4M3 ? dev::cvt_e4m3x2(a, b) : dev::cvt_e5m2x2(a, b);
     }
+  }
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
     reinterpret_cast<uint2*>(payload + uint64_t{row} * kD)[c * kLanes + lane] =
-        make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+        make_uint2(r[4 * c] | r[4 * c + 1] << 16, r[4 * c + 2] | r[4 * c + 3] << 16);
   }
   if (lane == 0) reinterpret_cast<float*>(payload + code_bytes)[row] = scale;
   return 0;
 }
+
+// Where a token's K and V go: resolved once per token and CTA.
+struct Place {
+  uint8_t* payload;
+  uint32_t f;      // format; kSkip: no store; kPadding: nothing at all
+  uint32_t token;  // slot in the block
+};
+constexpr uint32_t kSkip = 16, kPadding = 17;
 
 template <int kD, int kMode>
 __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_constant__ Params p) {
   constexpr int kLanes = kD / 16;
   constexpr int kRowsPerIter = kThreads / kLanes;
   extern __shared__ float2 s_cs[];  // [tokens_per_cta][rotary_dim / 2]
+  __shared__ Place s_place[kMaxTokens];
   const uint32_t lane = threadIdx.x % kLanes;
   const uint32_t mask = dev::row_mask<kD, kChunks>();
   const uint32_t pairs = p.rope.rotary_dim / 2;
   const uint32_t token0 = blockIdx.x * p.tokens_per_cta;
   const uint32_t tokens = min(p.tokens_per_cta, p.n - token0);
+  const uint32_t rows = tokens * p.rows_per_token.d;
 
+  // A row's source: its loads do not wait for the angles or the targets.
+  auto source = [&](uint32_t g, uint32_t* t, uint32_t* r) {
+    *t = p.rows_per_token.div(g);
+    *r = g - *t * p.rows_per_token.d;
+    const uint32_t token = token0 + *t;
+    return *r < p.q_heads         ? p.q + token * p.q_stride + uint64_t{*r} * kD
+           : *r < p.q_heads + p.H ? p.k + token * p.k_stride + uint64_t{*r - p.q_heads} * kD
+                                  : p.v + token * p.v_stride + uint64_t{*r - p.q_heads - p.H} * kD;
+  };
+  uint32_t g = threadIdx.x / kLanes, t = 0, r = 0;
+  const uint16_t* src = nullptr;
+  uint4 next[kChunks];
+  if (g < rows) {
+    src = source(g, &t, &r);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) next[c] = __ldcs(reinterpret_cast<const uint4*>(src) + c * kLanes + lane);
+  }
+
+  // The last threads resolve the targets while the first ones take the angles.
+  const uint32_t back = kThreads - 1 - threadIdx.x;
+  if (back < tokens) {
+    const uint2 target = __ldg(p.targets + token0 + back);
+    Place place{nullptr, kSkip, target.y};
+    uint32_t bad = 0;
+    if (target.x == 0xFFFFFFFFu && target.y == 0xFFFFFFFFu) {
+      place.f = kPadding;
+    } else if (target.x >= p.table_size) {
+      bad = dev::kErrBlockIdRange;
+    } else {
+      const uint4 d = __ldg(p.table + target.x);
+      const uint32_t f = d.y & 0xFu, mode = (d.y >> 4) & 3u, layout = (d.y >> 6) & 0xFu;
+      if (d.w != target.x) bad = dev::kErrDescMismatch;
+      else if (f == dev::kInvalidFormat) bad = dev::kErrNotExecutable;
+      else if (f > 3 || p.pool[f].base == nullptr || p.pool[f].num_slots == 0) bad = dev::kErrBadFormat;
+      else if (layout != p.layout_id) bad = dev::kErrLayout;
+      else if (f != dev::kFp16 && mode != 0) bad = dev::kErrScaleMode;
+      else if (target.y >= p.T) bad = dev::kErrTokenRange;
+      else if (d.x >= p.pool[f].num_slots) bad = dev::kErrSlotRange;
+      else {
+        place.payload = p.pool[f].base + uint64_t{d.x} * p.pool[f].slot_bytes;
+        place.f = f;
+      }
+    }
+    if (bad) atomicOr(p.err, bad);
+    s_place[back] = place;
+  }
   for (uint32_t i = threadIdx.x; i < tokens * pairs; i += kThreads) {
-    const uint32_t t = i / pairs, j = i - t * pairs;
-    const int32_t pos = __ldg(p.positions + (token0 + t) * p.pos_token + p.rope.pair_axis[j] * p.pos_axis);
+    const uint32_t k = i / pairs, j = i - k * pairs;
+    const int32_t pos = __ldg(p.positions + (token0 + k) * p.pos_token + p.rope.pair_axis[j] * p.pos_axis);
     double sn, cs;
     sincos64(static_cast<double>(pos) * static_cast<double>(p.rope.inv_freq[j]), &sn, &cs);
     const double f = p.rope.factor;
@@ -198,25 +277,27 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_co
   }
   __syncthreads();
 
-  const uint32_t rows = tokens * p.rows_per_token.d;
-  for (uint32_t g = threadIdx.x / kLanes; g < rows; g += kRowsPerIter) {
+  for (; g < rows; g += kRowsPerIter) {
     // Everything below is uniform over the lanes of row g.
-    const uint32_t t = p.rows_per_token.div(g), r = g - t * p.rows_per_token.d, token = token0 + t;
-    const uint2 target = __ldg(p.targets + token);
-    if (target.x == 0xFFFFFFFFu && target.y == 0xFFFFFFFFu) continue;
-    const bool is_q = r < p.q_heads, is_v = r >= p.q_heads + p.H;
-    const uint16_t* src = is_q   ? p.q + token * p.q_stride + uint64_t{r} * kD
-                          : is_v ? p.v + token * p.v_stride + uint64_t{r - p.q_heads - p.H} * kD
-                                 : p.k + token * p.k_stride + uint64_t{r - p.q_heads} * kD;
+    const uint32_t token = token0 + t, row_t = t, row_r = r;
+    const uint16_t* const row_src = src;
     uint4 raw[kChunks];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) raw[c] = __ldcs(reinterpret_cast<const uint4*>(src) + c * kLanes + lane);
+    for (int c = 0; c < kChunks; ++c) raw[c] = next[c];
+    if (g + kRowsPerIter < rows) {  // the next row's loads
+      src = source(g + kRowsPerIter, &t, &r);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) next[c] = __ldcs(reinterpret_cast<const uint4*>(src) + c * kLanes + lane);
+    }
+    const uint32_t f = s_place[row_t].f;
+    const bool is_q = row_r < p.q_heads, is_v = row_r >= p.q_heads + p.H;
+    if (f == kPadding || (f == kSkip && !is_q)) continue;
 
     float x[16];
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) widen(raw[c], x + 8 * c);
     if (!is_v) {
-      const float2* cs = s_cs + t * pairs;
+      const float2* cs = s_cs + row_t * pairs;
       if constexpr (kMode == kHalves) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -249,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_co
           const uint32_t chunk = c * kLanes + lane;
           other[c] = raw[c];
           if (chunk < 2 * half) {
-            other[c] = __ldcs(reinterpret_cast<const uint4*>(src) + (chunk < half ? chunk + half : chunk - half));
+            other[c] = __ldcs(reinterpret_cast<const uint4*>(row_src) + (chunk < half ? chunk + half : chunk - half));
           }
         }
         __syncwarp(mask);  // d_q_out may be d_q: every lane has read its partner before one writes
@@ -269,36 +350,14 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const __grid_co
       }
     }
     if (is_q) {
-      uint4* dst = reinterpret_cast<uint4*>(p.q_out + token * p.q_out_stride + uint64_t{r} * kD);
+      uint4* dst = reinterpret_cast<uint4*>(p.q_out + token * p.q_out_stride + uint64_t{row_r} * kD);
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) dst[c * kLanes + lane] = narrow(x + 8 * c);
       continue;
     }
-
-    uint32_t bad = 0, f = 0, slot = 0;
-    if (target.x >= p.table_size) {
-      bad = dev::kErrBlockIdRange;
-    } else {
-      const uint4 d = __ldg(p.table + target.x);
-      f = d.y & 0xFu;
-      const uint32_t mode = (d.y >> 4) & 3u, layout = (d.y >> 6) & 0xFu;
-      slot = d.x;
-      if (d.w != target.x) bad = dev::kErrDescMismatch;
-      else if (f == dev::kInvalidFormat) bad = dev::kErrNotExecutable;
-      else if (f > 3 || p.pool[f].base == nullptr || p.pool[f].num_slots == 0) bad = dev::kErrBadFormat;
-      else if (layout != p.layout_id) bad = dev::kErrLayout;
-      else if (f != dev::kFp16 && mode != 0) bad = dev::kErrScaleMode;
-      else if (target.y >= p.T) bad = dev::kErrTokenRange;
-      else if (slot >= p.pool[f].num_slots) bad = dev::kErrSlotRange;
-    }
-    if (bad) {
-      if (r == p.q_heads && lane == 0) atomicOr(p.err, bad);  // once per target
-      continue;
-    }
-    const uint32_t h = r - p.q_heads - (is_v ? p.H : 0u);
-    const uint32_t row = ((is_v ? p.T : 0u) + target.y) * p.H + h;
-    uint8_t* payload = p.pool[f].base + uint64_t{slot} * p.pool[f].slot_bytes;
-    const uint32_t e = encode_row_f32<kD>(f, x, lane, mask, payload, row, p.code_bytes[f]);
+    const uint32_t h = row_r - p.q_heads - (is_v ? p.H : 0u);
+    const uint32_t row = ((is_v ? p.T : 0u) + s_place[row_t].token) * p.H + h;
+    const uint32_t e = encode_row_f32<kD>(f, x, lane, mask, s_place[row_t].payload, row, p.code_bytes[f]);
     if (e != 0 && lane == 0) atomicOr(p.err, e);
   }
 }
@@ -384,7 +443,15 @@ extern "C" int hlkv_rotary_append(const HlkvPools* pools, const HlkvLayout* layo
   p.n = n;
   p.rows_per_token = FastDiv(static_cast<uint32_t>(rows_per_token));
   p.rope = *rotary;
+  // Tokens of a CTA: rows enough for three rounds of its threads (8192 tokens of 48 rows with the gather: 63, 53, 54 us at
+  // 1, 2, 4 tokens a CTA; 1285 of 16 short rows: 11.2, 9.6, 8.8, 9.6 us at 1, 2, 4, 8), as long as every SM has two CTAs
+  // (64 tokens: 9.7 us at 1, 10.0 at 2).
+  const uint64_t threads = rows_per_token * (D / 16);
   p.tokens_per_cta = 1;
+  while (p.tokens_per_cta < kMaxTokens && p.tokens_per_cta * threads < 3 * kThreads &&
+         n / (2 * p.tokens_per_cta) >= 2 * static_cast<uint32_t>(sm_count())) {
+    p.tokens_per_cta *= 2;
+  }
   const int mode = rotary->interleaved ? kAdjacent : rotary->rotary_dim == D ? kHalves : kHalvesPartial;
   const unsigned grid = (n + p.tokens_per_cta - 1) / p.tokens_per_cta;
   const size_t smem = size_t{p.tokens_per_cta} * rotary->rotary_dim / 2 * sizeof(float2);

@@ -277,17 +277,30 @@ def layout_slot_bytes(fmt: int, layout: Layout) -> int:
     return int(lib().hlkv_layout_slot_bytes(fmt, C.byref(layout)))
 
 
+_torch = None
+
+
+def _cuda():
+    """torch, imported at the first call that launches."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
+
+
 def _stream_handle(stream) -> int | None:
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        # the handle alone: torch.cuda.current_stream() builds an object, 2 us of a call
+        c = _cuda()._C
+        return c._cuda_getCurrentRawStream(c._cuda_getDevice())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
 
 
 def _ptr(t) -> int | None:
-    return None if t is None else int(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 # ---- host table -----------------------------------------------------------------------------------
@@ -689,16 +702,15 @@ def _need(cond: bool, what: str) -> None:
         raise HlkvError(what)
 
 
-def _on_device_of(t, fn, *args, **kwargs):
-    """Runs fn with t's device current (the C entry points launch on the current device)."""
-    import torch
-    with torch.cuda.device(t.device):
-        return fn(*args, **kwargs)
+def _elsewhere(index: int) -> bool:
+    """Whether another device than `index` is current."""
+    return _cuda()._C._cuda_getDevice() != index
 
 
-def _current_device() -> int:
-    import torch
-    return torch.cuda.current_device()
+def _on_device(index: int, fn, *args):
+    """Runs fn with device `index` current (the C entry points launch on the current device)."""
+    with _cuda().cuda.device(index):
+        return fn(*args)
 
 
 class BatchPlan:
@@ -725,25 +737,28 @@ class BatchPlan:
         at = [buf.data_ptr() + 4 * o for o, _ in parts]
         self.c = PlanArrays(nseq, max_query, window, sinks, block_cap, token_cap, at[3], at[4], at[5], at[6], at[0],
                             at[1], at[2], at[7], at[8])
-        self.device = buf.device
+        self.device, self.index = buf.device, buf.get_device()
+        self.nseq, self.token_cap = nseq, token_cap
 
 
 def batch_plan(plan: BatchPlan, layout: Layout, table_ptr: int, table_size: int, arena_ptr: int, arena_size: int,
                segs, query_lens, err, stream=None) -> int:
     """Fills the plan from the device tables.  segs: device int32 [nseq, 2]; query_lens: device int32
     [nseq], or None for one new token each.  Raises on a non-OK status."""
-    if plan.device.index != _current_device():
-        return _on_device_of(plan.blocks, batch_plan, plan, layout, table_ptr, table_size, arena_ptr, arena_size, segs,
-                             query_lens, err, stream)
-    n = plan.c.nseq
-    _need(tuple(segs.shape) == (n, 2) and segs.is_contiguous() and segs.element_size() == 4 and segs.device == plan.device,
-          "batch_plan: segs is a contiguous int32 [nseq, 2] on the plan's device")
-    _need(query_lens is None or (query_lens.numel() == n and query_lens.is_contiguous() and query_lens.element_size() == 4
-                                 and query_lens.device == plan.device),
-          "batch_plan: query_lens is a contiguous int32 [nseq] on the plan's device")
-    st = lib().hlkv_batch_plan(C.byref(plan.c), C.byref(layout), table_ptr or None, table_size, arena_ptr or None,
-                               arena_size, segs.data_ptr(), _ptr(query_lens), _ptr(err), _stream_handle(stream))
-    check(st, "hlkv_batch_plan")
+    dev = plan.index
+    if _elsewhere(dev):
+        return _on_device(dev, batch_plan, plan, layout, table_ptr, table_size, arena_ptr, arena_size, segs, query_lens, err,
+                          stream)
+    if not (segs.shape == (plan.nseq, 2) and segs.is_contiguous() and segs.element_size() == 4
+            and segs.get_device() == dev and err.get_device() == dev):
+        raise HlkvError("batch_plan: segs is a contiguous int32 [nseq, 2], on the plan's device as err is")
+    if query_lens is not None and not (query_lens.shape == (plan.nseq,) and query_lens.is_contiguous()
+                                       and query_lens.element_size() == 4 and query_lens.get_device() == dev):
+        raise HlkvError("batch_plan: query_lens is a contiguous int32 [nseq] on the plan's device")
+    st = lib().hlkv_batch_plan(plan.c, layout, table_ptr or None, table_size, arena_ptr or None, arena_size,
+                               segs.data_ptr(), _ptr(query_lens), err.data_ptr(), _stream_handle(stream))
+    if st != OK:
+        check(st, "hlkv_batch_plan")
     return st
 
 
@@ -761,16 +776,15 @@ def make_rotary(inv_freq, axes: int | None = None, pair_axis=None, interleaved: 
     return r
 
 
-def _heads(t, what: str, layout: Layout, n: int | None = None, heads: int | None = None) -> None:
-    _need(t.dim() == 3 and t.shape[2] == layout.head_dim and t.element_size() == 2
-          and (t.shape[1] <= 1 or t.stride(1) == layout.head_dim) and t.stride(2) == 1
-          and (n is None or t.shape[0] == n) and (heads is None or t.shape[1] == heads),
-          f"{what} is a 16-bit [tokens, heads, head_dim] with contiguous heads")
-
-
-def _token_stride(t) -> int:
-    """A tensor of at most one token may have any stride: the row's length then."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+def _token_stride(t, what: str, n: int, heads: int, layout: Layout, dev: int) -> int:
+    """The token stride of a 16-bit [n, heads, head_dim] with contiguous heads on device dev; raises for
+    another tensor.  At most one token may have any stride: the row's length then."""
+    dim = layout.head_dim
+    tok, head, elem = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if not (t.shape == (n, heads, dim) and elem == 1 and (head == dim or heads <= 1) and t.element_size() == 2
+            and t.get_device() == dev):
+        raise HlkvError(f"{what} is a 16-bit [{n}, {heads}, {dim}] with contiguous heads, on the call's device")
+    return tok if n > 1 else heads * dim
 
 
 def rotary_append(pools: Pools, layout: Layout, table_ptr: int, table_size: int, targets, rotary: Rotary, positions,
@@ -779,39 +793,40 @@ def rotary_append(pools: Pools, layout: Layout, table_ptr: int, table_size: int,
     the targets' blocks.  targets: device int32 [n, 2]; positions: device int32 [n] or [n, axes], any
     strides; q, q_out: device 16-bit [n, q_heads, head_dim] (or None); k, v: [n, kv_heads, head_dim];
     token strides are free (slices of a fused projection).  Raises on a non-OK status."""
-    if k.device.index != _current_device():
-        return _on_device_of(k, rotary_append, pools, layout, table_ptr, table_size, targets, rotary, positions, q, k, v,
-                             q_out, err, stream)
-    n = int(targets.shape[0])
-    _heads(k, "rotary_append: k", layout, n, layout.kv_heads)
-    _heads(v, "rotary_append: v", layout, n, layout.kv_heads)
-    _need(targets.is_contiguous() and targets.element_size() == 4 and targets.dim() == 2 and targets.shape[1] == 2,
-          "rotary_append: targets is a contiguous int32 [n, 2]")
-    _need(positions.element_size() == 4 and positions.shape[0] == n
-          and (positions.dim() == 2 and positions.shape[1] >= rotary.axes or positions.dim() == 1 and rotary.axes == 1),
-          "rotary_append: positions is an int32 [n] or [n, axes]")
-    heads = 0
+    dev = k.get_device()
+    if _elsewhere(dev):
+        return _on_device(dev, rotary_append, pools, layout, table_ptr, table_size, targets, rotary, positions, q, k, v, q_out,
+                          err, stream)
+    n = targets.shape[0]
+    if not (targets.shape == (n, 2) and targets.is_contiguous() and targets.element_size() == 4
+            and targets.get_device() == dev and err.get_device() == dev):
+        raise HlkvError("rotary_append: targets is a contiguous int32 [n, 2], on k's device as err is")
+    steps, axes = positions.stride(), rotary.axes
+    if not (positions.shape[0] == n and positions.element_size() == 4 and positions.get_device() == dev
+            and (len(steps) == 2 and positions.shape[1] >= axes or len(steps) == 1 and axes == 1)):
+        raise HlkvError("rotary_append: positions is an int32 [n] or [n, axes] on k's device")
+    heads = layout.kv_heads
+    ks = _token_stride(k, "rotary_append: k", n, heads, layout, dev)
+    vs = _token_stride(v, "rotary_append: v", n, heads, layout, dev)
+    qh = qs = os_ = 0
     if q is not None:
-        heads = int(q.shape[1])
-        _heads(q, "rotary_append: q", layout, n)
-        _heads(q_out, "rotary_append: q_out", layout, n, heads)
-    for t in (targets, positions, v, q, q_out, err):
-        _need(t is None or t.device == k.device, "rotary_append: tensors on one device")
-    st = lib().hlkv_rotary_append(C.byref(pools), C.byref(layout), table_ptr or None, table_size, targets.data_ptr(), n,
-                                  C.byref(rotary), positions.data_ptr(), positions.stride(0),
-                                  positions.stride(1) if positions.dim() == 2 else 0, _ptr(q), heads,
-                                  _token_stride(q) if heads else 0, k.data_ptr(), _token_stride(k), v.data_ptr(),
-                                  _token_stride(v), _ptr(q_out), _token_stride(q_out) if heads else 0, _ptr(err),
+        qh = q.shape[1]
+        qs = _token_stride(q, "rotary_append: q", n, qh, layout, dev)
+        os_ = _token_stride(q_out, "rotary_append: q_out", n, qh, layout, dev)
+    st = lib().hlkv_rotary_append(pools, layout, table_ptr or None, table_size, targets.data_ptr(), n, rotary,
+                                  positions.data_ptr(), steps[0], steps[1] if len(steps) == 2 else 0, _ptr(q), qh, qs,
+                                  k.data_ptr(), ks, v.data_ptr(), vs, _ptr(q_out) if qh else None, os_, err.data_ptr(),
                                   _stream_handle(stream))
-    check(st, "hlkv_rotary_append")
+    if st != OK:
+        check(st, "hlkv_rotary_append")
     return st
 
 
 def batch_attention_workspace_bytes(plan: BatchPlan, layout: Layout, q_heads: int) -> int:
     """Workspace that batch_attention needs for this plan on its device."""
-    if plan.device.index != _current_device():
-        return _on_device_of(plan.blocks, batch_attention_workspace_bytes, plan, layout, q_heads)
-    return lib().hlkv_batch_attention_workspace_bytes(C.byref(plan.c), C.byref(layout), q_heads)
+    if _elsewhere(plan.index):
+        return _on_device(plan.index, batch_attention_workspace_bytes, plan, layout, q_heads)
+    return lib().hlkv_batch_attention_workspace_bytes(plan.c, layout, q_heads)
 
 
 def batch_attention(pools: Pools, layout: Layout, plan: BatchPlan, q, softmax_scale: float, out, err, workspace=None,
@@ -819,19 +834,24 @@ def batch_attention(pools: Pools, layout: Layout, plan: BatchPlan, q, softmax_sc
     """Attention of the plan's new tokens over their sequences' blocks.  q, out: device 16-bit
     [token_cap, q_heads, head_dim] with free token strides; workspace: a device tensor of
     batch_attention_workspace_bytes(...) bytes.  Raises on a non-OK status."""
-    if plan.device.index != _current_device():
-        return _on_device_of(plan.blocks, batch_attention, pools, layout, plan, q, softmax_scale, out, err, workspace,
-                             stream)
-    heads = int(q.shape[1])
-    _heads(q, "batch_attention: q", layout, plan.c.token_cap)
-    _heads(out, "batch_attention: out", layout, plan.c.token_cap, heads)
-    _need(q.device == plan.device and out.device == plan.device and err.device == plan.device
-          and (workspace is None or workspace.device == plan.device), "batch_attention: tensors on the plan's device")
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    st = lib().hlkv_batch_attention(C.byref(pools), C.byref(layout), C.byref(plan.c), q.data_ptr(), heads,
-                                    _token_stride(q), softmax_scale, _ptr(workspace) if ws_bytes else None, ws_bytes,
-                                    out.data_ptr(), _token_stride(out), _ptr(err), _stream_handle(stream))
-    check(st, "hlkv_batch_attention")
+    dev = plan.index
+    if _elsewhere(dev):
+        return _on_device(dev, batch_attention, pools, layout, plan, q, softmax_scale, out, err, workspace, stream)
+    heads, n = q.shape[1], plan.token_cap
+    qs = _token_stride(q, "batch_attention: q", n, heads, layout, dev)
+    os_ = _token_stride(out, "batch_attention: out", n, heads, layout, dev)
+    ws_bytes = 0
+    if workspace is not None:
+        ws_bytes = workspace.numel() * workspace.element_size()
+        if not workspace.is_contiguous():
+            raise HlkvError("batch_attention: a contiguous workspace")
+    if err.get_device() != dev or (ws_bytes and workspace.get_device() != dev):
+        raise HlkvError("batch_attention: tensors on the plan's device")
+    st = lib().hlkv_batch_attention(pools, layout, plan.c, q.data_ptr(), heads, qs, softmax_scale,
+                                    workspace.data_ptr() if ws_bytes else None, ws_bytes, out.data_ptr(), os_, err.data_ptr(),
+                                    _stream_handle(stream))
+    if st != OK:
+        check(st, "hlkv_batch_attention")
     return st
 
 
