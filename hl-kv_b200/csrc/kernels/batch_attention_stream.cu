@@ -705,6 +705,7 @@ struct Producer {
   uint32_t oldest = 0;  // the first stage whose data is still in use
   uint32_t head = 0;
   uint32_t first_st = 0;  // of the piece
+  bool finished = false;
   bool ok = true;
 
   __device__ __forceinline__ void pop() {
@@ -908,11 +909,16 @@ struct Producer {
         __syncwarp();
         uint32_t first;
         const uint32_t count = count_of(p, i, &first);
+        finished = x1 - ub <= w;  // the share ends in this piece
         piece(first, count, lo, hi);
       }
       base += uint64_t{p.head_groups} * w;
     }
-    for (uint32_t k = 0; k < C::kStep && ok; ++k) emit(0, 0, false, kDone);
+    if (!finished) {  // no piece: a share without work
+      if (lane == 0) sh.pieces[half] = Piece{};
+      __syncwarp();
+      for (uint32_t k = 0; k < C::kStep && ok; ++k) emit(0, 0, false, kDone);
+    }
   }
 
   // The blocks of a unit whose cost begins in [lo, hi).
@@ -972,7 +978,7 @@ struct Producer {
       j0 += 32;
     }
     const uint32_t done = st - first_st, fill = (C::kStep - done % C::kStep) % C::kStep + C::kStep;
-    for (uint32_t k = 0; k < fill && ok; ++k) emit(0, 0, false, kFirstStages | (k + C::kStep >= fill ? kLast : 0u));
+    for (uint32_t k = 0; k < fill && ok; ++k) emit(0, 0, false, kFirstStages | (k + C::kStep >= fill ? kLast | (finished ? kDone : 0u) : 0u));
   }
 };
 
@@ -1076,7 +1082,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
     }
     const uint32_t m = stages_at + si * static_cast<uint32_t>(sizeof(Stage));  // address of its description
     constexpr uint32_t kHead = offsetof(Stage, tiles), kHead2 = offsetof(Stage, heads);
-    if (lds32(m + kHead + 4) & kDone) break;
+    if ((lds32(m + kHead + 4) & (kDone | kLast)) == kDone) break;  // a share without work
     if (lds32(m + kHead + 4) & kFirst) {
       WarpRows<kD, kNB>* wr = reinterpret_cast<WarpRows<kD, kNB>*>(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp;
       const uint32_t heads = lds32(m + kHead2), seq = lds32(m + kHead + 8), head0 = lds32(m + kHead + 12);
@@ -1225,23 +1231,27 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
         if (lane == 0) atomicOr(p.err, dev::kErrInternal);
         break;
       }
+      if (flags & kDone) break;
     }
   }
 }
 
-// Joins the partial results of the units that several CTAs took: one CTA per (sequence, head, row), its warps
-// taking the partials in turn, each with its own running maximum.  Also writes the zeros of rows whose sequence
-// lists no block.
-constexpr int kMergeWarps = 8;
-template <int kD>
+// Joins the partial results of the units that several CTAs took: kSplit warps for each (sequence, head, row), taking
+// the partials in turn with a running maximum of their own.  Also writes the zeros of rows whose sequence lists
+// no block.
+constexpr uint32_t kMergeWarps = 8;
+template <int kD, uint32_t kSplit>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Params p) {
   constexpr int kPad = kD + 4, kPer = kD / 32;  // floats of a row; elements of a lane
-  __shared__ float s_o[kMergeWarps][kD];
+  __shared__ float s_o[kSplit > 1 ? kMergeWarps : 1][kD];
   __shared__ float2 s_ml[kMergeWarps];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t r = blockIdx.x % p.slot_rows, unit_head = blockIdx.x / p.slot_rows;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kSplit;
+  const uint32_t id = blockIdx.x * (kMergeWarps / kSplit) + warp / kSplit;
+  const uint32_t r = id % p.slot_rows, unit_head = id / p.slot_rows;
   const uint32_t i = unit_head / p.H, head = unit_head % p.H, hg = head / 8, h = head % 8;
   dev::wait_for_prerequisites();
+  // (uniform over the warps of a row; with kSplit > 1 a CTA has one row)
+  if (i >= p.nseq) return;
   const Rows rows = rows_of(p, i);
   const uint32_t n_rows = rows.q * p.group;
   if (r >= n_rows || uint64_t{rows.q} * p.group > kStreamRows) return;
@@ -1262,8 +1272,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
     const float* base = p.partial + (c0 + uint64_t{i} * p.head_groups + hg) * step + (uint64_t{h} * p.slot_rows + r) * kPad;
     // a CTA whose range is empty (more CTAs than cost) took nothing and may have written nothing
     auto empty = [&](uint32_t c) { return p.ctas > W && c * W / p.ctas == (uint64_t{c} + 1) * W / p.ctas; };
-#pragma unroll 2
-    for (uint32_t c = c0 + warp; c <= c1; c += kMergeWarps) {
+#pragma unroll 4
+    for (uint32_t c = c0 + part; c <= c1; c += kSplit) {
       if (empty(c)) continue;
       const float* s = base + (c - c0) * step;
       const float2 ml = *reinterpret_cast<const float2*>(s + kD);
@@ -1278,26 +1288,36 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
       for (int k = 0; k < kPer; ++k) o[k] = fmaf(o[k], fo, x[k] * ft);
     }
   }
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) s_o[warp][lane * kPer + k] = o[k];
-  if (lane == 0) s_ml[warp] = make_float2(M, L);
-  __syncthreads();
-  const uint32_t e = threadIdx.x;
-  if (e >= kD) return;
-  M = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < kMergeWarps; ++k) M = fmaxf(M, s_ml[k].x);
-  float sum = 0.0f;
-  L = 0.0f;
-#pragma unroll
-  for (int k = 0; k < kMergeWarps; ++k) {
-    const float a = M == -INFINITY ? 1.0f : exp2f(s_ml[k].x - M);
-    L = fmaf(s_ml[k].y, a, L);
-    sum = fmaf(s_o[k][e], a, sum);
-  }
-  if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros
   const uint32_t tok = r / p.group, gi = r % p.group;
-  p.out[(rows.first + tok) * p.out_stride + uint64_t{head * p.group + gi} * kD + e] = __half_as_ushort(__float2half_rn(sum / L));
+  uint16_t* dst = p.out + (rows.first + tok) * p.out_stride + uint64_t{head * p.group + gi} * kD;
+  if constexpr (kSplit == 1) {
+    if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros
+    if constexpr (kPer == 4) {
+      *reinterpret_cast<uint2*>(dst + 4 * lane) = make_uint2(dev::pack_f16x2(o[0] / L, o[1] / L), dev::pack_f16x2(o[2] / L, o[3] / L));
+    } else {
+      *reinterpret_cast<uint32_t*>(dst + 2 * lane) = dev::pack_f16x2(o[0] / L, o[1] / L);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) s_o[warp][lane * kPer + k] = o[k];
+    if (lane == 0) s_ml[warp] = make_float2(M, L);
+    __syncthreads();
+    const uint32_t e = threadIdx.x;
+    if (e >= kD) return;
+    M = -INFINITY;
+#pragma unroll
+    for (uint32_t k = 0; k < kSplit; ++k) M = fmaxf(M, s_ml[k].x);
+    float sum = 0.0f;
+    L = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < kSplit; ++k) {
+      const float a = M == -INFINITY ? 1.0f : exp2f(s_ml[k].x - M);
+      L = fmaf(s_ml[k].y, a, L);
+      sum = fmaf(s_o[k][e], a, sum);
+    }
+    if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros
+    dst[e] = __half_as_ushort(__float2half_rn(sum / L));
+  }
 }
 
 template <int kD, bool kTwo>
@@ -1311,7 +1331,6 @@ cudaError_t launch(const Params& p, cudaStream_t s) {
   if (e2 != cudaSuccess) return e2;
   // The merge's CTAs start while the stream's last ones run, and wait for them.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.nseq * p.H * p.slot_rows);
   cfg.blockDim = dim3(kMergeWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -1319,7 +1338,15 @@ cudaError_t launch(const Params& p, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<kD>, p);
+  // A warp a row where a unit has few partials (32 windows of 16 rows, 5 each: 3 us against 12 us), a CTA a row where it
+  // has many (4 short sequences, 37 each).
+  const uint32_t rows = p.nseq * p.H * p.slot_rows;
+  if (uint64_t{p.nseq} * p.head_groups * 12 > p.ctas) {
+    cfg.gridDim = dim3((rows + kMergeWarps - 1) / kMergeWarps);
+    return cudaLaunchKernelEx(&cfg, merge_kernel<kD, 1>, p);
+  }
+  cfg.gridDim = dim3(rows);
+  return cudaLaunchKernelEx(&cfg, merge_kernel<kD, kMergeWarps>, p);
 }
 
 uint64_t prefix_bytes(uint32_t nseq) { return ((uint64_t{nseq} + 1) * 8 + 15) / 16 * 16; }

@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
   const uint32_t n_ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const uint32_t i = blockIdx.x / n_ctas;
   const HlkvBatchPlan& plan = p.plan;
+  if (n_ctas > 1) cluster.barrier_arrive();  // waited for before the first write into another CTA's shared memory
   const uint2 seg = p.segs[i];
   const uint32_t q = p.qlens ? __ldg(p.qlens + i) : 1u;
   uint64_t first, tfirst;
@@ -201,6 +202,7 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
   Sum before{0, 0, 0}, total{0, 0, 0};
   if (one_round) {
     load(0);
+    if (n_ctas > 1) cluster.barrier_wait();
     before = cluster_scan(cluster, s, own_sum(), phase++, &total);
   } else {
     Sum x{0, 0, 0};
@@ -208,6 +210,7 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
       load(static_cast<uint32_t>(base));
       x = x + own_sum();
     }
+    if (n_ctas > 1) cluster.barrier_wait();
     cluster_scan(cluster, s, x, phase++, &total);
   }
   const uint32_t context = total.tokens;
