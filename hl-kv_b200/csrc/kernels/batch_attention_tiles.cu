@@ -37,12 +37,18 @@ struct Config {
   static constexpr uint32_t kSmem = kEnd + 1024;  // the operands start on 1024 bytes
 };
 
+// 256 rows of a sequence.
+struct RowTile {
+  uint32_t seq, tile;  // tile 0xFFFFFFFF: none
+};
+
 struct Shared {
+  RowTile mine;
   uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];  // of the two stages
   uint64_t s_full[2], p_full[2], o_done[2];               // of the two accumulator tiles
   // Of the tokens of the last four tiles: a K half may be written again while the softmax of the tile two before
   // still reads these.
-  float ks[4][kTile], kb[4][kTile], vs[4][kTile], vb[4][kTile];
+  alignas(16) float ks[4][kTile], kb[4][kTile], vs[4][kTile], vb[4][kTile];  // read four at a time
   int exponent[4][kStageWarps];
   uint32_t kind[4][kStageWarps];  // of 16 tokens: 1 a scale, 2 a bias, 4 some token does not exist
   uint32_t exists[4][kStageWarps];
@@ -213,6 +219,64 @@ struct Walk {
   }
 };
 
+// The r-th (sequence, row tile) of the batch when they are ordered by the tiles of tokens that they walk, most first:
+// CTAs start in that order, and the last ones to end are short.  Found by a warp: the level of r by bisection over
+// counts (a sequence's tiles of a level and above are its last ones), then its place among the level's tiles.
+constexpr uint32_t kOrdered = 256;  // most sequences to look through
+__device__ __forceinline__ RowTile row_tile_of_rank(const Params& p, uint32_t r) {
+  const uint32_t lane = threadIdx.x & 31;
+  // A tile sees at most `cap` tokens; its level is its last token's tile of 128, or the one of the cap.
+  const uint64_t cap64 = p.window == 0 ? 0x7FFFFFFFu : uint64_t{p.window} + p.sinks + kRowsCta / p.group + 1;
+  const uint32_t cap = static_cast<uint32_t>(min(cap64, uint64_t{0x7FFFFFFFu}));
+  // Row tiles of sequence i at level x and above: from the first one whose last token lies behind (x - 1) 128.
+  auto above = [&](uint32_t i, uint32_t x) -> uint32_t {
+    const Rows rows = rows_of(p, i);
+    const uint64_t n_rows = uint64_t{rows.q} * p.group;
+    if (n_rows <= kStreamRows) return 0u;
+    const uint32_t n = static_cast<uint32_t>((n_rows + kRowsCta - 1) / kRowsCta);
+    if (x == 0) return n;
+    const uint64_t from = uint64_t{x - 1} * kTile;
+    const int64_t tok = static_cast<int64_t>(from) - (int64_t{p.context[i]} - rows.q);  // that token as a new one
+    if (from >= cap || tok >= int64_t{rows.q}) return 0u;
+    return tok <= 0 ? n : n - static_cast<uint32_t>(uint64_t(tok) * p.group / kRowsCta);
+  };
+  auto count = [&](uint32_t x) {
+    uint32_t c = 0;
+    for (uint32_t i = lane; i < p.nseq; i += 32) c += above(i, x);
+    return __reduce_add_sync(0xFFFFFFFFu, c);
+  };
+  uint32_t longest = 0;
+  for (uint32_t i = lane; i < p.nseq; i += 32) longest = max(longest, min(p.context[i], cap));
+  uint32_t lo = 0, hi = (__reduce_max_sync(0xFFFFFFFFu, longest) + kTile - 1) / kTile + 1;  // count(hi) == 0
+  if (r >= count(0)) return RowTile{0u, 0xFFFFFFFFu};
+  while (hi - lo > 1) {
+    const uint32_t x = (lo + hi) / 2;
+    if (count(x) > r) lo = x;
+    else hi = x;
+  }
+  uint32_t left = r - count(lo + 1);  // place among the level's tiles
+  for (uint32_t base = 0; base < p.nseq; base += 32) {
+    const uint32_t i = base + lane;
+    const uint32_t more = i < p.nseq ? above(i, lo) : 0u, less = i < p.nseq ? above(i, lo + 1) : 0u;
+    uint32_t upto = more - less;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= static_cast<uint32_t>(o)) upto += y;
+    }
+    const uint32_t here = __ballot_sync(0xFFFFFFFFu, upto > left);
+    if (here != 0) {
+      const uint32_t owner = __ffs(here) - 1;
+      const uint32_t before = __shfl_sync(0xFFFFFFFFu, upto - (more - less), owner), above_it = __shfl_sync(0xFFFFFFFFu, less, owner);
+      const uint32_t seq = base + owner;
+      const uint32_t n = static_cast<uint32_t>((uint64_t{rows_of(p, seq).q} * p.group + kRowsCta - 1) / kRowsCta);
+      return RowTile{seq, n - 1 - above_it - (left - before)};
+    }
+    left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+  }
+  return RowTile{0u, 0xFFFFFFFFu};
+}
+
 template <int kD>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ Params p) {
   using C = Config<kD>;
@@ -221,14 +285,27 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
 
-  // ---- the CTA's rows: tiles of the longest contexts first
-  const uint32_t units = p.nseq * p.H, tiles_max = gridDim.x / units;
-  const uint32_t unit = blockIdx.x % units, seq = unit / p.H, h = unit % p.H;
+  // ---- the CTA's rows: those that see most tokens first; the heads of the same rows side by side, since a token's
+  // heads lie together
+  const uint32_t h = blockIdx.x % p.H;
+  RowTile mine;
+  if (p.nseq <= kOrdered) {
+    if (warp == 0) {
+      mine = row_tile_of_rank(p, blockIdx.x / p.H);
+      if (lane == 0) sh.mine = mine;
+    }
+    __syncthreads();
+    mine = sh.mine;
+  } else {  // last tiles of all sequences first
+    const uint32_t seq = blockIdx.x / p.H % p.nseq, order = blockIdx.x / p.H / p.nseq;
+    const uint64_t n_rows = uint64_t{rows_of(p, seq).q} * p.group, n = (n_rows + kRowsCta - 1) / kRowsCta;
+    mine = RowTile{seq, n_rows > kStreamRows && order < n ? static_cast<uint32_t>(n) - 1 - order : 0xFFFFFFFFu};
+  }
+  if (mine.tile == 0xFFFFFFFFu) return;
+  const uint32_t seq = mine.seq;
   const Rows rows = rows_of(p, seq);
-  const uint32_t n_rows = rows.q * p.group, row_tiles = (n_rows + kRowsCta - 1) / kRowsCta;
-  const uint32_t order = blockIdx.x / units;
-  if (n_rows <= kStreamRows || order >= row_tiles || tiles_max == 0) return;
-  const uint32_t row0 = (row_tiles - 1 - order) * kRowsCta, rows_here = min(kRowsCta, n_rows - row0);
+  const uint32_t n_rows = rows.q * p.group;
+  const uint32_t row0 = mine.tile * kRowsCta, rows_here = min(kRowsCta, n_rows - row0);
   const uint32_t n_acc = rows_here > 128 ? 2 : 1;
   const uint32_t ctx = p.context[seq];
   const int32_t pos_base = static_cast<int32_t>(ctx) - static_cast<int32_t>(rows.q);  // of the first new token
@@ -293,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const uint32_t tok = row / p.group, head = h * p.group + row % p.group;
     const int32_t pos = pos_base + static_cast<int32_t>(tok);
     // the first token of the window
-  const int32_t low = p.window == 0 ? -1 : static_cast<int32_t>(max(int64_t{pos} - p.window + 1, int64_t{-1}));
+    const int32_t low = p.window == 0 ? -1 : static_cast<int32_t>(max(int64_t{pos} - p.window + 1, int64_t{-1}));
     float qsum = 0.0f;
     if (live) {
       const uint4* src = reinterpret_cast<const uint4*>(p.q + (rows.first + tok) * p.q_stride + uint64_t{head} * kD);
@@ -399,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // it by more than 8 (weights reach 2^8 at most), the maximum moves, and what was made with the old one
         // (O, the sums, this tile's weights so far) is scaled.
 #pragma unroll 1
-        for (uint32_t c = 0; c < 4; ++c) {
+        for (uint32_t c = 0; c < (n + 31) / 32; ++c) {  // the products take no further tokens
           // a group's weights are in units of 2^(its exponent), the sums in their own
           const uint32_t kind0 = sh.kind[info][2 * c], kind1 = sh.kind[info][2 * c + 1];
           const int d0 = (kind0 & 3u ? min(max(sh.exponent[info][2 * c], -60), 60) : 0) - E;
@@ -762,9 +839,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           if (!ok) break;
           fence_after();
           const uint32_t v = base + C::kV + (j & 1) * C::kOperand;
+          uint32_t tp, n;
+          walk.tile(j, &tp, &n);
+          const uint32_t steps = (n + 31) / 32 * 2;
 #pragma unroll
           for (uint32_t s = 0; s < kTile / 16; ++s) {
-            mma_ts(tmem + 256 + acc * kD, tmem + acc * 128 + s * 8, desc(v + s * 2048, C::kPanel, 1024), kIdO, j > 0 || s > 0);
+            if (s < steps) mma_ts(tmem + 256 + acc * kD, tmem + acc * 128 + s * 8, desc(v + s * 2048, C::kPanel, 1024), kIdO, j > 0 || s > 0);
           }
           commit(&sh.o_done[acc]);
           if (j + 1 < n_tiles) {
