@@ -96,8 +96,10 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   p.qscale = softmax_scale * kLog2e;
   p.ctas = static_cast<uint32_t>(sm_count());
   stream_layout(&p, d_workspace);
+  const uint64_t tiles = p.max_rows <= kStreamRows ? 0u : tile_ctas(p);
+  if (tiles > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const cudaError_t e = launch_stream(layout->head_dim, p, s);
-  if (e != cudaSuccess || p.max_rows <= kStreamRows) return cuda_status(e);
+  if (e != cudaSuccess || tiles == 0) return cuda_status(e);
   return cuda_status(launch_tiles(layout->head_dim, p, s));
 }

@@ -280,6 +280,7 @@ struct SharedMemoryOnce {
 cudaError_t launch_stream(uint32_t head_dim, const Params& p, cudaStream_t s);
 size_t stream_workspace(uint32_t nseq, uint32_t H, uint32_t head_dim, uint32_t max_rows, uint32_t ctas);
 void stream_layout(Params* p, void* ws);
+uint64_t tile_ctas(const Params& p);  // the tile kernel's grid: 0 when no sequence can have its rows
 cudaError_t launch_tiles(uint32_t head_dim, const Params& p, cudaStream_t s);
 
 }  // namespace battn

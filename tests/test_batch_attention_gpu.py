@@ -143,6 +143,43 @@ def test_uneven_batch(hlkv_lib, cuda_device):
     b.check(8, seed=2)
 
 
+@pytest.mark.parametrize("nseq", [128, 129])
+@pytest.mark.parametrize("window", [0, 40])
+def test_many_sequences_of_many_rows(hlkv_lib, cuda_device, nseq, window):
+    """Both orders of the tiles' CTAs: every row of every sequence once, next to short ones and absent ones."""
+    rng = np.random.default_rng(nseq)
+    q = [int(rng.choice([0, 1, 5, 17, 40, 140])) for _ in range(nseq)]
+    vt = [[16] * (n // 16 + int(rng.integers(0, 6))) + [n % 16 or 16] for n in q]
+    b = Batch(hlkv_lib, 16, 1, 64, vt, q, window=window, sinks=3 if window else 0, seed=nseq, pad=3)
+    b.check(3, seed=1)
+
+
+@pytest.mark.parametrize("q", [[30], [200, 17], [17, 0, 20]])
+def test_no_sequence_of_few_rows(hlkv_lib, cuda_device, q):
+    """Nothing for the streaming kernel to do."""
+    rng = np.random.default_rng(len(q))
+    b = Batch(hlkv_lib, 16, 1, 128, _vt(rng, 16, [20] * len(q), partial=0), q, seed=2)
+    b.check(32, seed=1)
+
+
+@pytest.mark.parametrize("group", [4, 32])
+def test_plan_larger_than_its_batch(hlkv_lib, cuda_device, group):
+    """A plan made for prompts that holds a decode step, and one with room for many more tokens."""
+    import torch
+    rng = np.random.default_rng(3)
+    for q in ([1, 1, 1], [1, 60, 2]):
+        b = Batch(hlkv_lib, 16, 1, 64, _vt(rng, 16, [20, 9, 30], partial=0), q, seed=2, pad=500)
+        b.plan = hlkv_lib.BatchPlan(3, b.plan.c.block_cap + 70, b.cap, 8192, 0, 0)
+        b.fill_plan()
+        x, d_q = b.queries(group, 1)
+        got = b.run(d_q, 0.125)
+        torch.cuda.synchronize()
+        want, tol, err = b.want(x, 0.125)
+        assert int(b.err.item()) == err == 0
+        close(got, want, tol, sum(q))
+        assert (got[sum(q):] == 0x1234).all()
+
+
 def _poke(wl, rng, what):
     """Overwrites cached rows: what = {(seq, position): value} in FP16 blocks of full tokens."""
     buf, sb, _ = wl.pools[0]
