@@ -42,7 +42,7 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   const uint64_t D = layout->head_dim;
   if (D != 64 && D != 128) return HLKV_INVALID_ARGUMENT;
   const uint32_t H = layout->kv_heads;
-  if (q_heads == 0 || q_heads % H != 0 || q_heads / H > kMaxGroup) return HLKV_INVALID_ARGUMENT;
+  if (H > kMaxKvHeads || q_heads == 0 || q_heads % H != 0 || q_heads / H > kMaxGroup) return HLKV_INVALID_ARGUMENT;
   if (!(softmax_scale > 0.0f) || !std::isfinite(softmax_scale)) return HLKV_INVALID_ARGUMENT;
   if (plan->nseq == 0 || plan->token_cap == 0) return HLKV_OK;
   if (plan->d_block_first == nullptr || plan->d_block_count == nullptr || plan->d_token_first == nullptr ||

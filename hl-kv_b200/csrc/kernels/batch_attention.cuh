@@ -16,7 +16,7 @@ namespace hlkv {
 namespace battn {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kMaxGroup = 32;
+constexpr uint32_t kMaxGroup = 32, kMaxKvHeads = 128;  // (a token's parameters of all heads come in one copy)
 // Sequences whose query rows per KV head (new tokens x group) are at most this many are streamed
 // (stream_kernel); the others go to the tile kernel.
 constexpr uint32_t kStreamRows = 16;

@@ -81,6 +81,7 @@ struct Config {
 struct Piece {
   uint32_t seq, head0, heads, slot, direct, single, q;
   int32_t pos0;  // of the first new token
+  uint32_t fit;  // tiles of any format that the ring holds: a copy's parameters are those of all heads
 };
 
 struct Shared {
@@ -849,11 +850,11 @@ struct Producer {
     // bit k: jobs k and k + 1 are alike and may share a step
     const uint32_t alike = __ballot_sync(0xFFFFFFFFu, lane + 1 < count && fn == next && fn >> 8 == (1u << 8 | 16u) && (fn & 0xFFu) != dev::kFp16);
     __syncwarp();
-    const uint32_t single = sh.pieces[half].single;
+    const uint32_t single = sh.pieces[half].single, fit = sh.pieces[half].fit;
     for (uint32_t from = 0, tiles; from < count && ok; from += tiles) {
       const uint32_t links = (1u << (2 * single - 1)) - 1u;
-      const bool pairs = ((alike >> from) & links) == links;
-      tiles = pairs ? 2 * single : min(single, count - from);
+      const bool pairs = 2 * single <= fit && ((alike >> from) & links) == links;
+      tiles = pairs ? 2 * single : min(min(single, fit), count - from);
       emit(from, tiles, pairs, kFirstStages);
     }
   }
@@ -903,6 +904,8 @@ struct Producer {
           pc.slot = blockIdx.x + i * p.head_groups + hg;
           pc.direct = lo == 0 && hi == w ? kDirect : 0u;
           pc.single = heads > 4 ? 1u : heads > 2 ? 2u : heads > 1 ? 4u : 8u;  // tiles that occupy a group's warps
+          const uint32_t codes = 16 * heads * kD, params = 16 * p.H * 4 + 32;
+          pc.fit = C::kRing / max(2 * codes, max(codes + params, codes / 2 + 2 * params));
           pc.q = rows.q;
           pc.pos0 = static_cast<int32_t>(p.context[i] - rows.q);
         }

@@ -128,6 +128,16 @@ def test_several_new_tokens(hlkv_lib, cuda_device, T, H, D, group, q, window, si
     b.check(H * group, seed=group)
 
 
+@pytest.mark.parametrize("H,D", [(33, 128), (58, 128), (41, 64), (100, 64), (128, 128)])
+@pytest.mark.parametrize("probs", [(0, 0, 0, 1), (1, 1, 1, 1)])
+def test_many_heads(hlkv_lib, cuda_device, H, D, probs):
+    """A token's parameters of all heads next to the codes of the last few: the ring holds fewer tiles."""
+    rng = np.random.default_rng(H)
+    for q in ([1, 1], [20, 1]):
+        b = Batch(hlkv_lib, 16, H, D, _vt(rng, 16, [20, 45]), q, probs=probs, seed=H)
+        b.check(H, seed=1)
+
+
 def test_long_context_and_few_rows(hlkv_lib, cuda_device):
     """The work of one sequence spread over the GPU, at decode and with a chunk."""
     rng = np.random.default_rng(0)

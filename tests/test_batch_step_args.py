@@ -89,7 +89,9 @@ def test_attention_arguments(hlkv_lib):
                dict(scale=float("nan")), dict(layout=hlkv_lib.Layout(16, 8, 256, 1)), dict(layout=hlkv_lib.Layout(1024, 8, 128, 1)),
                dict(plan=_plan(hlkv_lib, blocks=None)), dict(plan=_plan(hlkv_lib, blocks=4104)),
                dict(plan=_plan(hlkv_lib, context=None)), dict(plan=_plan(hlkv_lib, token_first=None)),
-               dict(ws=None), dict(ws=ODD), dict(plan=_plan(hlkv_lib, max_query=0)), dict(plan=_plan(hlkv_lib, block_cost=None)), dict(plan=_plan(hlkv_lib, cost=None)), dict(plan=_plan(hlkv_lib, token_cap=1 << 30))):
+               dict(ws=None), dict(ws=ODD), dict(plan=_plan(hlkv_lib, max_query=0)), dict(plan=_plan(hlkv_lib, block_cost=None)), dict(plan=_plan(hlkv_lib, cost=None)), dict(plan=_plan(hlkv_lib, token_cap=1 << 30)),
+               dict(layout=hlkv_lib.Layout(16, 129, 128, 1), heads=129, qs=129 * 128, os=129 * 128),
+               dict(plan=_plan(hlkv_lib, nseq=1 << 20, max_query=1 << 20))):
         assert call(**kw) == INV, kw
     assert L.hlkv_last_cuda_error() == 0
     need = L.hlkv_batch_attention_workspace_bytes(C.byref(_plan(hlkv_lib)), C.byref(hlkv_lib.Layout(16, 8, 128, 1)), 32)
