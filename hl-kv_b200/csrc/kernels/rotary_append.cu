@@ -106,6 +106,10 @@ __device__ __forceinline__ float turned_y(float x, float y, float2 cs) {
   return __fadd_rn(__fmul_rn(y, cs.x), __fmul_rn(x, cs.y));
 }
 
+// Scales whose reciprocal, and so the bracket around a quotient, is exact to 2^-24: outside of them (a factor far from
+// one) the reciprocal overflows or is subnormal, and every quotient is a division.
+__device__ __forceinline__ bool reciprocal_ok(float scale) { return scale >= 0x1p-126f && scale <= 0x1p126f; }
+
 // One row of binary32 values (two chunks of 8 per lane) in format f into row `row` of a slot.  The
 // rules are dev::encode_row's (the reference's quantize_reference) but for the scale, which is the
 // product amax * (1 / max_finite) or range * (1 / 15) with the reciprocal in binary32 instead of the
@@ -150,7 +154,7 @@ __device__ __forceinline__ uint32_t encode_row_f32(uint32_t f, const float (&x)[
         diff |= qa ^ qb;
         word[i / 8] |= min(qa, 15u) << (4 * (i % 8));
       }
-      if (diff != 0) {  // near the middle of two codes: the divisions themselves
+      if (diff != 0 || !reciprocal_ok(scale)) {  // near the middle of two codes: the divisions themselves
         word[0] = word[1] = 0u;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -184,7 +188,7 @@ __device__ __forceinline__ uint32_t encode_row_f32(uint32_t f, const float (&x)[
     r[i] = f == dev::kE4M3 ? dev::cvt_e4m3x2(a0, a1) : dev::cvt_e5m2x2(a0, a1);
     diff |= r[i] ^ (f == dev::kE4M3 ? dev::cvt_e4m3x2(b0, b1) : dev::cvt_e5m2x2(b0, b1));
   }
-  if (diff != 0) {  // near the middle of two codes: the divisions themselves
+  if (diff != 0 || !reciprocal_ok(scale)) {  // near the middle of two codes: the divisions themselves
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float a = __fdiv_rn(x[2 * i], scale), b = __fdiv_rn(x[2 * i + 1], scale);

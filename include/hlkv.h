@@ -455,8 +455,9 @@ int hlkv_rotary_append(const HlkvPools* pools, const HlkvLayout* layout, const H
  * result is rounded to binary16.  A row that sees no token is zeros.  Tokens that a row does not
  * see do not touch it, whatever they hold.
  *  - d_q and d_out: binary16, token rows at the plan's d_token_first[i] + r, heads contiguous
- *    ([q_heads][head_dim]), token strides in elements (multiples of 8), 16-byte aligned.  Rows
- *    behind the last new token are left as they were.
+ *    ([q_heads][head_dim]), token strides in elements (multiples of 8), 16-byte aligned; d_out
+ *    overlaps nothing else.  Rows behind the last new token are left as they were; those of a
+ *    sequence that the plan could not hold (HLKV_ERR_PLAN_RANGE) are zeros or as they were.
  *  - head_dim 64 or 128; kv_heads at most 128; q_heads / kv_heads 1 .. 32; softmax_scale finite
  *    and > 0.
  *  - d_workspace: 16-byte aligned, hlkv_batch_attention_workspace_bytes(plan, layout, q_heads)

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from batch_helpers import E4M3, E5M2, FP16, INT4, PAD, rotate
-from helpers import host_pools
+from helpers import device_table_words, host_pools
 
 pytestmark = pytest.mark.gpu
 
@@ -207,3 +207,29 @@ def test_factor_scales_the_rotation(hlkv_lib, cuda_device):
     want[..., :32] *= 1.5
     got = out.cpu().numpy().view(np.float16).astype(np.float64)
     assert (np.abs(got - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -20 * 1.5 * np.abs(x).max()).all()
+
+
+@pytest.mark.parametrize("factor", [2.0 ** -136, 2.0 ** -128, 1e34])
+def test_scales_whose_reciprocal_is_not_normal(hlkv_lib, cuda_device, factor):
+    """At position 0 K is x times the factor: rows so small or large that the scale's reciprocal overflows or is
+    subnormal still get the quotients' codes."""
+    import torch
+    T, H, D, n = 16, 2, 64, 40
+    wl, rng, targets = _setup(T, H, D, n, seed=3)
+    x = rng.standard_normal((n, 3 * H, D)).astype(np.float16)
+    d = torch.from_numpy(x.view(np.int16)).cuda()
+    q, k, v = d.split((H, H, H), 1)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want, table = host_pools(wl), device_table_words(wl)
+    hlkv_lib.rotary_append(wl.hlkv_pools(), wl.layout, wl.dt.table_ptr, wl.dt.table_size,
+                           torch.from_numpy(targets.view(np.int32)).cuda(), hlkv_lib.make_rotary(_freqs(32), factor=factor),
+                           torch.zeros(n, dtype=torch.int32, device="cuda"), q, k, v, torch.zeros_like(q.contiguous()), err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    with np.errstate(over="ignore"):
+        for i in range(n):
+            rows = np.stack([x[i, H:2 * H].astype(np.float32) * np.float32(factor), x[i, 2 * H:].astype(np.float32)])
+            _store(want, table, T, H, D, targets[i], rows)
+    got = host_pools(wl)
+    for f in want:
+        assert np.array_equal(got[f][0], want[f][0]), f
