@@ -15,6 +15,16 @@
 // rounded once, to binary16, in units of 2^E that follow the exponents of the value scales (one for 16 tokens).
 // Codes are laid in the order (0, 4, 1, 5, 2, 6, 3, 7) of each 8, where the formats' words hold them: Q's elements
 // lie the same way, and the outputs are put back in order at the end.
+//
+// Measured (8 KV heads of 128, 32 query heads; six chunks of up to 1645 new tokens over contexts of up to 8024, formats
+// mixed): 928 us, 402 TFLOP/s, 0.24 of the matrix rate; the caches of one format alone: FP16 816, E4M3 885, INT4 993 us.
+// The products alone would take 370 us, the conversion without the softmax 640, the softmax without the conversion
+// 950.  The softmax's two warps per scheduler wait on their own chains (an issue every 2.2 cycles), and the per-token
+// parameters are broadcast from shared memory: a float4 load returns 512 bytes to a warp, 2048 cycles of a tile for FP8
+// and 4096 for INT4.  Five prompts of heads of 64 with a window of 1024: 147 us; a CTA there walks ten tiles, of which
+// the last and the sinks' are short.
+// Tried and slower: halves of 64 tokens with scores of their own (1020 us), products issued by a softmax warp (1190),
+// half the loads in flight (1070), FP8 and INT4 rows in 16-byte pieces a tile ahead (985).
 #include <algorithm>
 #include <cmath>
 

@@ -14,6 +14,11 @@
 // distributed shared memory.  A sequence longer than the cluster's kRound blocks is taken in
 // rounds, after a first pass that only adds up its tokens (the window and the new tokens are
 // counted from the end).
+//
+// The bound is latency: launch, the segment, the arena, the descriptor, the scan and the stores follow one another,
+// and the bytes (20 read and at most 20 written for a block) take less than a microsecond.  Measured: 8 sequences of
+// 100 to 900 tokens, 5.3 us; 64 of 8192 tokens, 5.4 us; 48 of 1000 to 131072 with a window, 10.7 us with clusters of up
+// to 8 CTAs a sequence and 43.5 us with one.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
