@@ -17,7 +17,7 @@
 //
 // The bound is latency: launch, the segment, the arena, the descriptor, the scan and the stores follow one another,
 // and the bytes (20 read and at most 20 written for a block) take less than a microsecond.  Measured: 8 sequences of
-// 100 to 900 tokens, 5.3 us; 64 of 8192 tokens, 5.4 us; 48 of 1000 to 131072 with a window, 10.7 us with clusters of up
+// 100 to 900 tokens, 5.3 us; 64 of 8192 tokens, 5.4 us; 48 of 1000 to 131072 with a window, 9.9 us with clusters of up
 // to 8 CTAs a sequence and 43.5 us with one.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
   };
 
   Sum before{0, 0, 0}, total{0, 0, 0};
+  if (threadIdx.x < 4) s.border[threadIdx.x] = 0xFFFFFFFFu;  // written by all after the scan's barrier
   if (one_round) {
     load(0);
     if (n_ctas > 1) cluster.barrier_wait();
@@ -229,9 +230,6 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
   Sum carry{0, 0, 0};
   const uint32_t token_base = static_cast<uint32_t>(tfirst);  // used for rows of a sequence that fits only
   const uint32_t missing = q > context ? q - context : 0u;    // new tokens that the sequence does not have
-  if (threadIdx.x < 4) {
-    s.border[threadIdx.x] = threadIdx.x == 0 ? total.blocks : threadIdx.x == 2 ? total.cost : 0xFFFFFFFFu;
-  }
   for (uint64_t base64 = 0; base64 < n; base64 += round) {
     if (!one_round) {
       load(static_cast<uint32_t>(base64));
@@ -242,10 +240,6 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
     if (trimmed) {
       // The least ranks of a non-empty block behind the sinks and of one in the window, to every
       // CTA of the cluster.  Both conditions hold from some rank on, so the minima are the borders.
-      if (base64 == 0) {
-        __syncthreads();
-        if (n_ctas > 1) cluster.sync();  // every CTA has set its borders
-      }
       uint32_t behind = 0xFFFFFFFFu, within = 0xFFFFFFFFu, cost_behind = 0xFFFFFFFFu, cost_within = 0xFFFFFFFFu;
       Sum x = before;
 #pragma unroll
@@ -278,9 +272,9 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
       }
       if (n_ctas > 1) cluster.sync();
       else __syncthreads();
-      n_first = s.border[0];
+      n_first = min(s.border[0], total.blocks);
       n_skip = s.border[1];
-      cost_first = s.border[2];
+      cost_first = min(s.border[2], total.cost);
       cost_skip = s.border[3];
     }
     const uint32_t skip = max(n_skip, n_first), cost_gap = max(cost_skip, cost_first) - cost_first;
@@ -335,7 +329,7 @@ __global__ void __launch_bounds__(kThreads) batch_plan_kernel(const Params p) {
       }
     }
   }
-  if (n_ctas > 1) cluster.sync();  // no CTA leaves while another may write into its shared memory
+  // (Every write into another CTA's shared memory lies before a barrier of the cluster: no CTA leaves too early.)
 }
 
 // d_block_first and d_token_first of a large batch: one CTA, a chunked scan.  A sum beyond its
