@@ -27,9 +27,10 @@ extern "C" size_t hlkv_batch_attention_workspace_bytes(const HlkvBatchPlan* plan
     return 0;
   }
   const uint64_t rows = uint64_t{plan->max_query} * (q_heads / layout->kv_heads);
-  return hlkv::battn::stream_workspace(plan->nseq, layout->kv_heads, layout->head_dim,
-                                       static_cast<uint32_t>(rows < 0xFFFFFFFFu ? rows : 0xFFFFFFFFu),
-                                       static_cast<uint32_t>(hlkv::sm_count()));
+  const uint32_t max_rows = static_cast<uint32_t>(rows < 0xFFFFFFFFu ? rows : 0xFFFFFFFFu);
+  const uint32_t ctas = static_cast<uint32_t>(hlkv::sm_count());
+  return hlkv::battn::stream_workspace(plan->nseq, layout->kv_heads, layout->head_dim, max_rows, ctas) +
+         hlkv::battn::tile_workspace(plan->nseq, layout->head_dim, max_rows, ctas);
 }
 
 extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* layout, const HlkvBatchPlan* plan,
@@ -43,7 +44,7 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   if (D != 64 && D != 128) return HLKV_INVALID_ARGUMENT;
   const uint32_t H = layout->kv_heads;
   if (H > kMaxKvHeads || q_heads == 0 || q_heads % H != 0 || q_heads / H > kMaxGroup) return HLKV_INVALID_ARGUMENT;
-  if (!(softmax_scale > 0.0f) || !std::isfinite(softmax_scale)) return HLKV_INVALID_ARGUMENT;
+  if (!(softmax_scale > 0.0f) || softmax_scale > 0x1p60f) return HLKV_INVALID_ARGUMENT;
   if (plan->nseq == 0 || plan->token_cap == 0) return HLKV_OK;
   if (plan->d_block_first == nullptr || plan->d_block_count == nullptr || plan->d_token_first == nullptr ||
       plan->d_context == nullptr || plan->d_cost == nullptr ||
@@ -96,6 +97,10 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   p.qscale = softmax_scale * kLog2e;
   p.ctas = static_cast<uint32_t>(sm_count());
   stream_layout(&p, d_workspace);
+  // behind the stream kernel's part, a multiple of 16 bytes
+  p.tile_partial = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) +
+                                            stream_workspace(p.nseq, H, layout->head_dim, p.max_rows, p.ctas));
+  p.tile_redo = reinterpret_cast<uint32_t*>(p.tile_partial + uint64_t{p.ctas} * 256 * (D + 4));
   const uint64_t tiles = p.max_rows <= kStreamRows ? 0u : tile_ctas(p);
   if (tiles > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

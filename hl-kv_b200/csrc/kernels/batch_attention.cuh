@@ -45,6 +45,9 @@ struct Params {
   uint32_t slot_rows;    // rows per head of a partial result
   uint64_t* prefix;      // [nseq + 1] cost of the sequences before
   float* partial;        // [ctas + nseq * head_groups][8][slot_rows][kD + 4]: outputs, max, sum
+  // tile kernel and join
+  float* tile_partial;  // [ctas][256][kD + 4]
+  uint32_t* tile_redo;  // [ctas]
 };
 
 // The new tokens of sequence i: rows [first, first + q) of Q, kept inside the arrays whatever the
@@ -280,6 +283,7 @@ struct SharedMemoryOnce {
 cudaError_t launch_stream(uint32_t head_dim, const Params& p, cudaStream_t s);
 size_t stream_workspace(uint32_t nseq, uint32_t H, uint32_t head_dim, uint32_t max_rows, uint32_t ctas);
 void stream_layout(Params* p, void* ws);
+size_t tile_workspace(uint32_t nseq, uint32_t head_dim, uint32_t max_rows, uint32_t ctas);
 uint64_t tile_ctas(const Params& p);  // the tile kernel's grid: 0 when no sequence can have its rows
 cudaError_t launch_tiles(uint32_t head_dim, const Params& p, cudaStream_t s);
 

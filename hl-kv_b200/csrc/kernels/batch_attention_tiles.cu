@@ -55,6 +55,7 @@ struct RowTile {
 
 struct Shared {
   RowTile mine;
+  uint32_t splits, part;  // of the row tile's tokens
   uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];  // of the two stages
   uint64_t s_full[2], p_full[2], o_done[2];               // of the two accumulator tiles
   // Of the tokens of the last four tiles: a K half may be written again while the softmax of the tile two before
@@ -213,12 +214,14 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t base, uint32_t r, uint32_t
   return base + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// The tokens that a CTA's rows see, as positions: [0, a) and [b0, b1), walked in tiles of 128.
+// The tokens that a row tile's rows see, as positions: [0, a) and [b0, b1), walked in tiles of 128 from tile `from` on.
 struct Walk {
-  uint32_t a, b0, b1;
+  uint32_t a, b0, b1, from;
   __device__ __forceinline__ uint32_t first_tiles() const { return (a + kTile - 1) / kTile; }
   __device__ __forceinline__ uint32_t tiles() const { return first_tiles() + (b1 - b0 + kTile - 1) / kTile; }
+  __device__ __forceinline__ bool begins(uint32_t j) const { return j == 0 || j + from == first_tiles(); }  // a run of tiles
   __device__ __forceinline__ void tile(uint32_t j, uint32_t* pos, uint32_t* n) const {
+    j += from;
     const uint32_t fa = first_tiles();
     if (j < fa) {
       *pos = j * kTile;
@@ -230,29 +233,65 @@ struct Walk {
   }
 };
 
-// The r-th (sequence, row tile) of the batch when they are ordered by the tiles of tokens that they walk, most first:
-// CTAs start in that order, and the last ones to end are short.  Found by a warp: the level of r by bisection over
-// counts (a sequence's tiles of a level and above are its last ones), then its place among the level's tiles.
+__device__ __forceinline__ Walk walk_of(const Params& p, uint32_t n_blocks, int32_t p_lo, int32_t p_hi) {
+  if (p_hi < 0 || n_blocks == 0) return Walk{0, 0, 0, 0};
+  const uint32_t end = static_cast<uint32_t>(p_hi) + 1;
+  const int64_t low = p.window == 0 ? 0 : int64_t{p_lo} - p.window + 1;
+  if (low <= int64_t{p.sinks}) return Walk{0, 0, end, 0};
+  return Walk{min(p.sinks, end), static_cast<uint32_t>(low), end, 0};
+}
+
+// Positions that the rows [row0, row0 + rows) of a sequence with `base` tokens before its new ones have.
+__device__ __forceinline__ int32_t position_of(const Params& p, int32_t base, uint32_t row) {
+  return base + static_cast<int32_t>(row / p.group);
+}
+
+// Few row tiles over long contexts: each one's tokens are split over as many CTAs as the GPU has left, kSplitTiles tiles
+// each at least, and joined by join_kernel.  A batch whose row tiles fill half the GPU is not split.
+constexpr uint32_t kMaxSplits = 16, kSplitTiles = 4;
+__device__ __forceinline__ uint32_t splits_of(const Params& p, uint32_t row_tiles) {
+  const uint32_t units = row_tiles * p.H;
+  return units == 0 ? 1u : max(1u, min(kMaxSplits, p.ctas / units));
+}
+__device__ __forceinline__ uint32_t parts_of(uint32_t splits, uint32_t n_tiles) {
+  return max(1u, min(splits, n_tiles / kSplitTiles));
+}
+
 // Most sequences to look through: 30 sequences of up to 300 new tokens over up to 3000 took 419 us so and 447 us with
 // the last tiles of all first, 100 of them 1401 and 1417 us, 250 of them 3875 and 3742 us.
 constexpr uint32_t kOrdered = 128;
+
+// A tile sees at most `cap` tokens; its level is its last token's tile of 128, or the one of the cap.
+__device__ __forceinline__ uint32_t token_cap_of(const Params& p) {
+  const uint64_t cap = p.window == 0 ? 0x7FFFFFFFu : uint64_t{p.window} + p.sinks + kRowsCta / p.group + 1;
+  return static_cast<uint32_t>(min(cap, uint64_t{0x7FFFFFFFu}));
+}
+// Row tiles of sequence i at level x and above: from the first one whose last token lies behind (x - 1) 128.
+__device__ __forceinline__ uint32_t row_tiles_above(const Params& p, uint32_t i, uint32_t x, uint32_t cap) {
+  const Rows rows = rows_of(p, i);
+  const uint64_t n_rows = uint64_t{rows.q} * p.group;
+  if (n_rows <= kStreamRows) return 0u;
+  const uint32_t n = static_cast<uint32_t>((n_rows + kRowsCta - 1) / kRowsCta);
+  if (x == 0) return n;
+  const uint64_t from = uint64_t{x - 1} * kTile;
+  const int64_t tok = static_cast<int64_t>(from) - (int64_t{p.context[i]} - rows.q);  // that token as a new one
+  if (from >= cap || tok >= int64_t{rows.q}) return 0u;
+  return tok <= 0 ? n : n - static_cast<uint32_t>(uint64_t(tok) * p.group / kRowsCta);
+}
+// All row tiles of the batch, counted by a warp.
+__device__ __forceinline__ uint32_t count_row_tiles(const Params& p) {
+  uint32_t c = 0;
+  for (uint32_t i = threadIdx.x & 31; i < p.nseq; i += 32) c += row_tiles_above(p, i, 0, 0);
+  return __reduce_add_sync(0xFFFFFFFFu, c);
+}
+
+// The r-th (sequence, row tile) of the batch when they are ordered by the tiles of tokens that they walk, most first:
+// CTAs start in that order, and the last ones to end are short.  Found by a warp: the level of r by bisection over
+// counts (a sequence's tiles of a level and above are its last ones), then its place among the level's tiles.
 __device__ __forceinline__ RowTile row_tile_of_rank(const Params& p, uint32_t r) {
   const uint32_t lane = threadIdx.x & 31;
-  // A tile sees at most `cap` tokens; its level is its last token's tile of 128, or the one of the cap.
-  const uint64_t cap64 = p.window == 0 ? 0x7FFFFFFFu : uint64_t{p.window} + p.sinks + kRowsCta / p.group + 1;
-  const uint32_t cap = static_cast<uint32_t>(min(cap64, uint64_t{0x7FFFFFFFu}));
-  // Row tiles of sequence i at level x and above: from the first one whose last token lies behind (x - 1) 128.
-  auto above = [&](uint32_t i, uint32_t x) -> uint32_t {
-    const Rows rows = rows_of(p, i);
-    const uint64_t n_rows = uint64_t{rows.q} * p.group;
-    if (n_rows <= kStreamRows) return 0u;
-    const uint32_t n = static_cast<uint32_t>((n_rows + kRowsCta - 1) / kRowsCta);
-    if (x == 0) return n;
-    const uint64_t from = uint64_t{x - 1} * kTile;
-    const int64_t tok = static_cast<int64_t>(from) - (int64_t{p.context[i]} - rows.q);  // that token as a new one
-    if (from >= cap || tok >= int64_t{rows.q}) return 0u;
-    return tok <= 0 ? n : n - static_cast<uint32_t>(uint64_t(tok) * p.group / kRowsCta);
-  };
+  const uint32_t cap = token_cap_of(p);
+  auto above = [&](uint32_t i, uint32_t x) { return row_tiles_above(p, i, x, cap); };
   auto count = [&](uint32_t x) {
     uint32_t c = 0;
     for (uint32_t i = lane; i < p.nseq; i += 32) c += above(i, x);
@@ -261,7 +300,6 @@ __device__ __forceinline__ RowTile row_tile_of_rank(const Params& p, uint32_t r)
   uint32_t longest = 0;
   for (uint32_t i = lane; i < p.nseq; i += 32) longest = max(longest, min(p.context[i], cap));
   uint32_t lo = 0, hi = (__reduce_max_sync(0xFFFFFFFFu, longest) + kTile - 1) / kTile + 1;  // count(hi) == 0
-  if (r >= count(0)) return RowTile{0u, 0xFFFFFFFFu};
   while (hi - lo > 1) {
     const uint32_t x = (lo + hi) / 2;
     if (count(x) > r) lo = x;
@@ -300,15 +338,28 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 
   // ---- the CTA's rows: those that see most tokens first; the heads of the same rows side by side, since a token's
   // heads lie together
+  dev::allow_dependents_to_launch();  // join_kernel, which waits for this kernel's end
   const uint32_t h = blockIdx.x % p.H;
   RowTile mine;
+  uint32_t splits = 1, part = 0;
   if (p.nseq <= kOrdered) {
     if (warp == 0) {
-      mine = row_tile_of_rank(p, blockIdx.x / p.H);
-      if (lane == 0) sh.mine = mine;
+      const uint32_t n = count_row_tiles(p);
+      splits = splits_of(p, n);
+      uint32_t rank = blockIdx.x / p.H;
+      if (n > 0) part = rank / n;
+      mine = RowTile{0u, 0xFFFFFFFFu};
+      if (n > 0 && part < splits) mine = row_tile_of_rank(p, rank - part * n);
+      if (lane == 0) {
+        sh.mine = mine;
+        sh.splits = splits;
+        sh.part = part;
+      }
     }
     __syncthreads();
     mine = sh.mine;
+    splits = sh.splits;
+    part = sh.part;
   } else {  // last tiles of all sequences first
     const uint32_t seq = blockIdx.x / p.H % p.nseq, order = blockIdx.x / p.H / p.nseq;
     const uint64_t n_rows = uint64_t{rows_of(p, seq).q} * p.group, n = (n_rows + kRowsCta - 1) / kRowsCta;
@@ -323,19 +374,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   const uint32_t ctx = p.context[seq];
   const int32_t pos_base = static_cast<int32_t>(ctx) - static_cast<int32_t>(rows.q);  // of the first new token
   const int32_t p_lo = pos_base + static_cast<int32_t>(row0 / p.group), p_hi = pos_base + static_cast<int32_t>((row0 + rows_here - 1) / p.group);
-  Walk walk{0, 0, 0};
   uint32_t first_block;
   const uint32_t n_blocks = count_of(p, seq, &first_block);
-  if (p_hi >= 0 && n_blocks > 0) {
-    const uint32_t end = static_cast<uint32_t>(p_hi) + 1;
-    const int64_t low = p.window == 0 ? 0 : int64_t{p_lo} - p.window + 1;
-    if (low <= int64_t{p.sinks}) {
-      walk = Walk{0, 0, end};
-    } else {
-      walk = Walk{min(p.sinks, end), static_cast<uint32_t>(low), end};
-    }
+  Walk walk = walk_of(p, n_blocks, p_lo, p_hi);
+  uint32_t n_tiles = walk.tiles();
+  const uint32_t parts = parts_of(splits, n_tiles);
+  if (part >= parts) return;
+  if (parts > 1) {  // this CTA's share of the tiles
+    walk.from = static_cast<uint32_t>(uint64_t{n_tiles} * part / parts);
+    n_tiles = static_cast<uint32_t>(uint64_t{n_tiles} * (part + 1) / parts) - walk.from;
   }
-  const uint32_t n_tiles = walk.tiles();
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -592,6 +640,19 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             wait_ld();
           }
           __syncwarp();
+          if (parts > 1) {
+            float* dst = p.tile_partial + (uint64_t{blockIdx.x} * kRowsCta + acc * 128 + r) * (kD + 4);
+            if (c == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(m, l);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {  // in the order of the accumulators: join_kernel puts it right
+              float4 y;
+              float* x = &y.x;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = none ? 0.0f : fmaf(__uint_as_float(o[4 * k + i]), unit, bias);
+              reinterpret_cast<float4*>(dst + c * 32)[k] = y;
+            }
+            continue;
+          }
           uint4* dst = reinterpret_cast<uint4*>(p.out + (rows.first + tok) * p.out_stride + uint64_t{head} * kD + c * 32);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -641,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     auto look = [&](uint32_t j) {
       uint32_t t;
       const bool in = position(j, &t);
-      if (j == 0 || j == walk.first_tiles()) {  // a run begins: the last block that starts at or before the first token
+      if (walk.begins(j)) {  // a run begins: the last block that starts at or before the first token
         const uint32_t first = __shfl_sync(0xFFFFFFFFu, t, 0);
         uint32_t a = 0, b = n_blocks;
         while (b - a > 1) {
@@ -881,10 +942,79 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   if (warp == kSoftmaxWarps + kStageWarps) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
-  if (sh.redo) {
+  if (parts > 1) {
+    if (threadIdx.x == 0) p.tile_redo[blockIdx.x] = sh.redo;
+  } else if (sh.redo) {
     for (uint32_t r = warp; r < rows_here; r += kThreads / 32) {
       const uint32_t row = row0 + r, tok = row / p.group;
       attend_row<kD>(p, seq, rows.first + tok, int64_t{pos_base} + tok, h * p.group + row % p.group);
+    }
+  }
+}
+
+// Joins the parts of split row tiles: a CTA for 32 rows of a (row tile, head), a warp for a row at a time.  Rows of which
+// some part asks for it are done over, token by token.
+constexpr uint32_t kJoinWarps = 8, kJoinRows = 32;
+template <int kD>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ Params p) {
+  constexpr int kPer = kD / 32;
+  __shared__ RowTile s_mine;
+  __shared__ uint32_t s_n, s_splits;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr uint32_t kGroups = kRowsCta / kJoinRows;
+  const uint32_t unit = blockIdx.x / kGroups, rank = unit / p.H, h = unit % p.H;
+  if (warp == 0) {  // of the plan, which is older than the kernel before
+    const uint32_t n = count_row_tiles(p), splits = splits_of(p, n);
+    RowTile mine{0u, 0xFFFFFFFFu};
+    if (splits > 1 && rank < n) mine = row_tile_of_rank(p, rank);
+    if (lane == 0) {
+      s_mine = mine;
+      s_n = n;
+      s_splits = splits;
+    }
+  }
+  __syncthreads();
+  dev::wait_for_prerequisites();
+  const RowTile mine = s_mine;
+  if (mine.tile == 0xFFFFFFFFu) return;
+  const Rows rows = rows_of(p, mine.seq);
+  const uint32_t n_rows = rows.q * p.group, row0 = mine.tile * kRowsCta, rows_here = min(kRowsCta, n_rows - row0);
+  const int32_t base = static_cast<int32_t>(p.context[mine.seq]) - static_cast<int32_t>(rows.q);
+  uint32_t first_block;
+  const uint32_t n_blocks = count_of(p, mine.seq, &first_block);
+  const uint32_t parts =
+      parts_of(s_splits, walk_of(p, n_blocks, position_of(p, base, row0), position_of(p, base, row0 + rows_here - 1)).tiles());
+  if (parts == 1) return;  // written already
+  // CTA (part, rank, head) of the tile kernel
+  auto slot = [&](uint32_t part) { return (uint64_t{part} * s_n + rank) * p.H + h; };
+  uint32_t redo = 0;
+  for (uint32_t k = 0; k < parts; ++k) redo |= p.tile_redo[slot(k)];
+  for (uint32_t r = blockIdx.x % kGroups * kJoinRows + warp; r < (blockIdx.x % kGroups + 1) * kJoinRows && r < rows_here; r += kJoinWarps) {
+    const uint32_t row = row0 + r, tok = row / p.group, head = h * p.group + row % p.group;
+    if (redo != 0) {
+      attend_row<kD>(p, mine.seq, rows.first + tok, int64_t{base} + tok, head);
+      continue;
+    }
+    float M = -INFINITY, L = 0.0f, o[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = 0.0f;
+#pragma unroll 4
+    for (uint32_t k = 0; k < parts; ++k) {
+      const float* src = p.tile_partial + (slot(k) * kRowsCta + r) * (kD + 4);
+      const float2 ml = *reinterpret_cast<const float2*>(src + kD);
+      const float m = fmaxf(M, ml.x);
+      const float fo = m == -INFINITY ? 1.0f : exp2f(M - m), ft = m == -INFINITY ? 1.0f : exp2f(ml.x - m);
+      M = m;
+      L = fmaf(L, fo, ml.y * ft);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], fo, src[i * 32 + lane] * ft);
+    }
+    if (L == 0.0f && M == -INFINITY) L = 1.0f;  // sees nothing: zeros
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      // place x of a chunk of 8 is element (x / 2) + 4 (x % 2)
+      const uint32_t at = i * 32 + lane, x = at & 7, e = (at & ~7u) + (x >> 1) + 4 * (x & 1);
+      p.out[(rows.first + tok) * p.out_stride + uint64_t{head} * kD + e] = __half_as_ushort(__float2half_rn(o[i] / L));
     }
   }
 }
@@ -895,7 +1025,19 @@ cudaError_t launch(const Params& p, cudaStream_t s) {
   const cudaError_t e = once.allow(reinterpret_cast<const void*>(tile_kernel<kD>), Config<kD>::kSmem);
   if (e != cudaSuccess) return e;
   tile_kernel<kD><<<static_cast<unsigned>(tile_ctas(p)), kThreads, Config<kD>::kSmem, s>>>(p);
-  return cudaGetLastError();
+  const cudaError_t e2 = cudaGetLastError();
+  if (e2 != cudaSuccess || p.nseq > kOrdered) return e2;
+  // At most half as many (row tile, head) as the GPU has SMs are split.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.ctas / 2 * (kRowsCta / kJoinRows));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<kD>, p);
 }
 
 }  // namespace
@@ -907,8 +1049,13 @@ uint64_t tile_ctas(const Params& p) {
     // sequence of more than kStreamRows rows.
     const uint64_t rows = uint64_t{p.token_cap} * p.group, most = rows / kRowsCta + std::min<uint64_t>(p.nseq, rows / (kStreamRows + 1));
     tiles = std::min(tiles, most);
+    return tiles == 0 ? 0u : std::max<uint64_t>(tiles * p.H, p.ctas);  // (parts of few)
   }
   return tiles * p.H;
+}
+size_t tile_workspace(uint32_t nseq, uint32_t head_dim, uint32_t max_rows, uint32_t ctas) {
+  if (max_rows <= kStreamRows || nseq > kOrdered) return 0;
+  return size_t{ctas} * kRowsCta * (head_dim + 4) * sizeof(float) + size_t{ctas} * sizeof(uint32_t);
 }
 
 cudaError_t launch_tiles(uint32_t head_dim, const Params& p, cudaStream_t s) {

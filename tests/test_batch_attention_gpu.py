@@ -153,6 +153,34 @@ def test_uneven_batch(hlkv_lib, cuda_device):
     b.check(8, seed=2)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5), (130, 0)])
+@pytest.mark.parametrize("q", [[60], [5, 70, 1], [260, 33]])
+def test_few_row_tiles_over_long_contexts(hlkv_lib, cuda_device, D, window, sinks, q):
+    """A row tile's tokens split over several CTAs and joined; short contexts next to them are not."""
+    rng = np.random.default_rng(D + window)
+    b = Batch(hlkv_lib, 16, 2, D, _vt(rng, 16, [150, 90, 40][:len(q)], partial=0.05), q, window=window, sinks=sinks, seed=D, pad=4)
+    b.check(8, seed=1)
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, 65504.0])
+def test_hidden_tokens_do_not_matter_when_split(hlkv_lib, cuda_device, value):
+    import torch
+    T, H, D = 16, 1, 128
+    q, ctx = [40], [2400]
+    b = Batch(hlkv_lib, T, H, D, [[16] * 150], q, probs=(1, 0, 0, 0), seed=9)
+    _poke(b.wl, None, {(0, ctx[0] - q[0] + r): value for r in (20, 39)})
+    x, d_q = b.queries(4, 1)
+    got = b.run(d_q, D ** -0.5)
+    torch.cuda.synchronize()
+    g = got.cpu().numpy().view(np.float16).astype(np.float64)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, tol, _ = b.want(x, D ** -0.5)
+    assert np.isfinite(want[:20]).all() and (np.abs(g - want)[:20] <= tol[:20]).all()
+    if not np.isfinite(value):
+        assert not np.isfinite(g[20:]).all(-1).any()
+
+
 @pytest.mark.parametrize("nseq", [128, 129])
 @pytest.mark.parametrize("window", [0, 40])
 def test_many_sequences_of_many_rows(hlkv_lib, cuda_device, nseq, window):

@@ -86,7 +86,7 @@ def test_attention_arguments(hlkv_lib):
     assert call(plan=_plan(hlkv_lib, token_cap=0)) == hlkv_lib.OK
     for kw in (dict(err=None), dict(q=None), dict(out=None), dict(q=ODD), dict(out=ODD), dict(qs=4088), dict(os=4092),
                dict(heads=12), dict(heads=0), dict(heads=8 * 33), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
-               dict(scale=float("nan")), dict(layout=hlkv_lib.Layout(16, 8, 256, 1)), dict(layout=hlkv_lib.Layout(1024, 8, 128, 1)),
+               dict(scale=float("nan")), dict(scale=2.0 ** 61), dict(layout=hlkv_lib.Layout(16, 8, 256, 1)), dict(layout=hlkv_lib.Layout(1024, 8, 128, 1)),
                dict(plan=_plan(hlkv_lib, blocks=None)), dict(plan=_plan(hlkv_lib, blocks=4104)),
                dict(plan=_plan(hlkv_lib, context=None)), dict(plan=_plan(hlkv_lib, token_first=None)),
                dict(ws=None), dict(ws=ODD), dict(plan=_plan(hlkv_lib, max_query=0)), dict(plan=_plan(hlkv_lib, block_cost=None)), dict(plan=_plan(hlkv_lib, cost=None)), dict(plan=_plan(hlkv_lib, token_cap=1 << 30)),
