@@ -17,13 +17,13 @@
 // lie the same way, and the outputs are put back in order at the end.
 //
 // Measured (8 KV heads of 128, 32 query heads; six chunks of up to 1645 new tokens over contexts of up to 8024, formats
-// mixed): 928 us, 402 TFLOP/s, 0.24 of the matrix rate; the caches of one format alone: FP16 816, E4M3 885, INT4 993 us.
+// mixed): 950 us, 393 TFLOP/s, 0.24 of the matrix rate; the caches of one format alone: FP16 816, E4M3 885, INT4 993 us.
 // The products alone would take 370 us, the conversion without the softmax 640, the softmax without the conversion
 // 950.  The softmax's two warps per scheduler wait on their own chains (an issue every 2.2 cycles), and the per-token
 // parameters are broadcast from shared memory: a float4 load returns 512 bytes to a warp, 2048 cycles of a tile for FP8
-// and 4096 for INT4.  Five prompts of heads of 64 with a window of 1024: 147 us; a CTA there walks ten tiles, of which
-// the last and the sinks' are short.
-// Tried and slower: halves of 64 tokens with scores of their own (1020 us), products issued by a softmax warp (1190),
+// and 4096 for INT4.  Five prompts of heads of 64 with a window of 1024: 154 us; a CTA there walks ten tiles, of which
+// the last and the sinks' are short.  250 new tokens over 8000, four row tiles a head: 124 us, and 340 without the split.
+// Tried and slower than 928 us (the same without the split over tokens, whose code costs 2 %): halves of 64 tokens with scores of their own (1020 us), products issued by a softmax warp (1190),
 // half the loads in flight (1070), FP8 and INT4 rows in 16-byte pieces a tile ahead (985).
 #include <algorithm>
 #include <cmath>
@@ -56,6 +56,7 @@ struct RowTile {
 struct Shared {
   RowTile mine;
   uint32_t splits, part;  // of the row tile's tokens
+  bool split;             // this row tile's
   uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];  // of the two stages
   uint64_t s_full[2], p_full[2], o_done[2];               // of the two accumulator tiles
   // Of the tokens of the last four tiles: a K half may be written again while the softmax of the tile two before
@@ -247,7 +248,9 @@ __device__ __forceinline__ int32_t position_of(const Params& p, int32_t base, ui
 }
 
 // Few row tiles over long contexts: each one's tokens are split over as many CTAs as the GPU has left, kSplitTiles tiles
-// each at least, and joined by join_kernel.  A batch whose row tiles fill half the GPU is not split.
+// each at least, and joined by join_kernel.  A batch whose row tiles fill half the GPU is not split.  (One sequence of 250
+// new tokens over 8000: 124 us, 340 without; two of 5 to 8 new tokens: 70 us and 283.  The join's launch costs an
+// unsplit batch 2 to 4 us.)
 constexpr uint32_t kMaxSplits = 16, kSplitTiles = 4;
 __device__ __forceinline__ uint32_t splits_of(const Params& p, uint32_t row_tiles) {
   const uint32_t units = row_tiles * p.H;
@@ -396,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       mbar_init(&sh.o_done[i], 1);
     }
     sh.redo = 0;
+    sh.split = parts > 1;
     mbar_fence_init();
   }
   if (warp == kSoftmaxWarps + kStageWarps) {
@@ -640,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             wait_ld();
           }
           __syncwarp();
-          if (parts > 1) {
+          if (sh.split) {
             float* dst = p.tile_partial + (uint64_t{blockIdx.x} * kRowsCta + acc * 128 + r) * (kD + 4);
             if (c == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(m, l);
 #pragma unroll
@@ -942,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   if (warp == kSoftmaxWarps + kStageWarps) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
-  if (parts > 1) {
+  if (sh.split) {
     if (threadIdx.x == 0) p.tile_redo[blockIdx.x] = sh.redo;
   } else if (sh.redo) {
     for (uint32_t r = warp; r < rows_here; r += kThreads / 32) {
@@ -952,9 +956,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   }
 }
 
-// Joins the parts of split row tiles: a CTA for 32 rows of a (row tile, head), a warp for a row at a time.  Rows of which
+// Joins the parts of split row tiles: a CTA for 16 rows of a (row tile, head), a warp for a row at a time.  Rows of which
 // some part asks for it are done over, token by token.
-constexpr uint32_t kJoinWarps = 8, kJoinRows = 32;
+constexpr uint32_t kJoinWarps = 8, kJoinRows = 16;
 template <int kD>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ Params p) {
   constexpr int kPer = kD / 32;
