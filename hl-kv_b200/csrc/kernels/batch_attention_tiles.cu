@@ -1031,6 +1031,10 @@ cudaError_t launch(const Params& p, cudaStream_t s) {
   tile_kernel<kD><<<static_cast<unsigned>(tile_ctas(p)), kThreads, Config<kD>::kSmem, s>>>(p);
   const cudaError_t e2 = cudaGetLastError();
   if (e2 != cudaSuccess || p.nseq > kOrdered) return e2;
+  // Rows that see so few tokens (at most a tile more for each of the walk's two runs) are not split: no join.
+  uint64_t most = uint64_t{p.block_cap} * p.T;
+  if (p.window != 0) most = std::min(most, uint64_t{p.window} + p.sinks + kRowsCta / p.group + 1);
+  if (most / kTile + 2 < 2 * kSplitTiles) return e2;
   // At most half as many (row tile, head) as the GPU has SMs are split.
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.ctas / 2 * (kRowsCta / kJoinRows));
