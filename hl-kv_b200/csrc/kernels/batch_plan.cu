@@ -393,7 +393,8 @@ extern "C" int hlkv_batch_plan(const HlkvBatchPlan* plan, const HlkvLayout* layo
       (plan->block_cap > 0 && (plan->d_blocks == nullptr || plan->d_block_cost == nullptr)) ||
       (plan->token_cap > 0 && (plan->d_targets == nullptr || plan->d_positions == nullptr)) ||
       (table_size > 0 && d_table == nullptr) || (arena_size > 0 && d_arena == nullptr) ||
-      (reinterpret_cast<uintptr_t>(plan->d_blocks) & 15u) != 0 || (reinterpret_cast<uintptr_t>(plan->d_targets) & 7u) != 0) {
+      (reinterpret_cast<uintptr_t>(plan->d_blocks) & 15u) != 0 || (reinterpret_cast<uintptr_t>(plan->d_targets) & 7u) != 0 ||
+      (reinterpret_cast<uintptr_t>(d_table) & 15u) != 0 || (reinterpret_cast<uintptr_t>(d_segs) & 7u) != 0) {
     return HLKV_INVALID_ARGUMENT;
   }
   // Grids stay below 2^31 CTAs with any cluster size.

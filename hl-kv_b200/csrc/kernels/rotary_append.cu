@@ -421,7 +421,7 @@ extern "C" int hlkv_rotary_append(const HlkvPools* pools, const HlkvLayout* layo
   if (n == 0) return HLKV_OK;
   const uint64_t D = layout->head_dim, H = layout->kv_heads;
   if (d_targets == nullptr || d_positions == nullptr || d_k == nullptr || d_v == nullptr ||
-      (table_size > 0 && d_table == nullptr) || (reinterpret_cast<uintptr_t>(d_targets) & 7u) != 0 || !aligned16(d_k) ||
+      (table_size > 0 && d_table == nullptr) || !aligned16(d_table) || (reinterpret_cast<uintptr_t>(d_targets) & 7u) != 0 || !aligned16(d_k) ||
       !aligned16(d_v) || k_stride % 8 != 0 || v_stride % 8 != 0 || k_stride < H * D || v_stride < H * D) {
     return HLKV_INVALID_ARGUMENT;
   }

@@ -391,7 +391,8 @@ typedef struct {
  *  - A sequence whose blocks or new tokens do not fit the arrays, or that has more than
  *    max_query new tokens, is planned as empty (context 0, no blocks, its rows padding) with
  *    HLKV_ERR_PLAN_RANGE.  New tokens beyond a sequence's tokens are padding, with the same bit.
- * block_cap * block_tokens is below 2^31 (positions are int32), and block_cap at most 2^27.
+ * block_cap * block_tokens is below 2^31 (positions are int32), and block_cap at most 2^27.  d_table is
+ * 16-byte aligned, d_segs 8-byte.
  * The device form of hlkv_table_build_exec_table (hetero_block_table.cpp:406-433) and of
  * hlkv_table_append_tokens' targets; the reference builds neither on the device.
  */
@@ -431,7 +432,8 @@ typedef struct {
  *    [kv_heads]), token strides in elements (multiples of 8); 16-byte aligned.  Slices of a fused
  *    projection need no copy.  d_q_out may be d_q with the same stride, and overlaps nothing else.
  *    q_heads 0: K and V only (d_q and d_q_out unused).
- *  - d_positions[k * position_token_stride + a * position_axis_stride], int32.
+ *  - d_positions[k * position_token_stride + a * position_axis_stride], int32.  d_table is 16-byte aligned,
+ *    d_targets 8-byte.
  *  - A target {0xFFFFFFFF, 0xFFFFFFFF} is padding: the row is skipped, its d_q_out left as it was.
  *  - A target failing hlkv_append_encode's checks stores nothing and sets its bit (Q is still
  *    written); a quantized row with a non-finite value is skipped with HLKV_ERR_NONFINITE.
