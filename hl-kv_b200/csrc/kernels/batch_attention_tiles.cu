@@ -568,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             l *= a;
             bias *= a;
             const uint32_t a2 = dev::pack_f16x2(a, a);
+            wait_st();  // this tile's weights so far: a load is ordered behind the stores before it by this alone
 #pragma unroll 1
             for (uint32_t k = 0; k < c; ++k) {
               uint32_t w[16];
