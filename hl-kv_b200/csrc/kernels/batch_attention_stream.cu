@@ -823,7 +823,7 @@ struct Producer {
       // The parameters of all heads of the tile's tokens, rounded out to 16 bytes (the slot's end is).
       uint64_t pa = 0;
       uint32_t pn = 0;
-      if (f != dev::kFp16 && mode == 0) {
+      if (live && f != dev::kFp16 && mode == 0) {  // (a lane without a tile has no format)
         pa = p.code_bytes[f] + uint64_t{row0} * p.H * pb;
         pn = static_cast<uint32_t>(((pa + n * p.H * pb + 15) & ~uint64_t{15}) - (pa & ~uint64_t{15}));
       }
