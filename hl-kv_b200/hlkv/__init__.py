@@ -278,13 +278,15 @@ def layout_slot_bytes(fmt: int, layout: Layout) -> int:
 
 
 _torch = None
+_HALF = _WORD = ()  # types whose bits a kernel takes as binary16, and as 32-bit integers
 
 
 def _cuda():
     """torch, imported at the first call that launches."""
-    global _torch
+    global _torch, _HALF, _WORD
     if _torch is None:
         import torch
+        _HALF, _WORD = (torch.float16, torch.int16, torch.uint16), (torch.int32, torch.uint32)
         _torch = torch
     return _torch
 
@@ -749,11 +751,11 @@ def batch_plan(plan: BatchPlan, layout: Layout, table_ptr: int, table_size: int,
     if _elsewhere(dev):
         return _on_device(dev, batch_plan, plan, layout, table_ptr, table_size, arena_ptr, arena_size, segs, query_lens, err,
                           stream)
-    if not (segs.shape == (plan.nseq, 2) and segs.is_contiguous() and segs.element_size() == 4
-            and segs.get_device() == dev and err.get_device() == dev):
-        raise HlkvError("batch_plan: segs is a contiguous int32 [nseq, 2], on the plan's device as err is")
+    if not (segs.shape == (plan.nseq, 2) and segs.is_contiguous() and segs.dtype in _WORD
+            and segs.get_device() == dev and err.get_device() == dev and err.dtype in _WORD):
+        raise HlkvError("batch_plan: segs is a contiguous int32 [nseq, 2], on the plan's device as err (int32) is")
     if query_lens is not None and not (query_lens.shape == (plan.nseq,) and query_lens.is_contiguous()
-                                       and query_lens.element_size() == 4 and query_lens.get_device() == dev):
+                                       and query_lens.dtype in _WORD and query_lens.get_device() == dev):
         raise HlkvError("batch_plan: query_lens is a contiguous int32 [nseq] on the plan's device")
     st = lib().hlkv_batch_plan(plan.c, layout, table_ptr or None, table_size, arena_ptr or None, arena_size,
                                segs.data_ptr(), _ptr(query_lens), err.data_ptr(), _stream_handle(stream))
@@ -777,13 +779,13 @@ def make_rotary(inv_freq, axes: int | None = None, pair_axis=None, interleaved: 
 
 
 def _token_stride(t, what: str, n: int, heads: int, layout: Layout, dev: int) -> int:
-    """The token stride of a 16-bit [n, heads, head_dim] with contiguous heads on device dev; raises for
-    another tensor.  At most one token may have any stride: the row's length then."""
+    """The token stride of a binary16 [n, heads, head_dim] (or its bits as 16-bit integers) with contiguous heads on
+    device dev; raises for another tensor.  At most one token may have any stride: the row's length then."""
     dim = layout.head_dim
     tok, head, elem = t.stride() if t.dim() == 3 else (0, 0, 0)
-    if not (t.shape == (n, heads, dim) and elem == 1 and (head == dim or heads <= 1) and t.element_size() == 2
+    if not (t.shape == (n, heads, dim) and elem == 1 and (head == dim or heads <= 1) and t.dtype in _HALF
             and t.get_device() == dev):
-        raise HlkvError(f"{what} is a 16-bit [{n}, {heads}, {dim}] with contiguous heads, on the call's device")
+        raise HlkvError(f"{what} is a float16 [{n}, {heads}, {dim}] with contiguous heads, on the call's device")
     return tok if n > 1 else heads * dim
 
 
@@ -791,18 +793,18 @@ def rotary_append(pools: Pools, layout: Layout, table_ptr: int, table_size: int,
                   q, k, v, q_out, err, stream=None) -> int:
     """Rotates q and k by their positions, writes q to q_out (which may be q) and stores k and v in
     the targets' blocks.  targets: device int32 [n, 2]; positions: device int32 [n] or [n, axes], any
-    strides; q, q_out: device 16-bit [n, q_heads, head_dim] (or None); k, v: [n, kv_heads, head_dim];
-    token strides are free (slices of a fused projection).  Raises on a non-OK status."""
+    strides; q, q_out: device float16 [n, q_heads, head_dim] (or None); k, v: [n, kv_heads, head_dim];
+    token strides are free (slices of a fused projection); int16 and uint16 tensors are taken as binary16 bits.  Raises on a non-OK status."""
     dev = k.get_device()
     if _elsewhere(dev):
         return _on_device(dev, rotary_append, pools, layout, table_ptr, table_size, targets, rotary, positions, q, k, v, q_out,
                           err, stream)
     n = targets.shape[0]
-    if not (targets.shape == (n, 2) and targets.is_contiguous() and targets.element_size() == 4
-            and targets.get_device() == dev and err.get_device() == dev):
-        raise HlkvError("rotary_append: targets is a contiguous int32 [n, 2], on k's device as err is")
+    if not (targets.shape == (n, 2) and targets.is_contiguous() and targets.dtype in _WORD
+            and targets.get_device() == dev and err.get_device() == dev and err.dtype in _WORD):
+        raise HlkvError("rotary_append: targets is a contiguous int32 [n, 2], on k's device as err (int32) is")
     steps, axes = positions.stride(), rotary.axes
-    if not (positions.shape[0] == n and positions.element_size() == 4 and positions.get_device() == dev
+    if not (positions.shape[0] == n and positions.dtype in _WORD and positions.get_device() == dev
             and (len(steps) == 2 and positions.shape[1] >= axes or len(steps) == 1 and axes == 1)):
         raise HlkvError("rotary_append: positions is an int32 [n] or [n, axes] on k's device")
     heads = layout.kv_heads
@@ -831,7 +833,7 @@ def batch_attention_workspace_bytes(plan: BatchPlan, layout: Layout, q_heads: in
 
 def batch_attention(pools: Pools, layout: Layout, plan: BatchPlan, q, softmax_scale: float, out, err, workspace=None,
                     stream=None) -> int:
-    """Attention of the plan's new tokens over their sequences' blocks.  q, out: device 16-bit
+    """Attention of the plan's new tokens over their sequences' blocks.  q, out: device float16 (or its bits)
     [token_cap, q_heads, head_dim] with free token strides; workspace: a device tensor of
     batch_attention_workspace_bytes(...) bytes.  Raises on a non-OK status."""
     dev = plan.index
@@ -845,8 +847,8 @@ def batch_attention(pools: Pools, layout: Layout, plan: BatchPlan, q, softmax_sc
         ws_bytes = workspace.numel() * workspace.element_size()
         if not workspace.is_contiguous():
             raise HlkvError("batch_attention: a contiguous workspace")
-    if err.get_device() != dev or (ws_bytes and workspace.get_device() != dev):
-        raise HlkvError("batch_attention: tensors on the plan's device")
+    if err.get_device() != dev or err.dtype not in _WORD or (ws_bytes and workspace.get_device() != dev):
+        raise HlkvError("batch_attention: tensors on the plan's device, err an int32")
     st = lib().hlkv_batch_attention(pools, layout, plan.c, q.data_ptr(), heads, qs, softmax_scale,
                                     workspace.data_ptr() if ws_bytes else None, ws_bytes, out.data_ptr(), os_, err.data_ptr(),
                                     _stream_handle(stream))
