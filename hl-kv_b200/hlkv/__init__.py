@@ -735,6 +735,7 @@ class BatchPlan:
         buf = torch.zeros(max(total, 4), dtype=torch.int32, device=device)
         v = [buf[o:o + n] for o, n in parts]
         self.blocks, self.targets, self.positions = v[0].view(-1, 4), v[1].view(-1, 2), v[2]
+        self.targets.fill_(-1)  # padding: a plan that was not filled yet, or of no sequence, has no new token
         self.block_first, self.block_count, self.token_first, self.context, self.block_cost, self.cost = v[3:]
         at = [buf.data_ptr() + 4 * o for o, _ in parts]
         self.c = PlanArrays(nseq, max_query, window, sinks, block_cap, token_cap, at[3], at[4], at[5], at[6], at[0],

@@ -391,6 +391,7 @@ typedef struct {
  *  - A sequence whose blocks or new tokens do not fit the arrays, or that has more than
  *    max_query new tokens, is planned as empty (context 0, no blocks, its rows padding) with
  *    HLKV_ERR_PLAN_RANGE.  New tokens beyond a sequence's tokens are padding, with the same bit.
+ *  - nseq 0 fills nothing, the padding rows included: there is no new token, so no row to append or attend.
  * block_cap * block_tokens is below 2^31 (positions are int32), and block_cap at most 2^27.  d_table is
  * 16-byte aligned, d_segs 8-byte.
  * The device form of hlkv_table_build_exec_table (hetero_block_table.cpp:406-433) and of

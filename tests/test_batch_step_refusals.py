@@ -94,3 +94,11 @@ def test_tensors_of_another_type(hlkv_lib, device0):
     for call, other in wrong:
         with pytest.raises(hlkv_lib.HlkvError):
             call(**other)
+
+
+def test_a_plan_begins_as_padding(hlkv_lib):
+    """A plan that was not filled, or of no sequence (which batch_plan leaves as it is), appends nothing: a target of
+    zeros would be token 0 of block 0."""
+    for nseq in (0, 2):
+        plan = hlkv_lib.BatchPlan(nseq, 4, 5, device="cpu")
+        assert (plan.targets == -1).all() and (plan.positions == 0).all() and (plan.token_first == 0).all()
