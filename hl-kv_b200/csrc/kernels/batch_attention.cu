@@ -92,6 +92,7 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   p.block_cost = plan->d_block_cost;
   p.cost = plan->d_cost;
   p.token_cap = plan->token_cap;
+  p.max_query = plan->max_query;
   const uint64_t max_rows = uint64_t{plan->max_query} * p.group;
   p.max_rows = static_cast<uint32_t>(max_rows < 0xFFFFFFFFu ? max_rows : 0xFFFFFFFFu);
   p.qscale = softmax_scale * kLog2e;

@@ -37,6 +37,7 @@ struct Params {
   uint64_t q_stride, out_stride;
   uint32_t* err;
   uint32_t nseq, T, H, q_heads, group, window, sinks, block_cap, token_cap;
+  uint32_t max_query;
   uint32_t max_rows;  // most query rows per (sequence, KV head): max_query * group
   float qscale;       // softmax_scale * log2(e)
   // stream kernel and merge
@@ -51,13 +52,14 @@ struct Params {
 };
 
 // The new tokens of sequence i: rows [first, first + q) of Q, kept inside the arrays whatever the
-// plan holds.
+// plan holds.  A sequence with more than max_query of them, which the plan rejected, has none here: grids and
+// workspaces are made for max_query.
 struct Rows {
   uint32_t first, q;
 };
 __device__ __forceinline__ Rows rows_of(const Params& p, uint32_t i) {
   const uint32_t a = min(p.token_first[i], p.token_cap), b = min(p.token_first[i + 1], p.token_cap);
-  return Rows{a, b > a ? b - a : 0u};
+  return Rows{a, b > a && b - a <= p.max_query ? b - a : 0u};
 }
 __device__ __forceinline__ uint32_t count_of(const Params& p, uint32_t i, uint32_t* first) {
   *first = min(p.block_first[i], p.block_cap);
