@@ -560,14 +560,15 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           const float top = fmaxf(top0 - static_cast<float>(d0), top1 - static_cast<float>(d1));  // above the reference
           const bool grow = top > (m == -INFINITY ? -INFINITY : 8.0f);
           if (__any_sync(0xFFFFFFFFu, grow)) {
-            const float up = grow ? top : 0.0f;  // the maximum moves to ref + up
+            // The maximum moves to ref + up, by a whole number: the factor is a power of two, so that the weights made
+            // so far are not rounded again (but those that fall below binary16's normal range).
+            const float up = grow ? ceilf(top) : 0.0f;
             const float a = m == -INFINITY ? (grow ? 0.0f : 1.0f) : exp2f(-up);
             ok = rescale(a);
             if (!ok) break;
-            if (grow) m = ref + top;
+            if (grow) m = ref + up;
             l *= a;
             bias *= a;
-            const uint32_t a2 = dev::pack_f16x2(a, a);
             wait_st();  // this tile's weights so far: a load is ordered behind the stores before it by this alone
 #pragma unroll 1
             for (uint32_t k = 0; k < c; ++k) {
@@ -575,7 +576,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
               tmem_load16(t_s + k * 16, w);
               wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = hmul2(w[i], a2);
+              for (int i = 0; i < 16; ++i) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                w[i] = dev::pack_f16x2(v.x * a, v.y * a);
+              }
               tmem_store16(t_s + k * 16, w);
             }
             const Pair down = pair(-up, -up);
