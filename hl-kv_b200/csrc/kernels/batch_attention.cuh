@@ -142,6 +142,8 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// 2^-k for a whole k >= 0.
+__device__ __forceinline__ float halvings(float k) { return k > 126.0f ? 0.0f : __int_as_float((127 - static_cast<int>(k)) << 23); }
 
 // ---- barriers in shared memory and bulk copies ------------------------------------------------
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }

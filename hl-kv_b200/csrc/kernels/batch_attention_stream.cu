@@ -14,9 +14,9 @@
 // A code's binary16 value is exact (E4M3, E5M2, an INT4 code's integer), so the parameters stay out of
 // the matrices: the K row's scale multiplies the score in binary32 and its bias enters as
 // bias * sum(q); the V row's scale multiplies the weight, and its bias is summed apart in binary32.
-// A weight is rounded once, to binary16 (2^-12 of it), after being scaled by 2^-E: E follows the
-// exponents of the tiles' scales, so that weights stay in binary16's normal range whatever the values'
-// size, and the accumulators are in units of 2^E.
+// A weight is rounded once, to binary16 (2^-12 of it; the matrix unit takes no wider one at this rate), in a unit of its row
+// that follows the row's weights: those down to 2^-20 of the largest one stay in binary16's normal range, whatever sizes other
+// rows' and tokens' values have.
 // The order of contraction is free, so every lane takes contiguous bytes of a row and pairs them
 // where they lie: K elements (j, j + 4) of each 8, V tokens (2q, 2q + 1).
 //
@@ -213,11 +213,11 @@ __device__ __forceinline__ float2 lds_f2(uint32_t a) {
 // 2q + 1 of each column block, and head elements [g kD/8, (g + 1) kD/8).
 template <int kD, int kNB>
 struct State {
-  float acc[kNB][kD / 16][4];  // [.][mt]: element 2 mt of columns 2q, 2q + 1, then element 2 mt + 1; units of 2^E
-  float m[kNB][2], l[kNB][2], bias[kNB][2];  // l and bias: this lane's tokens only
-  int E;
+  float acc[kNB][kD / 16][4];  // [.][mt]: element 2 mt of columns 2q, 2q + 1, then element 2 mt + 1; units of 2^m / down
+  float m[kNB][2], l[kNB][2], bias[kNB][2];  // l and bias: this lane's tokens only, in units of 2^m
+  float down[kNB][2];                        // a power of two
 };
-constexpr int kNoExponent = -1000;
+constexpr int kMostDown = 60;  // down is in 2^+-60: sizes of values from 2^-74 to 2^58 are followed
 
 // What a warp keeps in shared memory for a piece: its Q^T fragments, and per column the scaled sum of q
 // and the position.
@@ -270,11 +270,11 @@ __device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, 
     for (int c = 0; c < 2; ++c) {
       s.m[nb][c] = -INFINITY;
       s.l[nb][c] = s.bias[nb][c] = 0.0f;
+      s.down[nb][c] = pow2(kMostDown);
     }
 #pragma unroll
     for (int mt = 0; mt < kD / 16; ++mt) s.acc[nb][mt][0] = s.acc[nb][mt][1] = s.acc[nb][mt][2] = s.acc[nb][mt][3] = 0.0f;
   }
-  s.E = kNoExponent;
   __syncwarp();
 }
 
@@ -365,8 +365,10 @@ __device__ __forceinline__ void scores(const Params& p, const uint32_t (&t)[kNT]
   }
 }
 
-// The reference maximum moves only when a score passes it by 8: weights reach 2^8 at most.  `top`: this
-// lane's largest scores.
+__device__ __forceinline__ int exponent_of(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 0xFFu) - 127; }
+
+// The reference maximum moves only when a score passes it by 8: exponentials reach 2^8 at most.  It moves by whole numbers,
+// so that what is scaled keeps its bits.  `top`: this lane's largest scores.
 template <int kD, int kNB>
 __device__ __forceinline__ void follow_maximum(State<kD, kNB>& s, float (&top)[kNB][2]) {
   bool grow = false;
@@ -381,42 +383,91 @@ __device__ __forceinline__ void follow_maximum(State<kD, kNB>& s, float (&top)[k
         v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
         v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
         v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
-        const float mn = fmaxf(s.m[nb][c], v);
-        const float a = mn == -INFINITY ? 1.0f : exp2f(s.m[nb][c] - mn);
-        s.m[nb][c] = mn;
+        const float mn = fmaxf(s.m[nb][c], ceilf(v));
+        if (mn == s.m[nb][c]) continue;
+        const float up = mn - s.m[nb][c], a = halvings(up);
         s.l[nb][c] *= a;
         s.bias[nb][c] *= a;
+        if (s.m[nb][c] != -INFINITY) {  // (before it there is nothing in the outputs)
+          // the outputs' unit stays, unless it is too far from the maximum's
+          const float d = static_cast<float>(exponent_of(s.down[nb][c])) + up, over = fmaxf(d - kMostDown, 0.0f), f = halvings(over);
+          s.down[nb][c] = pow2(static_cast<int>(d - over));
+          if (over > 0.0f) {
 #pragma unroll
-        for (int mt = 0; mt < kD / 16; ++mt) {
-          s.acc[nb][mt][c] *= a;
-          s.acc[nb][mt][2 + c] *= a;
+            for (int mt = 0; mt < kD / 16; ++mt) {
+              s.acc[nb][mt][c] *= f;
+              s.acc[nb][mt][2 + c] *= f;
+            }
+          }
         }
+        s.m[nb][c] = mn;
       }
     }
   }
 }
 
-// The accumulators' unit follows a tile's exponent: that of the largest value scale among its tokens, `top`
-// its bits (scales beyond 2^60 or below 2^-60 are taken as those).
+// A row's outputs have a unit of their own, which follows its weights (the exponential times the value row's scale in its unit,
+// about the row's largest value): where one passes 2^14 in that unit, the unit grows until it is below 2^7.  So
+// the largest weight so far is 2^6 at least, and binary16 holds those down to 2^-20 of it without a loss, whatever sizes
+// other rows' and tokens' values have.  w: the weights of tokens g and g + 8 of columns 2 quad, 2 quad + 1 of each column block.
+__device__ __forceinline__ bool too_large(float a, float b, float c, float d) {
+  return fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d))) > 0x1p14f;
+}
 template <int kD, int kNB>
-__device__ __forceinline__ void follow_exponent(State<kD, kNB>& s, uint32_t top) {
-  const int d = static_cast<int>(top >> 23) - 127 - s.E;
-  if (d > 6 || d < -6) {
-    const int e = min(max(static_cast<int>(top >> 23) - 127, -60), 60);
-    if (e > s.E || top != 0) {
-      if (s.E != kNoExponent) {
-        const float f = exp2f(static_cast<float>(s.E - e));
+__device__ __forceinline__ void follow_weights(State<kD, kNB>& s, float (&w)[kNB][4]) {
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
+  for (int nb = 0; nb < kNB; ++nb) {
 #pragma unroll
-          for (int mt = 0; mt < kD / 16; ++mt) {
+    for (int c = 0; c < 2; ++c) {
+      // infinities (scales that are not finite) move nothing
+      const float a = fabsf(w[nb][c]), b = fabsf(w[nb][2 + c]);
+      float v = fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f);
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
+      if (!(v > 0x1p14f)) continue;
+      const int d = exponent_of(s.down[nb][c]), up = min(exponent_of(v) - 6, d + kMostDown);
+      const float f = halvings(static_cast<float>(up));
+      s.down[nb][c] = pow2(d - up);
+      w[nb][c] *= f;
+      w[nb][2 + c] *= f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s.acc[nb][mt][k] *= f;
-          }
-        }
+      for (int mt = 0; mt < kD / 16; ++mt) {
+        s.acc[nb][mt][c] *= f;
+        s.acc[nb][mt][2 + c] *= f;
       }
-      s.E = e;
     }
+  }
+}
+
+// Encoders store an FP8 row of zeros with scale 1, a size that its values do not have.  Whether this lane's tokens g (bit 0)
+// and g + 8 (bit 1) of tile t are such rows.
+template <int kD, uint32_t kF>
+__device__ __forceinline__ uint32_t zero_rows(uint32_t t, const Place& at) {
+  constexpr uint32_t kRb = kRow<kD, kF>;
+  const uint32_t base = lds32(t + 16) + (at.head_i + (at.lane >> 2) * at.heads) * kRb + (at.lane & 3) * (kRb / 4);
+  uint32_t zeros = 0;
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h) {
+    uint32_t any = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kRb / 64; ++i) {
+      const uint4 w = lds128(base + h * 8 * at.heads * kRb + i * 16);
+      any |= w.x | w.y | w.z | w.w;
+    }
+    any |= __shfl_xor_sync(0xFFFFFFFFu, any, 1);
+    any |= __shfl_xor_sync(0xFFFFFFFFu, any, 2);
+    if ((any & 0x7F7F7F7Fu) == 0) zeros |= 1u << h;
+  }
+  return zeros;
+}
+
+template <int kNB>
+__device__ __forceinline__ void without_zeros(uint32_t zeros, float (&w)[kNB][4]) {
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+    if (zeros & 1u) w[nb][0] = w[nb][1] = 0.0f;
+    if (zeros & 2u) w[nb][2] = w[nb][3] = 0.0f;
   }
 }
 
@@ -502,16 +553,27 @@ __device__ __forceinline__ bool step(const Params& p, State<kD, kNB>& s, const u
       if (g + 8 >= n[k]) vp[1] = make_float2(0.0f, 0.0f);
     }
     const float u0 = vp[0].x * kValueUnit<kF>, u1 = vp[1].x * kValueUnit<kF>;
-    follow_exponent(s, kF == dev::kFp16 ? 0x3F800000u
-                                        : __reduce_max_sync(0xFFFFFFFFu, max(__float_as_uint(u0) & 0x7FFFFFFFu,
-                                                                             __float_as_uint(u1) & 0x7FFFFFFFu)));
-    const float down = pow2(-s.E), f0 = u0 * down, f1 = u1 * down;
+    float w[kNB][4];
+    bool grow = false;
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        w[nb][c] = pr[k][nb][c] * (u0 * s.down[nb][c]);
+        w[nb][2 + c] = pr[k][nb][2 + c] * (u1 * s.down[nb][c]);
+      }
+      grow = grow || too_large(w[nb][0], w[nb][1], w[nb][2], w[nb][3]);
+    }
+    if (__any_sync(0xFFFFFFFFu, grow)) {
+      if constexpr (kF == dev::kE4M3 || kF == dev::kE5M2) without_zeros<kNB>(zero_rows<kD, kF>(t[k], at), w);
+      follow_weights(s, w);
+    }
     const float beta0 = fmaf(8.0f, vp[0].x, vp[0].y), beta1 = fmaf(8.0f, vp[1].x, vp[1].y);
     uint32_t pb[kNB][2];
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
-      pb[nb][0] = transpose8(dev::pack_f16x2(pr[k][nb][0] * f0, pr[k][nb][1] * f0));
-      pb[nb][1] = transpose8(dev::pack_f16x2(pr[k][nb][2] * f1, pr[k][nb][3] * f1));
+      pb[nb][0] = transpose8(dev::pack_f16x2(w[nb][0], w[nb][1]));
+      pb[nb][1] = transpose8(dev::pack_f16x2(w[nb][2], w[nb][3]));
       if constexpr (kF == dev::kInt4) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) s.bias[nb][c] = fmaf(pr[k][nb][2 + c], beta1, fmaf(pr[k][nb][c], beta0, s.bias[nb][c]));
@@ -554,8 +616,8 @@ __device__ __forceinline__ int32_t position(const Place& at, uint32_t col) {
   return static_cast<int32_t>(lds32(at.rows + kNB * (kD / 32) * 512 + 32 * kNB + col * 4));
 }
 
-// O^T += V^T W^T of such a tile.  Where it holds values that are not finite, or scales far apart, it is taken
-// row by row, so that a row is not touched by what it does not see.
+// O^T += V^T W^T of such a tile.  Where it holds values that are not finite, it is taken row by row, so that a row is
+// not touched by what it does not see.
 template <int kD, int kNB, uint32_t kF>
 __device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, const View& v, const Place& at,
                                             const float (&pr)[kNB][4]) {
@@ -563,34 +625,34 @@ __device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, 
   constexpr uint32_t kRb = kRow<kD, kF>;
   float2 vp[2];
   row_params<kF>(v.t, 20, at, vp);
-  if (g >= v.n) vp[0] = make_float2(0.0f, 0.0f);
-  if (g + 8 >= v.n) vp[1] = make_float2(0.0f, 0.0f);
   const float u0 = vp[0].x * kValueUnit<kF>, u1 = vp[1].x * kValueUnit<kF>;
-  const uint32_t b0 = __float_as_uint(u0) & 0x7FFFFFFFu, b1 = __float_as_uint(u1) & 0x7FFFFFFFu;
-  const uint32_t fin0 = b0 < 0x7F800000u ? b0 : 0u, fin1 = b1 < 0x7F800000u ? b1 : 0u;
-  const uint32_t high = __reduce_max_sync(0xFFFFFFFFu, max(fin0, fin1));
-  const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, min(g < v.n ? b0 : 0xFFFFFFFFu, g + 8 < v.n ? b1 : 0xFFFFFFFFu));
-  const bool apart = __any_sync(0xFFFFFFFFu, b0 >= 0x7F800000u || b1 >= 0x7F800000u) || high > low + (8u << 23);
-  follow_exponent(s, high);
-  const float down = pow2(-s.E), f0 = u0 * down, f1 = u1 * down;
   const float beta0 = fmaf(8.0f, vp[0].x, vp[0].y), beta1 = fmaf(8.0f, vp[1].x, vp[1].y);  // INT4: what (code - 8) / 8 leaves
-  uint32_t pb[kNB][2];
+  float w[kNB][4];
+  bool grow = false;
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
-    float w[4];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const float p0 = pr[nb][c], p1 = pr[nb][2 + c];
       // a hidden token's weight is 0 whatever its parameters hold
-      w[c] = p0 == 0.0f ? 0.0f : p0 * f0;
-      w[2 + c] = p1 == 0.0f ? 0.0f : p1 * f1;
+      w[nb][c] = p0 == 0.0f ? 0.0f : p0 * (u0 * s.down[nb][c]);
+      w[nb][2 + c] = p1 == 0.0f ? 0.0f : p1 * (u1 * s.down[nb][c]);
       if constexpr (kF == dev::kInt4) {
         if (p0 != 0.0f) s.bias[nb][c] = fmaf(p0, beta0, s.bias[nb][c]);
         if (p1 != 0.0f) s.bias[nb][c] = fmaf(p1, beta1, s.bias[nb][c]);
       }
     }
-    pb[nb][0] = transpose8(dev::pack_f16x2(w[0], w[1]));
-    pb[nb][1] = transpose8(dev::pack_f16x2(w[2], w[3]));
+    grow = grow || too_large(w[nb][0], w[nb][1], w[nb][2], w[nb][3]);
+  }
+  if (__any_sync(0xFFFFFFFFu, grow)) {
+    if constexpr (kF == dev::kE4M3 || kF == dev::kE5M2) without_zeros<kNB>(zero_rows<kD, kF>(v.t, at), w);
+    follow_weights(s, w);
+  }
+  uint32_t pb[kNB][2];
+#pragma unroll
+  for (int nb = 0; nb < kNB; ++nb) {
+    pb[nb][0] = transpose8(dev::pack_f16x2(w[nb][0], w[nb][1]));
+    pb[nb][1] = transpose8(dev::pack_f16x2(w[nb][2], w[nb][3]));
   }
   const uint32_t token_bytes = at.heads * kRb;
   const uint32_t base = lds32(v.t + 16) + (at.head_i + 2 * quad * at.heads) * kRb + g * (kRb / 8);
@@ -602,24 +664,13 @@ __device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, 
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < 8; ++k) bad = bad || has_nonfinite(lo[k]) || has_nonfinite(hi[k]);
-    if (__any_sync(0xFFFFFFFFu, bad) || apart) {
+    if (__any_sync(0xFFFFFFFFu, bad)) {
 #pragma unroll 1
       for (int col = 0; col < 8 * kNB; ++col) {
-        // this row's view of the 16 tokens, and the exponent of the scales that it sees
+        // this row's view of the 16 tokens
         const int32_t row_at = position<kD, kNB>(at, col);
-        const uint32_t mine = __reduce_max_sync(0xFFFFFFFFu, max(visible(p, row_at, v, g) ? fin0 : 0u,
-                                                                visible(p, row_at, v, g + 8) ? fin1 : 0u));
-        const int ec = min(max(static_cast<int>(mine >> 23) - 127, -60), 60);
-        const float dc = pow2(-ec), up = exp2f(static_cast<float>(ec - s.E));
         const int nb = col >> 3;
-        float x[4];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float p0 = nb == 0 ? pr[0][c] : pr[kNB - 1][c], p1 = nb == 0 ? pr[0][2 + c] : pr[kNB - 1][2 + c];
-          x[c] = p0 == 0.0f ? 0.0f : p0 * (u0 * dc);
-          x[2 + c] = p1 == 0.0f ? 0.0f : p1 * (u1 * dc);
-        }
-        const uint32_t x0 = transpose8(dev::pack_f16x2(x[0], x[1])), x1 = transpose8(dev::pack_f16x2(x[2], x[3]));
+        const uint32_t x0 = nb == 0 ? pb[0][0] : pb[kNB - 1][0], x1 = nb == 0 ? pb[0][1] : pb[kNB - 1][1];
         const uint32_t keep_lo = (visible(p, row_at, v, 2 * quad) ? 0xFFFFu : 0u) | (visible(p, row_at, v, 2 * quad + 1) ? 0xFFFF0000u : 0u);
         const uint32_t keep_hi = (visible(p, row_at, v, 2 * quad + 8) ? 0xFFFFu : 0u) |
                                  (visible(p, row_at, v, 2 * quad + 9) ? 0xFFFF0000u : 0u);
@@ -632,8 +683,8 @@ __device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, 
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               if (static_cast<int>(b * 8 + quad * 2 + c) == col) {
-                s.acc[b][4 * i + k][c] = fmaf(t[c], up, s.acc[b][4 * i + k][c]);
-                s.acc[b][4 * i + k][2 + c] = fmaf(t[2 + c], up, s.acc[b][4 * i + k][2 + c]);
+                s.acc[b][4 * i + k][c] += t[c];
+                s.acc[b][4 * i + k][2 + c] += t[2 + c];
               }
             }
           }
@@ -1163,7 +1214,6 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
       // turn: the second leaves its state in the buffer, the first joins it to its own warp by warp and
       // leaves the sum there.  Groups of different rows use the buffer one after the other.
       const uint32_t g = lane >> 2, quad = lane & 3;
-      const float unit = s.E == kNoExponent ? 0.0f : exp2f(static_cast<float>(s.E));
       float* mine = merge + w8 * 8 * C::kRowsPad;
       const Rows rows = rows_of(p, head.z);
       const uint32_t head0 = head.w, heads = at.heads, n_rows = rows.q * p.group;
@@ -1175,6 +1225,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float l = s.l[0][c], b = s.bias[0][c], m_own = s.m[0][c], fo = 1.0f, ft = 0.0f;
+            const float unit = pow2(-exponent_of(s.down[0][c]));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               l += __shfl_xor_sync(0xFFFFFFFFu, l, o);

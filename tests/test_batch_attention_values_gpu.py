@@ -63,3 +63,116 @@ def test_weights_keep_their_sum_when_the_maximum_moves(hlkv_lib, cuda_device, D)
     s = k[:, 0, 0].astype(np.float64)
     want = (np.exp2(s) * v[:, 0, 0]).sum() / np.exp2(s).sum()
     assert 0.5 < want < 1 and np.abs(g - want).max() <= 2.0 ** -12 + 2.0 ** -18
+
+
+def _value_rows(wl, f):
+    """(slots of all of format f, codes [slots, T, H, row bytes], parameters [slots, T, H, floats]) of the V rows, on the
+    host; the arrays are views of what `_write` puts back."""
+    T, H, D = wl.T, wl.H, wl.D
+    rb, n = {1: (D, 1), 2: (D, 1), 3: (D // 2, 2)}[f]
+    host = wl.pools[f][0].cpu().numpy()
+    rows = T * H
+    codes = host[:, rows * rb:2 * rows * rb].reshape(-1, T, H, rb)
+    at = 2 * rows * rb + rows * n * 4
+    par = host[:, at:at + rows * n * 4].view(np.float32).reshape(-1, T, H, n)
+    return host, codes, par
+
+
+def _write(wl, f, host):
+    import torch
+    wl.pools[f][0].copy_(torch.from_numpy(host))
+
+
+def by_weight(b, x, scale):
+    """(out, bound) as attention_oracle's, with the part of weights below binary16's normal range counted against the
+    row's largest weighted value instead of its largest value.  A weight below the range is off by 2^-25 at most, its codes
+    in their unit are 1.75 at most, and a row's largest value is half its scale's unit at least.  The streaming kernel
+    keeps the largest weight at 2^6 or more: 2^-25 * 1.75 * 2 / 2^6 = 2^-29 of the largest weighted value.  The tile kernel keeps
+    it at 2^5, and less by the 2^6 that 16 tokens' scales may lie apart without being told apart: 2^-22.  Both are
+    below what is allowed, 2^-24 for each visible token, from 4 tokens on; and fewer tokens than 4 have no such weights
+    in these caches."""
+    from batch_helpers import block_rows, plan_oracle
+    from helpers import device_arena, device_table_words, host_pools
+    wl = b.wl
+    seqs, _, _, tf, _, err = plan_oracle(wl.segs_host, b.q, device_arena(wl), device_table_words(wl), b.T, 1, b.plan.c.block_cap,
+                                         b.cap, b.plan.c.max_query, b.window, b.sinks)
+    assert err == 0
+    pools, g = host_pools(wl), x.shape[1] // b.H
+    out, tol = np.zeros(x.shape), np.zeros(x.shape)
+    for i, s in enumerate(seqs):
+        rows = [block_rows(pools[info & 15], info & 15, slot, b.T, b.H, b.D)[0][:, :info >> 10 & 0x3FF] for slot, info, _, _ in s["blocks"]]
+        K, V = np.concatenate([r[0] for r in rows]), np.concatenate([r[1] for r in rows])
+        t = np.concatenate([start + np.arange(info >> 10 & 0x3FF) for _, info, _, start in s["blocks"]])
+        for r in range(s["q"]):
+            p = s["context"] - s["q"] + r
+            see = (t <= p) & ((b.window == 0) | (p - t < b.window) | (t < b.sinks))
+            for qh in range(x.shape[1]):
+                k, v, y = K[see, qh // g], V[see, qh // g], x[tf[i] + r, qh].astype(np.float64)
+                sc = scale * (k @ y)
+                w = np.exp(sc - sc.max())
+                w /= w.sum()
+                big = np.abs(v).max(1)
+                ds = scale * b.D * 2.0 ** -23 * (np.abs(k) @ np.abs(y)).max()
+                out[tf[i] + r, qh] = w @ v
+                tol[tf[i] + r, qh] = (2.0 ** -11 * np.abs(w @ v) + (2.0 ** -11 + 2 * ds) * 16 / 15 * (w @ big)
+                                      + len(v) * 2.0 ** -24 * (w * big).max() + 2.0 ** -25)
+    return out, tol
+
+
+def _attend(b, heads, scale):
+    import torch
+    x, d_q = b.queries(heads, 1)
+    got = b.run(d_q, scale)
+    again = b.run(d_q, scale)
+    torch.cuda.synchronize()
+    assert torch.equal(got, again) and int(b.err.item()) == 0
+    want, tol = by_weight(b, x, scale)
+    close(got, want, tol, sum(b.q))
+
+
+ROWS = [[1, 1], [3, 4]]  # new tokens: up to 8 rows, up to 16
+
+
+@pytest.mark.parametrize("sigma", [1.0, 0.1, 0.01])
+@pytest.mark.parametrize("f", [1, 2])
+@pytest.mark.parametrize("q", ROWS)
+@pytest.mark.parametrize("zeros", ["one of 16", "tiles"])
+def test_value_rows_of_zeros(hlkv_lib, cuda_device, sigma, f, q, zeros):
+    """Encoders give a row of zeros the scale 1, far above its neighbours'."""
+    def change(wl):
+        host, codes, par = _value_rows(wl, f)
+        par *= np.float32(sigma)
+        which = (slice(None), slice(5, 6)) if zeros == "one of 16" else (slice(0, None, 3), slice(None))
+        codes[which], par[which] = 0, 1.0
+        codes[which][..., ::2] = 0x80  # of both signs
+        _write(wl, f, host)
+
+    probs = [0, 0, 0, 0]
+    probs[f] = 1
+    b = Batch(hlkv_lib, 16, 2, 128, [[16] * 40, [16] * 21 + [9]], q, probs=probs, seed=5, change=change)
+    _attend(b, 8, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("probs", [(0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (0, 1, 1, 1)])
+@pytest.mark.parametrize("q", ROWS)
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("by", ["token", "block"])
+def test_value_scales_far_apart(hlkv_lib, cuda_device, probs, q, window, by):
+    """Value rows of 2^-14 to 2^6 side by side, and blocks of them, under flat scores and steep ones: the rows with much
+    weight may be the small ones."""
+    rng = np.random.default_rng(sum(q))
+
+    def change(wl):
+        for f in (1, 2, 3):
+            if not probs[f]:
+                continue
+            host, _, par = _value_rows(wl, f)
+            size = rng.uniform(-14, 6, par.shape[:3] if by == "token" else (par.shape[0], 1, 1))
+            par *= np.float32(2.0) ** size[..., None].astype(np.float32)
+            par[rng.random(par.shape[:3]) < 0.02] = 0  # constant rows of 0
+            _write(wl, f, host)
+
+    for D, scale in ((128, 128 ** -0.5), (64, 0.5)):
+        b = Batch(hlkv_lib, 16, 2, D, [[16] * 40, [16] * 21 + [9]], q, probs=probs, window=window, sinks=5 if window else 0, seed=7,
+                  change=change)
+        _attend(b, 8, scale)
