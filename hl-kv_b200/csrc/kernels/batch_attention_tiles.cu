@@ -12,7 +12,8 @@
 // the other's products run.  Tensor memory: S0, S1, O0, O1; P overwrites S.
 // As in the stream kernel a code's binary16 value is exact and its parameters stay outside: the K row's scale and
 // bias in the score, the V row's scale in the weight, its bias in a sum of its own, all in binary32.  A weight is
-// rounded once, to binary16, in units of 2^E that follow the exponents of the value scales (one for 16 tokens).
+// rounded once, to binary16 (2^-12 of it; the matrix unit takes no wider one at this rate), against a reference of its row
+// that follows scores and value scales together.
 // Codes are laid in the order (0, 4, 1, 5, 2, 6, 3, 7) of each 8, where the formats' words hold them: Q's elements
 // lie the same way, and the outputs are put back in order at the end.
 //
@@ -62,8 +63,9 @@ struct Shared {
   // Of the tokens of the last four tiles: a K half may be written again while the softmax of the tile two before
   // still reads these.
   alignas(16) float ks[4][kTile], kb[4][kTile], vs[4][kTile], vb[4][kTile];  // read four at a time
+  alignas(16) float es[4][kTile];  // where the scales of 16 tokens lie far apart: a token's exponent under theirs
   int exponent[4][kStageWarps];
-  uint32_t kind[4][kStageWarps];  // of 16 tokens: 1 a scale, 2 a bias, 4 some token does not exist
+  uint32_t kind[4][kStageWarps];  // of 16 tokens: 1 a scale, 2 a bias, 4 some token does not exist, 8 scales far apart
   uint32_t exists[4][kStageWarps];
   uint32_t tmem, redo;
 };
@@ -331,6 +333,16 @@ __device__ __forceinline__ RowTile row_tile_of_rank(const Params& p, uint32_t r)
   return RowTile{0u, 0xFFFFFFFFu};
 }
 
+// Whether an FP8 row holds zeros alone.  Out of line: few rows are looked at.
+__device__ __noinline__ bool zero_row(const uint8_t* row, uint32_t bytes) {
+  uint32_t any = 0;
+  for (uint32_t i = 0; i < bytes; i += 16) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + i));
+    any |= w.x | w.y | w.z | w.w;
+  }
+  return (any & 0x7F7F7F7Fu) == 0;
+}
+
 template <int kD>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ Params p) {
   using C = Config<kD>;
@@ -450,8 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       }
     }
     qsum *= p.qscale;
-    float m = -INFINITY, l = 0.0f, bias = 0.0f;
-    int E = 0;
+    float ref = -INFINITY, l = 0.0f, bias = 0.0f;  // of the row; l, bias and O in units of 2^ref
     if (acc < n_acc) {
       for (uint32_t j = 0; j < n_tiles; ++j) {
         const uint32_t info = j & 3;
@@ -464,12 +475,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // Whether all 128 rows see all 128 tokens.
         const int32_t t0 = static_cast<int32_t>(tp), acc_lo = pos_base + static_cast<int32_t>((row0 + acc * 128) / p.group);
         uint32_t any_kind = 0;
-        int e_tile = -1000;
 #pragma unroll
-        for (int g = 0; g < kStageWarps; ++g) {
-          any_kind |= sh.kind[info][g];
-          e_tile = max(e_tile, sh.exponent[info][g]);
-        }
+        for (int g = 0; g < kStageWarps; ++g) any_kind |= sh.kind[info][g];
         const bool masked = n < kTile || (any_kind & 4u) != 0 || t0 + 127 > acc_lo ||
                             (p.window != 0 && t0 + 128 > static_cast<int32_t>(min(p.sinks, 0x7FFFFF00u)) &&
                              p_hi - t0 >= static_cast<int32_t>(min(p.window, 0x7FFFFFFFu)));
@@ -512,7 +519,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           }
         };
         const Pair zero = pair(0.0f, 0.0f);
-        // ---- the accumulator's unit
         auto rescale = [&](float f) {  // O of this tile's row, once the products before have been added to it
           if (j == 0) return true;
           if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh.o_done[acc], (j - 1) & 1))) return false;
@@ -529,25 +535,19 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           wait_st();
           return true;
         };
-        const int e_new = min(max(e_tile, -60), 60);
-        if (j == 0) {
-          E = e_tile == -1000 ? 0 : e_new;
-        } else if (e_tile != -1000 && (e_new > E + 6 || e_new < E - 6)) {
-          ok = rescale(exp2f(static_cast<float>(E - e_new)));
-          if (!ok) break;
-          E = e_new;
-        }
-        // ---- weights, in one pass: 32 tokens at a time, against the reference maximum so far.  Where a score passes
-        // it by more than 8 (weights reach 2^8 at most), the maximum moves, and what was made with the old one
-        // (O, the sums, this tile's weights so far) is scaled.
+        // ---- weights, in one pass: 32 tokens at a time, against the row's reference so far.  A token counts by its score
+        // and the exponent of its 16 tokens' value scales (its own where these lie far apart), so that a weight, the
+        // exponential times the scale, is at most 2^14 where no sum passes the reference by more than kAbove.  Where one
+        // does, the reference moves to kBelow under it, by a whole number, and what was made with the old one (O, the
+        // sums, this tile's weights so far) is scaled by a power of two.  So the largest weight is in [2^5, 2^14], and
+        // binary16 holds those down to 2^-19 of it without a loss, whatever other rows and tokens hold.
+        constexpr float kAbove = 14.0f, kBelow = 6.0f;
 #pragma unroll 1
         for (uint32_t c = 0; c < (n + 31) / 32; ++c) {  // the products take no further tokens
-          // a group's weights are in units of 2^(its exponent), the sums in their own
           const uint32_t kind0 = sh.kind[info][2 * c], kind1 = sh.kind[info][2 * c + 1];
-          const int d0 = (kind0 & 3u ? min(max(sh.exponent[info][2 * c], -60), 60) : 0) - E;
-          const int d1 = (kind1 & 3u ? min(max(sh.exponent[info][2 * c + 1], -60), 60) : 0) - E;
-          const float ref = m == -INFINITY ? 0.0f : m;
-          const float add0 = static_cast<float>(d0) - ref, add1 = static_cast<float>(d1) - ref;
+          const int e0 = kind0 & 3u ? sh.exponent[info][2 * c] : 0, e1 = kind1 & 3u ? sh.exponent[info][2 * c + 1] : 0;
+          const float from = ref == -INFINITY ? 0.0f : ref;
+          const float add0 = static_cast<float>(e0) - from, add1 = static_cast<float>(e1) - from;
           Pair x[16];
           scores(c, pair(add0, add0), pair(add1, add1), x);
           float top0 = -INFINITY, top1 = -INFINITY;
@@ -557,40 +557,52 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             top0 = fmaxf(top0, fmaxf(u.x, u.y));
             top1 = fmaxf(top1, fmaxf(v.x, v.y));
           }
-          const float top = fmaxf(top0 - static_cast<float>(d0), top1 - static_cast<float>(d1));  // above the reference
-          const bool grow = top > (m == -INFINITY ? -INFINITY : 8.0f);
-          if (__any_sync(0xFFFFFFFFu, grow)) {
-            // The maximum moves to ref + up, by a whole number: the factor is a power of two, so that the weights made
-            // so far are not rounded again (but those that fall below binary16's normal range).
-            const float up = grow ? ceilf(top) : 0.0f;
-            const float a = m == -INFINITY ? (grow ? 0.0f : 1.0f) : exp2f(-up);
-            ok = rescale(a);
-            if (!ok) break;
-            if (grow) m = ref + up;
-            l *= a;
-            bias *= a;
-            wait_st();  // this tile's weights so far: a load is ordered behind the stores before it by this alone
-#pragma unroll 1
-            for (uint32_t k = 0; k < c; ++k) {
-              uint32_t w[16];
-              tmem_load16(t_s + k * 16, w);
-              wait_ld();
+          float top = fmaxf(top0, top1);  // above the reference
+          const float above = ref == -INFINITY ? -INFINITY : kAbove;
+          if (__any_sync(0xFFFFFFFFu, top > above)) {
+            if ((kind0 | kind1) & 8u) {  // each token by its own scale
+              const float4* es = reinterpret_cast<const float4*>(&sh.es[info][c * 32]);
+              top = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                w[i] = dev::pack_f16x2(v.x * a, v.y * a);
+              for (int i = 0; i < 8; ++i) {
+                const float4 d = (i < 4 ? kind0 : kind1) & 8u ? es[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float2 u = split(x[2 * i]), v = split(x[2 * i + 1]);
+                top = fmaxf(top, fmaxf(fmaxf(u.x + d.x, u.y + d.y), fmaxf(v.x + d.z, v.y + d.w)));
               }
-              tmem_store16(t_s + k * 16, w);
             }
-            const Pair down = pair(-up, -up);
+            const bool grow = top > above;
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+              const float up = grow ? ceilf(top) - kBelow : 0.0f;
+              const float a = ref == -INFINITY ? (grow ? 0.0f : 1.0f) : halvings(up);
+              ok = rescale(a);
+              if (!ok) break;
+              if (grow) ref = from + up;
+              l *= a;
+              bias *= a;
+              wait_st();  // this tile's weights so far: a load is ordered behind the stores before it by this alone
+#pragma unroll 1
+              for (uint32_t k = 0; k < c; ++k) {
+                uint32_t w[16];
+                tmem_load16(t_s + k * 16, w);
+                wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = add2(x[i], down);
+                for (int i = 0; i < 16; ++i) {
+                  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                  w[i] = dev::pack_f16x2(v.x * a, v.y * a);
+                }
+                tmem_store16(t_s + k * 16, w);
+              }
+              const Pair down = pair(-up, -up);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = add2(x[i], down);
+            }
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 v = split(x[i]);
             x[i] = pair(ex2(v.x), ex2(v.y));
           }
+          const float back0 = pow2(-e0), back1 = pow2(-e1);  // the sums leave the exponents out
           Pair s0 = x[0], s1 = x[8];
 #pragma unroll
           for (int i = 1; i < 8; ++i) {
@@ -598,7 +610,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             s1 = add2(s1, x[8 + i]);
           }
           const float2 l0 = split(s0), l1 = split(s1);
-          const float back0 = pow2(-d0), back1 = pow2(-d1);
           l = fmaf(l0.x + l0.y, back0, fmaf(l1.x + l1.y, back1, l));
           if ((kind0 | kind1) & 2u) {
             const float4* vb = reinterpret_cast<const float4*>(&sh.vb[info][c * 32]);
@@ -639,8 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       if (ok && n_tiles > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh.o_done[acc], (n_tiles - 1) & 1));
       if (ok) {
         fence_after();
-        const float unit = exp2f(static_cast<float>(E));
-        const bool none = m == -INFINITY && l == 0.0f;
+        const bool none = ref == -INFINITY && l == 0.0f;
 #pragma unroll 1
         for (uint32_t c = 0; c < kD / 32; ++c) {
           uint32_t o[32];
@@ -651,13 +661,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           __syncwarp();
           if (sh.split) {
             float* dst = p.tile_partial + (uint64_t{blockIdx.x} * kRowsCta + acc * 128 + r) * (kD + 4);
-            if (c == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(m, l);
+            if (c == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(ref, l);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {  // in the order of the accumulators: join_kernel puts it right
               float4 y;
               float* x = &y.x;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[i] = none ? 0.0f : fmaf(__uint_as_float(o[4 * k + i]), unit, bias);
+              for (int i = 0; i < 4; ++i) x[i] = none ? 0.0f : __uint_as_float(o[4 * k + i]) + bias;
               reinterpret_cast<float4*>(dst + c * 32)[k] = y;
             }
             continue;
@@ -670,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             for (int i = 0; i < 4; ++i) {
               // elements 2 i and 2 i + 1 of the 8 lie at 0 4 1 5 2 6 3 7
               const int e0 = 8 * k + (i < 2 ? 4 * i : 4 * (i - 2) + 1), e1 = e0 + 2;
-              const float a = none ? 0.0f : fmaf(__uint_as_float(o[e0]), unit, bias) / l, b = none ? 0.0f : fmaf(__uint_as_float(o[e1]), unit, bias) / l;
+              const float a = none ? 0.0f : (__uint_as_float(o[e0]) + bias) / l, b = none ? 0.0f : (__uint_as_float(o[e1]) + bias) / l;
               y[i] = dev::pack_f16x2(a, b);
             }
             if (live) dst[k] = make_uint4(y[0], y[1], y[2], y[3]);
@@ -746,6 +756,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             tok.k = reinterpret_cast<uint64_t>(payload) + uint64_t{row} * (tok.f == dev::kFp16 ? kD * 2 : tok.f == dev::kInt4 ? kD / 2 : kD);
             tok.kp = params_of_row(tok.f, entry.y, entry.z, payload + p.code_bytes[tok.f], row);
             tok.vp = params_of_row(tok.f, entry.y, entry.z, payload + p.code_bytes[tok.f], row + p.T * p.H);
+            if (tok.f != dev::kFp16 && tok.f != dev::kInt4 && ((entry.y >> 4) & 3u) == 0 && tok.vp.x == 1.0f) {
+              // What encoders store for an FP8 row of zeros: a size that its values do not have.
+              if (zero_row(payload + (uint64_t{row} + uint64_t{p.T} * p.H) * kD, kD)) tok.vp.x = 0.0f;
+            }
           }
         }
       }
@@ -850,9 +864,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       const float unit = f == dev::kFp16 ? 1.0f : f == dev::kE4M3 ? 0x1p8f : f == dev::kE5M2 ? 0x1p15f : 8.0f;
       const float u = f > 3 ? 0.0f : tok.vp.x * unit;
       const uint32_t ub = __float_as_uint(u) & 0x7FFFFFFFu;
+      // The 16 tokens' exponent is that of their largest scale.  Where others, zeros among them, lie more than 2^6 below
+      // it, each token counts in the reference by its own (2^-100 of the largest at least: the exponentials, of up to
+      // 2^113 then, and their sums stay in binary32's range).
       const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, ub < 0x7F800000u ? ub : 0u);
+      const bool apart = __any_sync(0xFFFFFFFFu, f <= 3 && ub < 0x7F800000u && top > ub + (6u << 23));
+      auto exponent_of = [](uint32_t bits) { return min(max(static_cast<int>(bits >> 23) - 127, -60), 60); };
+      const int e = exponent_of(top), below = ub < 0x7F800000u ? max(exponent_of(ub) - e, -100) : 0;
       const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, f > 3 ? 0xFFFFFFFFu : ub);
-      const int e = min(max(static_cast<int>(top >> 23) - 127, -60), 60);
       // A tile that some row sees in part: values that are not finite, or scales far apart, would touch rows that
       // do not see them.  Such a CTA's rows are done over, one by one.
       const int32_t t0 = static_cast<int32_t>(tp);
@@ -880,11 +899,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             sh.ks[info][i] = f > 3 ? 0.0f : tok.kp.x * (p.qscale * (f == dev::kInt4 ? 8.0f : 1.0f));
             sh.kb[info][i] = f == dev::kInt4 ? fmaf(8.0f, tok.kp.x, tok.kp.y) : 0.0f;
             sh.vs[info][i] = scaled ? u * pow2(-e) : 1.0f;
+            if (apart) sh.es[info][i] = static_cast<float>(below);
             sh.vb[info][i] = f == dev::kInt4 ? fmaf(8.0f, tok.vp.x, tok.vp.y) : 0.0f;
             if (lane == 0) {
-              sh.kind[info][sw] = kinds;
+              sh.kind[info][sw] = kinds | (apart ? 8u : 0u);
               sh.exists[info][sw] = exists;
-              sh.exponent[info][sw] = scaled ? (top ? e : -1000) : 0;
+              sh.exponent[info][sw] = e;
             }
           }
         }

@@ -130,7 +130,7 @@ def _attend(b, heads, scale):
     close(got, want, tol, sum(b.q))
 
 
-ROWS = [[1, 1], [3, 4]]  # new tokens: up to 8 rows, up to 16
+ROWS = [[1, 1], [3, 4], [70, 40]]  # new tokens: up to 8 rows, up to 16, row tiles
 
 
 @pytest.mark.parametrize("sigma", [1.0, 0.1, 0.01])
