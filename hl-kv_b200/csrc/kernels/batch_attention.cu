@@ -102,8 +102,9 @@ extern "C" int hlkv_batch_attention(const HlkvPools* pools, const HlkvLayout* la
   p.tile_partial = reinterpret_cast<float*>(static_cast<uint8_t*>(d_workspace) +
                                             stream_workspace(p.nseq, H, layout->head_dim, p.max_rows, p.ctas));
   p.tile_redo = reinterpret_cast<uint32_t*>(p.tile_partial + uint64_t{p.ctas} * 256 * (D + 4));
+  p.tile_ranks = tile_ranks(p);
   const uint64_t tiles = p.max_rows <= kStreamRows ? 0u : tile_ctas(p);
-  if (tiles > 0x7FFFFFFFull) return HLKV_INVALID_ARGUMENT;
+  if (tiles > 0x7FFFFFFFull || (p.tile_ranks != 0 && tiles_of_plan(p) * H > 0x7FFFFFFFull)) return HLKV_INVALID_ARGUMENT;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const cudaError_t e = launch_stream(layout->head_dim, p, s);
   if (e != cudaSuccess || tiles == 0) return cuda_status(e);

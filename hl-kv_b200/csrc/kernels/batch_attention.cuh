@@ -49,6 +49,7 @@ struct Params {
   // tile kernel and join
   float* tile_partial;  // [ctas][256][kD + 4]
   uint32_t* tile_redo;  // [ctas]
+  uint32_t tile_ranks;  // more than 128 sequences: CTAs (of a head) take ranks; 0: one for each tile of the plan
 };
 
 // The new tokens of sequence i: rows [first, first + q) of Q, kept inside the arrays whatever the
@@ -288,6 +289,8 @@ cudaError_t launch_stream(uint32_t head_dim, const Params& p, cudaStream_t s);
 size_t stream_workspace(uint32_t nseq, uint32_t H, uint32_t head_dim, uint32_t max_rows, uint32_t ctas);
 void stream_layout(Params* p, void* ws);
 size_t tile_workspace(uint32_t nseq, uint32_t head_dim, uint32_t max_rows, uint32_t ctas);
+uint64_t tiles_of_plan(const Params& p);
+uint32_t tile_ranks(const Params& p);
 uint64_t tile_ctas(const Params& p);  // the tile kernel's grid: 0 when no sequence can have its rows
 cudaError_t launch_tiles(uint32_t head_dim, const Params& p, cudaStream_t s);
 

@@ -68,6 +68,7 @@ struct Shared {
   uint32_t kind[4][kStageWarps];  // of 16 tokens: 1 a scale, 2 a bias, 4 some token does not exist, 8 scales far apart
   uint32_t exists[4][kStageWarps];
   uint32_t tmem, redo;
+  uint32_t sums[kThreads / 32];
 };
 
 // ---- tcgen05 ---------------------------------------------------------------------------------------
@@ -343,6 +344,57 @@ __device__ __noinline__ bool zero_row(const uint8_t* row, uint32_t bytes) {
   return (any & 0x7F7F7F7Fu) == 0;
 }
 
+// The r-th (sequence, row tile) of a batch of many sequences, the last tiles of all sequences first: tiles o from a
+// sequence's last one on make level o, and the levels before it hold the sum of min(row tiles, o).  Found by the CTA, a
+// thread for consecutive sequences.
+__device__ __noinline__ RowTile row_tile_of_many(const Params& p, uint32_t r, uint32_t* sums, RowTile* found) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t chunk = (p.nseq + kThreads - 1) / kThreads, a = min(threadIdx.x * chunk, p.nseq), b = min(a + chunk, p.nseq);
+  auto before = [&](uint32_t o) {
+    uint32_t c = 0;
+    for (uint32_t i = a; i < b; ++i) c += min(row_tiles_above(p, i, 0, 0), o);
+    c = __reduce_add_sync(0xFFFFFFFFu, c);
+    if (lane == 0) sums[warp] = c;
+    __syncthreads();
+    uint32_t all = 0;
+    for (uint32_t w = 0; w < kThreads / 32; ++w) all += sums[w];
+    __syncthreads();
+    return all;
+  };
+  uint32_t lo = 0, hi = static_cast<uint32_t>((uint64_t{p.max_rows} + kRowsCta - 1) / kRowsCta), skip = 0;
+  if (r >= before(hi)) return RowTile{0u, 0xFFFFFFFFu};
+  while (hi - lo > 1) {
+    const uint32_t o = (lo + hi) / 2, n = before(o);
+    if (n <= r) {
+      lo = o;
+      skip = n;
+    } else {
+      hi = o;
+    }
+  }
+  uint32_t mine = 0;
+  for (uint32_t i = a; i < b; ++i) mine += row_tiles_above(p, i, 0, 0) > lo;
+  uint32_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+    if (lane >= static_cast<uint32_t>(o)) upto += y;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  for (uint32_t w = 0; w < warp; ++w) upto += sums[w];
+  uint32_t left = r - skip;  // place in the level
+  if (left < upto && left >= upto - mine) {
+    left -= upto - mine;
+    for (uint32_t i = a; i < b; ++i) {
+      const uint32_t n = row_tiles_above(p, i, 0, 0);
+      if (n > lo && left-- == 0) *found = RowTile{i, n - 1 - lo};
+    }
+  }
+  __syncthreads();
+  return *found;
+}
+
 template <int kD>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ Params p) {
   using C = Config<kD>;
@@ -375,6 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     mine = sh.mine;
     splits = sh.splits;
     part = sh.part;
+  } else if (p.tile_ranks != 0) {
+    mine = row_tile_of_many(p, blockIdx.x / p.H, sh.sums, &sh.mine);
   } else {  // last tiles of all sequences first
     const uint32_t seq = blockIdx.x / p.H % p.nseq, order = blockIdx.x / p.H / p.nseq;
     const uint64_t n_rows = uint64_t{rows_of(p, seq).q} * p.group, n = (n_rows + kRowsCta - 1) / kRowsCta;
@@ -1074,16 +1128,28 @@ cudaError_t launch(const Params& p, cudaStream_t s) {
 
 }  // namespace
 
+// A tile for each 256 rows that every sequence may have.
+uint64_t tiles_of_plan(const Params& p) { return uint64_t{p.nseq} * ((uint64_t{p.max_rows} + kRowsCta - 1) / kRowsCta); }
+// CTAs that take ranks need be no more than the batch's tokens can make: whole tiles, and one more for each sequence of
+// more than kStreamRows rows.
+uint64_t tiles_of_tokens(const Params& p) {
+  const uint64_t rows = uint64_t{p.token_cap} * p.group;
+  return rows / kRowsCta + std::min<uint64_t>(p.nseq, rows / (kStreamRows + 1));
+}
+
+// Past kOrdered sequences a CTA for each tile of the plan needs no look-up, and a plan whose sequences may have many
+// more rows than its tokens make is taken by ranks.  (250 sequences of up to 300 new tokens: 4421 us in a plan for 300 new
+// tokens each, without ranks; in one for 8192, 5955 us without and 4578 with them.  129 sequences of one new token
+// in that plan: 934 and 60 us.)
+uint32_t tile_ranks(const Params& p) {
+  if (p.nseq <= kOrdered || tiles_of_plan(p) <= 2 * tiles_of_tokens(p)) return 0;
+  return static_cast<uint32_t>(tiles_of_tokens(p));
+}
+
 uint64_t tile_ctas(const Params& p) {
-  uint64_t tiles = uint64_t{p.nseq} * ((uint64_t{p.max_rows} + kRowsCta - 1) / kRowsCta);
-  if (p.nseq <= kOrdered) {
-    // CTAs take ranks, so no more are needed than the batch's tokens can make: whole tiles, and one more for each
-    // sequence of more than kStreamRows rows.
-    const uint64_t rows = uint64_t{p.token_cap} * p.group, most = rows / kRowsCta + std::min<uint64_t>(p.nseq, rows / (kStreamRows + 1));
-    tiles = std::min(tiles, most);
-    return tiles == 0 ? 0u : std::max<uint64_t>(tiles * p.H, p.ctas);  // (parts of few)
-  }
-  return tiles * p.H;
+  if (p.nseq > kOrdered) return (p.tile_ranks != 0 ? p.tile_ranks : tiles_of_plan(p)) * p.H;
+  const uint64_t tiles = std::min(tiles_of_plan(p), tiles_of_tokens(p));
+  return tiles == 0 ? 0u : std::max<uint64_t>(tiles * p.H, p.ctas);  // (parts of few)
 }
 size_t tile_workspace(uint32_t nseq, uint32_t head_dim, uint32_t max_rows, uint32_t ctas) {
   if (max_rows <= kStreamRows || nseq > kOrdered) return 0;

@@ -462,7 +462,8 @@ int hlkv_rotary_append(const HlkvPools* pools, const HlkvLayout* layout, const H
  *    overlaps nothing else.  Rows behind the last new token are left as they were; those of a
  *    sequence that the plan could not hold (HLKV_ERR_PLAN_RANGE) are zeros or as they were.
  *  - head_dim 64 or 128; kv_heads at most 128; q_heads / kv_heads 1 .. 32; softmax_scale in
- *    (0, 2^60].
+ *    (0, 2^60]; token_cap * q_heads and, past 128 sequences, nseq * ceil(max_query * q_heads /
+ *    kv_heads / 256) * kv_heads below 2^31.
  *  - d_workspace: 16-byte aligned, hlkv_batch_attention_workspace_bytes(plan, layout, q_heads)
  *    bytes, needing no initial value.  Calls that overlap on the GPU must not share one.
  *  - A listed block whose pool or slot is missing is left out, with its HLKV_ERR_* bit.

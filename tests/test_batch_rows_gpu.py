@@ -63,3 +63,29 @@ def test_sequences_that_the_plan_cannot_hold(hlkv_lib, cuda_device, nseq, max_qu
 def test_blocks_that_do_not_fit(hlkv_lib, cuda_device, q):
     b = Batch(hlkv_lib, 16, 2, 64, [[16] * 9, [16] * 12, []], [q, q, q], seed=3)
     _check(hlkv_lib, b, 8, q, block_cap=15)
+
+
+@pytest.mark.parametrize("nseq", [129, 600, 1200])
+@pytest.mark.parametrize("q", ["one token", "some chunks", "all"])
+def test_many_sequences_in_a_plan_for_long_prompts(hlkv_lib, cuda_device, nseq, q):
+    """Past 128 sequences the tile kernel's grid goes by the batch's tokens where a plan holds more rows than they make."""
+    import torch
+    rng = np.random.default_rng(nseq)
+    lens = [1] * nseq
+    if q == "some chunks":
+        for i in (0, 7, nseq // 2, nseq - 1):
+            lens[i] = int(rng.integers(17, 700))
+    elif q == "all":
+        lens = [int(n) for n in rng.choice([0, 1, 5, 9, 40], nseq)]
+    vt = [[16] * (n // 16) + [n % 16 or 16] for n in lens]
+    b = Batch(hlkv_lib, 16, 1, 64, vt, lens, seed=nseq, pad=50)
+    b.plan = hlkv_lib.BatchPlan(nseq, b.plan.c.block_cap, b.cap, 1 << 20)
+    b.fill_plan()
+    x, d_q = b.queries(4, 1)
+    got = b.run(d_q, 0.125)
+    torch.cuda.synchronize()
+    want, tol, err = b.want(x, 0.125)
+    assert int(b.err.item()) == err == 0
+    n = sum(lens)
+    assert (got[n:] == 0x1234).all()
+    assert (np.abs(got.cpu().numpy().view(np.float16).astype(np.float64)[:n] - want[:n]) <= tol[:n]).all()
