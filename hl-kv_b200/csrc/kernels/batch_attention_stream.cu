@@ -3,8 +3,9 @@
 // The bound is memory: a token of a KV head is 512 (FP16), 264 (FP8) or 144 bytes (INT4) of K and V for
 // heads of 128, read once, against 4 * 128 operations for each of at most 16 query rows.
 //
-// One CTA per SM takes an equal share of the batch's cost (the plan's per-block costs, in proportion
-// to the bytes), whatever the sequences' lengths: its range of the line on which all (sequence, head
+// One CTA per SM takes an equal share of the batch's cost (the plan's per-block costs, in proportion to the time measured
+// for a tile of a cache of one format: 14 for FP16, 7 for FP8 and INT4, taken with 8 heads of 128 and used for all
+// shapes), whatever the sequences' lengths: its range of the line on which all (sequence, head
 // group) units lie end to end.  Two producer warps (K, V) copy the blocks' codes and parameters as they are,
 // by bulk copies, into a byte ring in shared memory: tiles of 16 tokens of a block, all heads of the
 // group (up to 8) at once, so that a copy is one long piece of the slot; a ring of bytes, not of
@@ -210,22 +211,22 @@ __device__ __forceinline__ float2 lds_f2(uint32_t a) {
 }
 
 // A warp's state for one (unit, head): lane (g, q) = (lane / 4, lane % 4) holds query columns 2q and
-// 2q + 1 of each column block, and head elements [g kD/8, (g + 1) kD/8).
-template <int kD, int kNB>
+// 2q + 1, and head elements [g kD/8, (g + 1) kD/8).
+template <int kD>
 struct State {
-  float acc[kNB][kD / 16][4];  // [.][mt]: element 2 mt of columns 2q, 2q + 1, then element 2 mt + 1; units of 2^m / down
-  float m[kNB][2], l[kNB][2], bias[kNB][2];  // l and bias: this lane's tokens only, in units of 2^m
-  float down[kNB][2];                        // a power of two
+  float acc[kD / 16][4];       // [mt]: element 2 mt of columns 2q, 2q + 1, then element 2 mt + 1; units of 2^m / down
+  float m[2], l[2], bias[2];   // l and bias: this lane's tokens only, in units of 2^m
+  float down[2];               // a power of two
 };
 constexpr int kMostDown = 60;  // down is in 2^+-60: sizes of values from 2^-74 to 2^58 are followed
 
 // What a warp keeps in shared memory for a piece: its Q^T fragments, and per column the scaled sum of q
 // and the position.
-template <int kD, int kNB>
+template <int kD>
 struct WarpRows {
-  uint4 q[kNB * (kD / 32)][32];  // column g, pairs (j, j + 4) of the 8-element groups of a quarter row
-  float qsum[8 * kNB];
-  int32_t pos[8 * kNB];
+  uint4 q[kD / 32][32];  // column g, pairs (j, j + 4) of the 8-element groups of a quarter row
+  float qsum[8];
+  int32_t pos[8];
   uint4 place;  // heads, head, first tile of a stage, tiles per round
 };
 
@@ -235,46 +236,43 @@ struct Place {
   uint32_t heads, head_i, lane;
 };
 
-template <int kD, int kNB>
-__device__ __forceinline__ void begin_piece(const Params& p, State<kD, kNB>& s, WarpRows<kD, kNB>* wr, Rows rows, uint32_t context,
+template <int kD>
+__device__ __forceinline__ void begin_piece(const Params& p, State<kD>& s, WarpRows<kD>* wr, Rows rows, uint32_t context,
                                             uint32_t head, uint32_t row0, uint32_t lane) {
   const uint32_t g = lane >> 2, quad = lane & 3;
+  const uint32_t r = row0 + g, tok = r / p.group, in_group = r % p.group;
+  const bool live = r < rows.q * p.group;
+  const uint4* src = reinterpret_cast<const uint4*>(p.q + (rows.first + (live ? tok : 0u)) * p.q_stride +
+                                                    uint64_t{head * p.group + (live ? in_group : 0u)} * kD) +
+                     quad * (kD / 32);
+  float sum = 0.0f;
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
-    const uint32_t r = row0 + nb * 8 + g, tok = r / p.group, in_group = r % p.group;
-    const bool live = r < rows.q * p.group;
-    const uint4* src = reinterpret_cast<const uint4*>(p.q + (rows.first + (live ? tok : 0u)) * p.q_stride +
-                                                      uint64_t{head * p.group + (live ? in_group : 0u)} * kD) +
-                       quad * (kD / 32);
-    float sum = 0.0f;
+  for (int i = 0; i < kD / 32; ++i) {
+    const uint4 w = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    uint32_t a[4];
+    k_pairs<dev::kFp16>(x, a);
+    wr->q[i][lane] = make_uint4(a[0], a[1], a[2], a[3]);
 #pragma unroll
-    for (int i = 0; i < kD / 32; ++i) {
-      const uint4 w = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-      uint32_t a[4];
-      k_pairs<dev::kFp16>(x, a);
-      wr->q[nb * (kD / 32) + i][lane] = make_uint4(a[0], a[1], a[2], a[3]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[j]));
-        sum += f.x + f.y;
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[j]));
+      sum += f.x + f.y;
     }
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-    if (quad == 0) {
-      wr->qsum[nb * 8 + g] = sum * p.qscale;
-      wr->pos[nb * 8 + g] = static_cast<int32_t>(context - rows.q + tok);
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      s.m[nb][c] = -INFINITY;
-      s.l[nb][c] = s.bias[nb][c] = 0.0f;
-      s.down[nb][c] = pow2(kMostDown);
-    }
-#pragma unroll
-    for (int mt = 0; mt < kD / 16; ++mt) s.acc[nb][mt][0] = s.acc[nb][mt][1] = s.acc[nb][mt][2] = s.acc[nb][mt][3] = 0.0f;
   }
+  sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+  sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+  if (quad == 0) {
+    wr->qsum[g] = sum * p.qscale;
+    wr->pos[g] = static_cast<int32_t>(context - rows.q + tok);
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    s.m[c] = -INFINITY;
+    s.l[c] = s.bias[c] = 0.0f;
+    s.down[c] = pow2(kMostDown);
+  }
+#pragma unroll
+  for (int mt = 0; mt < kD / 16; ++mt) s.acc[mt][0] = s.acc[mt][1] = s.acc[mt][2] = s.acc[mt][3] = 0.0f;
   __syncwarp();
 }
 
@@ -298,8 +296,8 @@ __device__ __forceinline__ void row_params(uint32_t t, uint32_t word, const Plac
 }
 
 // Scores of tiles t[] in units of log2: lane (g, quad) has tokens g, g + 8 of columns 2 quad, 2 quad + 1.
-template <int kD, int kNB, uint32_t kF, int kNT>
-__device__ __forceinline__ void scores(const Params& p, const uint32_t (&t)[kNT], const Place& at, float (&sc)[kNT][kNB][4]) {
+template <int kD, uint32_t kF, int kNT>
+__device__ __forceinline__ void scores(const Params& p, const uint32_t (&t)[kNT], const Place& at, float (&sc)[kNT][4]) {
   const uint32_t g = at.lane >> 2, quad = at.lane & 3;
   constexpr uint32_t kRb = kRow<kD, kF>;
   constexpr int kW = kWords<kF>;
@@ -311,8 +309,7 @@ __device__ __forceinline__ void scores(const Params& p, const uint32_t (&t)[kNT]
 #pragma unroll
   for (int k = 0; k < kNT; ++k) {
     r0[k] = lds32(t[k] + 8) + row;
-#pragma unroll
-    for (int nb = 0; nb < kNB; ++nb) sc[k][nb][0] = sc[k][nb][1] = sc[k][nb][2] = sc[k][nb][3] = 0.0f;
+    sc[k][0] = sc[k][1] = sc[k][2] = sc[k][3] = 0.0f;
   }
   const uint32_t qa = at.rows + at.lane * 16;
 #pragma unroll
@@ -334,12 +331,9 @@ __device__ __forceinline__ void scores(const Params& p, const uint32_t (&t)[kNT]
         uint32_t a[4], b[4];
         k_pairs<kF>(w[k][0] + j * kW, a);
         k_pairs<kF>(w[k][1] + j * kW, b);
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          const uint4 q = lds128(qa + (nb * kG8 + i + j) * 512);
-          mma16816(sc[k][nb], a[0], b[0], a[1], b[1], q.x, q.y);
-          mma16816(sc[k][nb], a[2], b[2], a[3], b[3], q.z, q.w);
-        }
+        const uint4 q = lds128(qa + (i + j) * 512);
+        mma16816(sc[k], a[0], b[0], a[1], b[1], q.x, q.y);
+        mma16816(sc[k], a[2], b[2], a[3], b[3], q.z, q.w);
       }
     }
   }
@@ -348,18 +342,15 @@ __device__ __forceinline__ void scores(const Params& p, const uint32_t (&t)[kNT]
     float2 kp[2];
     row_params<kF>(t[k], 12, at, kp);
     const float unit = p.qscale * kKeyUnit<kF>, k0 = kp[0].x * unit, k1 = kp[1].x * unit;
+    float2 qs = make_float2(0.0f, 0.0f);
+    if constexpr (kF == dev::kInt4) qs = lds_f2(at.rows + kG8 * 512 + quad * 2 * 4);
 #pragma unroll
-    for (int nb = 0; nb < kNB; ++nb) {
-      float2 qs = make_float2(0.0f, 0.0f);
-      if constexpr (kF == dev::kInt4) qs = lds_f2(at.rows + kNB * kG8 * 512 + (nb * 8 + quad * 2) * 4);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        sc[k][nb][c] *= k0;
-        sc[k][nb][2 + c] *= k1;
-        if constexpr (kF == dev::kInt4) {
-          sc[k][nb][c] = fmaf(kp[0].y, c ? qs.y : qs.x, sc[k][nb][c]);
-          sc[k][nb][2 + c] = fmaf(kp[1].y, c ? qs.y : qs.x, sc[k][nb][2 + c]);
-        }
+    for (int c = 0; c < 2; ++c) {
+      sc[k][c] *= k0;
+      sc[k][2 + c] *= k1;
+      if constexpr (kF == dev::kInt4) {
+        sc[k][c] = fmaf(kp[0].y, c ? qs.y : qs.x, sc[k][c]);
+        sc[k][2 + c] = fmaf(kp[1].y, c ? qs.y : qs.x, sc[k][2 + c]);
       }
     }
   }
@@ -369,39 +360,33 @@ __device__ __forceinline__ int exponent_of(float x) { return static_cast<int>((_
 
 // The reference maximum moves only when a score passes it by 8: exponentials reach 2^8 at most.  It moves by whole numbers,
 // so that what is scaled keeps its bits.  `top`: this lane's largest scores.
-template <int kD, int kNB>
-__device__ __forceinline__ void follow_maximum(State<kD, kNB>& s, float (&top)[kNB][2]) {
-  bool grow = false;
+template <int kD>
+__device__ __forceinline__ void follow_maximum(State<kD>& s, float (&top)[2]) {
+  if (__any_sync(0xFFFFFFFFu, top[0] > s.m[0] + 8.0f || top[1] > s.m[1] + 8.0f)) {
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) grow = grow || top[nb][0] > s.m[nb][0] + 8.0f || top[nb][1] > s.m[nb][1] + 8.0f;
-  if (__any_sync(0xFFFFFFFFu, grow)) {
+    for (int c = 0; c < 2; ++c) {
+      float v = top[c];
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
+      const float mn = fmaxf(s.m[c], ceilf(v));
+      if (mn == s.m[c]) continue;
+      const float up = mn - s.m[c], a = halvings(up);
+      s.l[c] *= a;
+      s.bias[c] *= a;
+      if (s.m[c] != -INFINITY) {  // (before it there is nothing in the outputs)
+        // the outputs' unit stays, unless it is too far from the maximum's
+        const float d = static_cast<float>(exponent_of(s.down[c])) + up, over = fmaxf(d - kMostDown, 0.0f), f = halvings(over);
+        s.down[c] = pow2(static_cast<int>(d - over));
+        if (over > 0.0f) {
 #pragma unroll
-    for (int nb = 0; nb < kNB; ++nb) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float v = top[nb][c];
-        v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
-        v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
-        v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
-        const float mn = fmaxf(s.m[nb][c], ceilf(v));
-        if (mn == s.m[nb][c]) continue;
-        const float up = mn - s.m[nb][c], a = halvings(up);
-        s.l[nb][c] *= a;
-        s.bias[nb][c] *= a;
-        if (s.m[nb][c] != -INFINITY) {  // (before it there is nothing in the outputs)
-          // the outputs' unit stays, unless it is too far from the maximum's
-          const float d = static_cast<float>(exponent_of(s.down[nb][c])) + up, over = fmaxf(d - kMostDown, 0.0f), f = halvings(over);
-          s.down[nb][c] = pow2(static_cast<int>(d - over));
-          if (over > 0.0f) {
-#pragma unroll
-            for (int mt = 0; mt < kD / 16; ++mt) {
-              s.acc[nb][mt][c] *= f;
-              s.acc[nb][mt][2 + c] *= f;
-            }
+          for (int mt = 0; mt < kD / 16; ++mt) {
+            s.acc[mt][c] *= f;
+            s.acc[mt][2 + c] *= f;
           }
         }
-        s.m[nb][c] = mn;
       }
+      s.m[c] = mn;
     }
   }
 }
@@ -409,33 +394,30 @@ __device__ __forceinline__ void follow_maximum(State<kD, kNB>& s, float (&top)[k
 // A row's outputs have a unit of their own, which follows its weights (the exponential times the value row's scale in its unit,
 // about the row's largest value): where one passes 2^14 in that unit, the unit grows until it is below 2^7.  So
 // the largest weight so far is 2^6 at least, and binary16 holds those down to 2^-20 of it without a loss, whatever sizes
-// other rows' and tokens' values have.  w: the weights of tokens g and g + 8 of columns 2 quad, 2 quad + 1 of each column block.
-__device__ __forceinline__ bool too_large(float a, float b, float c, float d) {
-  return fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d))) > 0x1p14f;
+// other rows' and tokens' values have.  w: the weights of tokens g and g + 8 of columns 2 quad, 2 quad + 1.
+__device__ __forceinline__ bool too_large(const float (&w)[4]) {
+  return fmaxf(fmaxf(fabsf(w[0]), fabsf(w[1])), fmaxf(fabsf(w[2]), fabsf(w[3]))) > 0x1p14f;
 }
-template <int kD, int kNB>
-__device__ __forceinline__ void follow_weights(State<kD, kNB>& s, float (&w)[kNB][4]) {
+template <int kD>
+__device__ __forceinline__ void follow_weights(State<kD>& s, float (&w)[4]) {
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int c = 0; c < 2; ++c) {
+    // infinities (scales that are not finite) move nothing
+    const float a = fabsf(w[c]), b = fabsf(w[2 + c]);
+    float v = fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f);
+    v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
+    v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
+    if (!(v > 0x1p14f)) continue;
+    const int d = exponent_of(s.down[c]), up = min(exponent_of(v) - 6, d + kMostDown);
+    const float f = halvings(static_cast<float>(up));
+    s.down[c] = pow2(d - up);
+    w[c] *= f;
+    w[2 + c] *= f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      // infinities (scales that are not finite) move nothing
-      const float a = fabsf(w[nb][c]), b = fabsf(w[nb][2 + c]);
-      float v = fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f);
-      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
-      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
-      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
-      if (!(v > 0x1p14f)) continue;
-      const int d = exponent_of(s.down[nb][c]), up = min(exponent_of(v) - 6, d + kMostDown);
-      const float f = halvings(static_cast<float>(up));
-      s.down[nb][c] = pow2(d - up);
-      w[nb][c] *= f;
-      w[nb][2 + c] *= f;
-#pragma unroll
-      for (int mt = 0; mt < kD / 16; ++mt) {
-        s.acc[nb][mt][c] *= f;
-        s.acc[nb][mt][2 + c] *= f;
-      }
+    for (int mt = 0; mt < kD / 16; ++mt) {
+      s.acc[mt][c] *= f;
+      s.acc[mt][2 + c] *= f;
     }
   }
 }
@@ -462,13 +444,10 @@ __device__ __forceinline__ uint32_t zero_rows(uint32_t t, const Place& at) {
   return zeros;
 }
 
-template <int kNB>
-__device__ __forceinline__ void without_zeros(uint32_t zeros, float (&w)[kNB][4]) {
-#pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
-    if (zeros & 1u) w[nb][0] = w[nb][1] = 0.0f;
-    if (zeros & 2u) w[nb][2] = w[nb][3] = 0.0f;
-  }
+// Takes the weights of rows of zeros out.
+__device__ __forceinline__ void without_zeros(uint32_t zeros, float (&w)[4]) {
+  if (zeros & 1u) w[0] = w[1] = 0.0f;
+  if (zeros & 2u) w[2] = w[3] = 0.0f;
 }
 
 // A lane's chunk of 8 elements (i-th of kD / 64) of tokens 2 quad, + 1, + 8, + 9 of a tile at `base` -> pairs of
@@ -499,53 +478,47 @@ struct Chunks {
 
 // Scores and exponentials of kNT tiles of one format that every row sees whole; kShort: with n[] tokens.
 // The K half of the stage is given back after the scores, if empty_k names it.
-template <int kD, int kNB, uint32_t kF, int kNT, bool kShort>
-__device__ __forceinline__ bool step(const Params& p, State<kD, kNB>& s, const uint32_t (&t)[kNT], const uint32_t (&n)[kNT],
+template <int kD, uint32_t kF, int kNT, bool kShort>
+__device__ __forceinline__ bool step(const Params& p, State<kD>& s, const uint32_t (&t)[kNT], const uint32_t (&n)[kNT],
                                      const Place& at, uint64_t* empty_k, uint64_t* full_v, uint32_t parity) {
   const uint32_t g = at.lane >> 2, quad = at.lane & 3;
   constexpr uint32_t kRb = kRow<kD, kF>;
-  float pr[kNT][kNB][4];
-  scores<kD, kNB, kF, kNT>(p, t, at, pr);
+  float pr[kNT][4];
+  scores<kD, kF, kNT>(p, t, at, pr);
   if (kNT == 2 || empty_k != nullptr) {
     __syncwarp();
     if (at.lane == 0) mbar_arrive(empty_k);
   }
-  float top[kNB][2];
+  float top[2];
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int c = 0; c < 2; ++c) {
+    top[c] = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      top[nb][c] = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < kNT; ++k) {
-        if constexpr (kShort) {
-          if (g >= n[k]) pr[k][nb][c] = -INFINITY;
-          if (g + 8 >= n[k]) pr[k][nb][2 + c] = -INFINITY;
-        }
-        top[nb][c] = fmaxf(top[nb][c], fmaxf(pr[k][nb][c], pr[k][nb][2 + c]));
+    for (int k = 0; k < kNT; ++k) {
+      if constexpr (kShort) {
+        if (g >= n[k]) pr[k][c] = -INFINITY;
+        if (g + 8 >= n[k]) pr[k][2 + c] = -INFINITY;
       }
+      top[c] = fmaxf(top[c], fmaxf(pr[k][c], pr[k][2 + c]));
     }
   }
   follow_maximum(s, top);
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int c = 0; c < 2; ++c) {
+    float ref = s.m[c];
+    if (kShort && ref == -INFINITY) ref = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float ref = s.m[nb][c];
-      if (kShort && ref == -INFINITY) ref = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kNT; ++k) {
-        pr[k][nb][c] = ex2(pr[k][nb][c] - ref);
-        pr[k][nb][2 + c] = ex2(pr[k][nb][2 + c] - ref);
-        s.l[nb][c] += pr[k][nb][c] + pr[k][nb][2 + c];
-      }
+    for (int k = 0; k < kNT; ++k) {
+      pr[k][c] = ex2(pr[k][c] - ref);
+      pr[k][2 + c] = ex2(pr[k][2 + c] - ref);
+      s.l[c] += pr[k][c] + pr[k][2 + c];
     }
   }
   if (!mbar_wait(full_v, parity)) return false;
 #pragma unroll
   for (int k = 0; k < kNT; ++k) {
     if (kShort && n[k] == 0) continue;
-    // ---- weights: the exponential times the value row's scale, in units of 2^E
+    // ---- weights: the exponential times the value row's scale, in the outputs' unit
     float2 vp[2];
     row_params<kF>(t[k], 20, at, vp);
     if constexpr (kShort) {
@@ -553,31 +526,21 @@ __device__ __forceinline__ bool step(const Params& p, State<kD, kNB>& s, const u
       if (g + 8 >= n[k]) vp[1] = make_float2(0.0f, 0.0f);
     }
     const float u0 = vp[0].x * kValueUnit<kF>, u1 = vp[1].x * kValueUnit<kF>;
-    float w[kNB][4];
-    bool grow = false;
+    float w[4];
 #pragma unroll
-    for (int nb = 0; nb < kNB; ++nb) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        w[nb][c] = pr[k][nb][c] * (u0 * s.down[nb][c]);
-        w[nb][2 + c] = pr[k][nb][2 + c] * (u1 * s.down[nb][c]);
-      }
-      grow = grow || too_large(w[nb][0], w[nb][1], w[nb][2], w[nb][3]);
+    for (int c = 0; c < 2; ++c) {
+      w[c] = pr[k][c] * (u0 * s.down[c]);
+      w[2 + c] = pr[k][2 + c] * (u1 * s.down[c]);
     }
-    if (__any_sync(0xFFFFFFFFu, grow)) {
-      if constexpr (kF == dev::kE4M3 || kF == dev::kE5M2) without_zeros<kNB>(zero_rows<kD, kF>(t[k], at), w);
+    if (__any_sync(0xFFFFFFFFu, too_large(w))) {
+      if constexpr (kF == dev::kE4M3 || kF == dev::kE5M2) without_zeros(zero_rows<kD, kF>(t[k], at), w);
       follow_weights(s, w);
     }
     const float beta0 = fmaf(8.0f, vp[0].x, vp[0].y), beta1 = fmaf(8.0f, vp[1].x, vp[1].y);
-    uint32_t pb[kNB][2];
+    const uint32_t pb[2] = {transpose8(dev::pack_f16x2(w[0], w[1])), transpose8(dev::pack_f16x2(w[2], w[3]))};
+    if constexpr (kF == dev::kInt4) {
 #pragma unroll
-    for (int nb = 0; nb < kNB; ++nb) {
-      pb[nb][0] = transpose8(dev::pack_f16x2(w[nb][0], w[nb][1]));
-      pb[nb][1] = transpose8(dev::pack_f16x2(w[nb][2], w[nb][3]));
-      if constexpr (kF == dev::kInt4) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) s.bias[nb][c] = fmaf(pr[k][nb][2 + c], beta1, fmaf(pr[k][nb][c], beta0, s.bias[nb][c]));
-      }
+      for (int c = 0; c < 2; ++c) s.bias[c] = fmaf(pr[k][2 + c], beta1, fmaf(pr[k][c], beta0, s.bias[c]));
     }
     // ---- O^T += V^T W^T
     const uint32_t token_bytes = at.heads * kRb;
@@ -589,10 +552,7 @@ __device__ __forceinline__ bool step(const Params& p, State<kD, kNB>& s, const u
       ch.take(base, token_bytes, i, quad, n[k], lo, hi);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          mma16816(s.acc[nb][4 * i + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[nb][0], pb[nb][1]);
-        }
+        mma16816(s.acc[4 * i + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[0], pb[1]);
       }
     }
   }
@@ -611,49 +571,39 @@ __device__ __forceinline__ bool visible(const Params& p, int32_t at, const View&
   return tok < v.n && d >= 0 && (p.window == 0 || static_cast<uint32_t>(d) < p.window || v.pos + tok < p.sinks);
 }
 // A query column's position.
-template <int kD, int kNB>
+template <int kD>
 __device__ __forceinline__ int32_t position(const Place& at, uint32_t col) {
-  return static_cast<int32_t>(lds32(at.rows + kNB * (kD / 32) * 512 + 32 * kNB + col * 4));
+  return static_cast<int32_t>(lds32(at.rows + (kD / 32) * 512 + 32 + col * 4));
 }
 
 // O^T += V^T W^T of such a tile.  Where it holds values that are not finite, it is taken row by row, so that a row is
 // not touched by what it does not see.
-template <int kD, int kNB, uint32_t kF>
-__device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, const View& v, const Place& at,
-                                            const float (&pr)[kNB][4]) {
+template <int kD, uint32_t kF>
+__device__ __forceinline__ void edge_values(const Params& p, State<kD>& s, const View& v, const Place& at,
+                                            const float (&pr)[4]) {
   const uint32_t g = at.lane >> 2, quad = at.lane & 3;
   constexpr uint32_t kRb = kRow<kD, kF>;
   float2 vp[2];
   row_params<kF>(v.t, 20, at, vp);
   const float u0 = vp[0].x * kValueUnit<kF>, u1 = vp[1].x * kValueUnit<kF>;
   const float beta0 = fmaf(8.0f, vp[0].x, vp[0].y), beta1 = fmaf(8.0f, vp[1].x, vp[1].y);  // INT4: what (code - 8) / 8 leaves
-  float w[kNB][4];
-  bool grow = false;
+  float w[4];
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float p0 = pr[nb][c], p1 = pr[nb][2 + c];
-      // a hidden token's weight is 0 whatever its parameters hold
-      w[nb][c] = p0 == 0.0f ? 0.0f : p0 * (u0 * s.down[nb][c]);
-      w[nb][2 + c] = p1 == 0.0f ? 0.0f : p1 * (u1 * s.down[nb][c]);
-      if constexpr (kF == dev::kInt4) {
-        if (p0 != 0.0f) s.bias[nb][c] = fmaf(p0, beta0, s.bias[nb][c]);
-        if (p1 != 0.0f) s.bias[nb][c] = fmaf(p1, beta1, s.bias[nb][c]);
-      }
+  for (int c = 0; c < 2; ++c) {
+    const float p0 = pr[c], p1 = pr[2 + c];
+    // a hidden token's weight is 0 whatever its parameters hold
+    w[c] = p0 == 0.0f ? 0.0f : p0 * (u0 * s.down[c]);
+    w[2 + c] = p1 == 0.0f ? 0.0f : p1 * (u1 * s.down[c]);
+    if constexpr (kF == dev::kInt4) {
+      if (p0 != 0.0f) s.bias[c] = fmaf(p0, beta0, s.bias[c]);
+      if (p1 != 0.0f) s.bias[c] = fmaf(p1, beta1, s.bias[c]);
     }
-    grow = grow || too_large(w[nb][0], w[nb][1], w[nb][2], w[nb][3]);
   }
-  if (__any_sync(0xFFFFFFFFu, grow)) {
-    if constexpr (kF == dev::kE4M3 || kF == dev::kE5M2) without_zeros<kNB>(zero_rows<kD, kF>(v.t, at), w);
+  if (__any_sync(0xFFFFFFFFu, too_large(w))) {
+    if constexpr (kF == dev::kE4M3 || kF == dev::kE5M2) without_zeros(zero_rows<kD, kF>(v.t, at), w);
     follow_weights(s, w);
   }
-  uint32_t pb[kNB][2];
-#pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
-    pb[nb][0] = transpose8(dev::pack_f16x2(w[nb][0], w[nb][1]));
-    pb[nb][1] = transpose8(dev::pack_f16x2(w[nb][2], w[nb][3]));
-  }
+  const uint32_t pb[2] = {transpose8(dev::pack_f16x2(w[0], w[1])), transpose8(dev::pack_f16x2(w[2], w[3]))};
   const uint32_t token_bytes = at.heads * kRb;
   const uint32_t base = lds32(v.t + 16) + (at.head_i + 2 * quad * at.heads) * kRb + g * (kRb / 8);
   Chunks<kD, kF, true> ch;
@@ -666,26 +616,21 @@ __device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, 
     for (int k = 0; k < 8; ++k) bad = bad || has_nonfinite(lo[k]) || has_nonfinite(hi[k]);
     if (__any_sync(0xFFFFFFFFu, bad)) {
 #pragma unroll 1
-      for (int col = 0; col < 8 * kNB; ++col) {
+      for (int col = 0; col < 8; ++col) {
         // this row's view of the 16 tokens
-        const int32_t row_at = position<kD, kNB>(at, col);
-        const int nb = col >> 3;
-        const uint32_t x0 = nb == 0 ? pb[0][0] : pb[kNB - 1][0], x1 = nb == 0 ? pb[0][1] : pb[kNB - 1][1];
+        const int32_t row_at = position<kD>(at, col);
         const uint32_t keep_lo = (visible(p, row_at, v, 2 * quad) ? 0xFFFFu : 0u) | (visible(p, row_at, v, 2 * quad + 1) ? 0xFFFF0000u : 0u);
         const uint32_t keep_hi = (visible(p, row_at, v, 2 * quad + 8) ? 0xFFFFu : 0u) |
                                  (visible(p, row_at, v, 2 * quad + 9) ? 0xFFFF0000u : 0u);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma16816(t, lo[2 * k] & keep_lo, lo[2 * k + 1] & keep_lo, hi[2 * k] & keep_hi, hi[2 * k + 1] & keep_hi, x0, x1);
+          mma16816(t, lo[2 * k] & keep_lo, lo[2 * k + 1] & keep_lo, hi[2 * k] & keep_hi, hi[2 * k + 1] & keep_hi, pb[0], pb[1]);
 #pragma unroll
-          for (int b = 0; b < kNB; ++b) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (static_cast<int>(b * 8 + quad * 2 + c) == col) {
-                s.acc[b][4 * i + k][c] += t[c];
-                s.acc[b][4 * i + k][2 + c] += t[2 + c];
-              }
+          for (int c = 0; c < 2; ++c) {
+            if (static_cast<int>(quad * 2 + c) == col) {
+              s.acc[4 * i + k][c] += t[c];
+              s.acc[4 * i + k][2 + c] += t[2 + c];
             }
           }
         }
@@ -693,57 +638,48 @@ __device__ __forceinline__ void edge_values(const Params& p, State<kD, kNB>& s, 
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          mma16816(s.acc[nb][4 * i + k], lo[2 * k], lo[2 * k + 1], hi[2 * k], hi[2 * k + 1], pb[nb][0], pb[nb][1]);
-        }
+        mma16816(s.acc[4 * i + k], lo[2 * k], lo[2 * k + 1], hi[2 * k], hi[2 * k + 1], pb[0], pb[1]);
       }
     }
   }
 }
 
-template <int kD, int kNB, uint32_t kF>
-__device__ __forceinline__ void edge_step(const Params& p, State<kD, kNB>& s, const View& v, const Place& at) {
+template <int kD, uint32_t kF>
+__device__ __forceinline__ void edge_step(const Params& p, State<kD>& s, const View& v, const Place& at) {
   const uint32_t g = at.lane >> 2, quad = at.lane & 3;
   const uint32_t t[1] = {v.t};
-  float sc[1][kNB][4], top[kNB][2];
-  scores<kD, kNB, kF, 1>(p, t, at, sc);
-  float(&pr)[kNB][4] = sc[0];
+  float sc[1][4], top[2];
+  scores<kD, kF, 1>(p, t, at, sc);
+  float(&pr)[4] = sc[0];
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int32_t row_at = position<kD, kNB>(at, nb * 8 + quad * 2 + c);
-      if (!visible(p, row_at, v, g)) pr[nb][c] = -INFINITY;
-      if (!visible(p, row_at, v, g + 8)) pr[nb][2 + c] = -INFINITY;
-      top[nb][c] = fmaxf(pr[nb][c], pr[nb][2 + c]);
-    }
+  for (int c = 0; c < 2; ++c) {
+    const int32_t row_at = position<kD>(at, quad * 2 + c);
+    if (!visible(p, row_at, v, g)) pr[c] = -INFINITY;
+    if (!visible(p, row_at, v, g + 8)) pr[2 + c] = -INFINITY;
+    top[c] = fmaxf(pr[c], pr[2 + c]);
   }
   follow_maximum(s, top);
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float ref = s.m[nb][c] == -INFINITY ? 0.0f : s.m[nb][c];  // nothing seen yet
-      pr[nb][c] = ex2(pr[nb][c] - ref);
-      pr[nb][2 + c] = ex2(pr[nb][2 + c] - ref);
-      s.l[nb][c] += pr[nb][c] + pr[nb][2 + c];
-    }
+  for (int c = 0; c < 2; ++c) {
+    const float ref = s.m[c] == -INFINITY ? 0.0f : s.m[c];  // nothing seen yet
+    pr[c] = ex2(pr[c] - ref);
+    pr[2 + c] = ex2(pr[2 + c] - ref);
+    s.l[c] += pr[c] + pr[2 + c];
   }
-  edge_values<kD, kNB, kF>(p, s, v, at, pr);
+  edge_values<kD, kF>(p, s, v, at, pr);
 }
 
 // Out of line, with the state in memory: these tiles are few, and their code's registers are not the stream's.
-template <int kD, int kNB>
-__device__ __noinline__ void edge_tile(const Params& p, State<kD, kNB>* state, uint32_t t, const Place at) {
-  State<kD, kNB> s = *state;
+template <int kD>
+__device__ __noinline__ void edge_tile(const Params& p, State<kD>* state, uint32_t t, const Place at) {
+  State<kD> s = *state;
   const uint2 a = lds64(t);
   const View v{t, (a.x >> 8) & 0xFFu, a.y};
   switch (a.x & 0xFFu) {
-    case dev::kFp16: edge_step<kD, kNB, dev::kFp16>(p, s, v, at); break;
-    case dev::kE4M3: edge_step<kD, kNB, dev::kE4M3>(p, s, v, at); break;
-    case dev::kE5M2: edge_step<kD, kNB, dev::kE5M2>(p, s, v, at); break;
-    default: edge_step<kD, kNB, dev::kInt4>(p, s, v, at); break;
+    case dev::kFp16: edge_step<kD, dev::kFp16>(p, s, v, at); break;
+    case dev::kE4M3: edge_step<kD, dev::kE4M3>(p, s, v, at); break;
+    case dev::kE5M2: edge_step<kD, dev::kE5M2>(p, s, v, at); break;
+    default: edge_step<kD, dev::kInt4>(p, s, v, at); break;
   }
   *state = s;
 }
@@ -1046,7 +982,6 @@ struct Producer {
 template <int kD, bool kTwo>
 __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_constant__ Params p) {
   using C = Config<kD, kTwo>;
-  constexpr int kNB = 1;  // column blocks of a warp
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
   float* merge = reinterpret_cast<float*>(smem + 2 * C::kRing);
@@ -1125,9 +1060,9 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
 
   // ---- consumers
   const uint32_t group = warp / 8, w8 = warp % 8;
-  const uint32_t wr_at = smem_addr(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp * static_cast<uint32_t>(sizeof(WarpRows<kD, kNB>));
+  const uint32_t wr_at = smem_addr(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp * static_cast<uint32_t>(sizeof(WarpRows<kD>));
   const uint32_t stages_at = smem_addr(stages);
-  State<kD, kNB> s;
+  State<kD> s;
   uint32_t meets = 0;
   // All consumer warps, with a limit as every wait.
   auto meet = [&]() {
@@ -1145,14 +1080,14 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
     constexpr uint32_t kHead = offsetof(Stage, tiles), kHead2 = offsetof(Stage, heads);
     if ((lds32(m + kHead + 4) & (kDone | kLast)) == kDone) break;  // a share without work
     if (lds32(m + kHead + 4) & kFirst) {
-      WarpRows<kD, kNB>* wr = reinterpret_cast<WarpRows<kD, kNB>*>(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp;
+      WarpRows<kD>* wr = reinterpret_cast<WarpRows<kD>*>(smem + 2 * C::kRing + C::kMergeBytes + sizeof(Stage) * kStages) + warp;
       const uint32_t heads = lds32(m + kHead2), seq = lds32(m + kHead + 8), head0 = lds32(m + kHead + 12);
       const uint32_t single = heads > 4 ? 1u : heads > 2 ? 2u : heads > 1 ? 4u : 8u;
       // a group's warps beyond `single` x heads have no tile
       if (lane == 0) wr->place = make_uint4(heads, w8 % heads, w8 / heads < single ? w8 / heads : 1u << 16, single);
-      begin_piece<kD, kNB>(p, s, wr, rows_of(p, seq), p.context[seq], head0 + w8 % heads, kTwo ? group * 8 : 0u, lane);
+      begin_piece<kD>(p, s, wr, rows_of(p, seq), p.context[seq], head0 + w8 % heads, kTwo ? group * 8 : 0u, lane);
     }
-    const uint4 place = lds128(wr_at + static_cast<uint32_t>(sizeof(WarpRows<kD, kNB>)) - 16);
+    const uint4 place = lds128(wr_at + static_cast<uint32_t>(sizeof(WarpRows<kD>)) - 16);
     const Place at{wr_at, place.x, place.y, lane};
     const uint32_t tile_i = place.z, single = place.w;
     // This warp's tiles of the stage: tile_i, and every `single`-th behind it.
@@ -1163,9 +1098,9 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
       const uint32_t t0 = m + tile_i * static_cast<uint32_t>(sizeof(Tile)), two[2] = {t0, t0 + single * static_cast<uint32_t>(sizeof(Tile))};
       const uint32_t n[2] = {16, 16};
       switch (lds32(t0) & 0xFFu) {
-        case dev::kE4M3: ok = step<kD, kNB, dev::kE4M3, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
-        case dev::kE5M2: ok = step<kD, kNB, dev::kE5M2, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
-        default: ok = step<kD, kNB, dev::kInt4, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
+        case dev::kE4M3: ok = step<kD, dev::kE4M3, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
+        case dev::kE5M2: ok = step<kD, dev::kE5M2, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
+        default: ok = step<kD, dev::kInt4, 2, false>(p, s, two, n, at, empty_k, full_v, parity); break;
       }
     } else {
       uint64_t* give = nullptr;  // the K half's barrier with the last tile's scores, null once it is given back
@@ -1176,21 +1111,21 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
         give = i + single < n_tiles || !(fn >> 16) ? nullptr : empty_k;
         if (fn >> 16) {
           switch (fn & 0xFFFFu) {
-            case dev::kFp16 | 16 << 8: ok = step<kD, kNB, dev::kFp16, 1, false>(p, s, one, n, at, give, full_v, parity); break;
-            case dev::kE4M3 | 16 << 8: ok = step<kD, kNB, dev::kE4M3, 1, false>(p, s, one, n, at, give, full_v, parity); break;
-            case dev::kInt4 | 16 << 8: ok = step<kD, kNB, dev::kInt4, 1, false>(p, s, one, n, at, give, full_v, parity); break;
+            case dev::kFp16 | 16 << 8: ok = step<kD, dev::kFp16, 1, false>(p, s, one, n, at, give, full_v, parity); break;
+            case dev::kE4M3 | 16 << 8: ok = step<kD, dev::kE4M3, 1, false>(p, s, one, n, at, give, full_v, parity); break;
+            case dev::kInt4 | 16 << 8: ok = step<kD, dev::kInt4, 1, false>(p, s, one, n, at, give, full_v, parity); break;
             default:
               switch (fn & 0xFFu) {
-                case dev::kFp16: ok = step<kD, kNB, dev::kFp16, 1, true>(p, s, one, n, at, give, full_v, parity); break;
-                case dev::kE4M3: ok = step<kD, kNB, dev::kE4M3, 1, true>(p, s, one, n, at, give, full_v, parity); break;
-                case dev::kE5M2: ok = step<kD, kNB, dev::kE5M2, 1, true>(p, s, one, n, at, give, full_v, parity); break;
-                default: ok = step<kD, kNB, dev::kInt4, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+                case dev::kFp16: ok = step<kD, dev::kFp16, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+                case dev::kE4M3: ok = step<kD, dev::kE4M3, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+                case dev::kE5M2: ok = step<kD, dev::kE5M2, 1, true>(p, s, one, n, at, give, full_v, parity); break;
+                default: ok = step<kD, dev::kInt4, 1, true>(p, s, one, n, at, give, full_v, parity); break;
               }
           }
         } else {
           ok = mbar_wait(full_v, parity);
-          State<kD, kNB> copy = s;
-          if (ok) edge_tile<kD, kNB>(p, &copy, one[0], at);
+          State<kD> copy = s;
+          if (ok) edge_tile<kD>(p, &copy, one[0], at);
           s = copy;
         }
       }
@@ -1224,8 +1159,8 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
           const bool join = !kTwo && turn == 1;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float l = s.l[0][c], b = s.bias[0][c], m_own = s.m[0][c], fo = 1.0f, ft = 0.0f;
-            const float unit = pow2(-exponent_of(s.down[0][c]));
+            float l = s.l[c], b = s.bias[c], m_own = s.m[c], fo = 1.0f, ft = 0.0f;
+            const float unit = pow2(-exponent_of(s.down[c]));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
@@ -1243,7 +1178,7 @@ __global__ void __launch_bounds__(kThreads, 1) stream_kernel(const __grid_consta
 #pragma unroll
             for (int mt = 0; mt < kD / 16; ++mt) {
               float2* at2 = reinterpret_cast<float2*>(row + g * (kD / 8) + 2 * mt);
-              float2 x = make_float2(fmaf(s.acc[0][mt][c], unit, b), fmaf(s.acc[0][mt][2 + c], unit, b));
+              float2 x = make_float2(fmaf(s.acc[mt][c], unit, b), fmaf(s.acc[mt][2 + c], unit, b));
               if (join) {
                 const float2 y = *at2;
                 x = make_float2(fmaf(x.x, fo, y.x * ft), fmaf(x.y, fo, y.y * ft));
