@@ -505,8 +505,7 @@ __device__ __forceinline__ bool step(const Params& p, State<kD>& s, const uint32
   follow_maximum(s, top);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    float ref = s.m[c];
-    if (kShort && ref == -INFINITY) ref = 0.0f;
+    const float ref = s.m[c] == -INFINITY ? 0.0f : s.m[c];  // no score so far that is not minus infinity
 #pragma unroll
     for (int k = 0; k < kNT; ++k) {
       pr[k][c] = ex2(pr[k][c] - ref);

@@ -176,3 +176,25 @@ def test_value_scales_far_apart(hlkv_lib, cuda_device, probs, q, window, by):
         b = Batch(hlkv_lib, 16, 2, D, [[16] * 40, [16] * 21 + [9]], q, probs=probs, window=window, sinks=5 if window else 0, seed=7,
                   change=change)
         _attend(b, 8, scale)
+
+
+@pytest.mark.parametrize("q", [[1], [3], [40]])
+@pytest.mark.parametrize("hidden", [16, 48, 200])
+def test_scores_of_minus_infinity(hlkv_lib, cuda_device, q, hidden):
+    """Keys whose scores are minus infinity, from the first token on: weights of 0, as if they were hidden."""
+    import torch
+    ctx, D = 256, 64
+    b = Batch(hlkv_lib, 16, 1, D, [[16] * (ctx // 16)], q, probs=(1, 0, 0, 0), seed=1)
+    rng = np.random.default_rng(hidden)
+    k, v = np.zeros((ctx, 1, D), np.float16), rng.standard_normal((ctx, 1, D)).astype(np.float16)
+    k[:hidden, :, 0] = -np.inf
+    put_rows(b.wl, 0, k, v)
+    x = np.zeros((b.cap, 4, D), np.float16)
+    x[..., 0] = 1
+    got = b.run(torch.from_numpy(x.view(np.int16)).cuda(), 1.0)
+    torch.cuda.synchronize()
+    g = got.cpu().numpy().view(np.float16).astype(np.float64)
+    for r in range(q[0]):
+        seen = v[hidden:ctx - q[0] + r + 1, 0].astype(np.float64)  # of equal weight
+        # the weights are powers of two; the result's rounding, and the sums'
+        assert (np.abs(g[r] - seen.mean(0)) <= 2.0 ** -11 * np.abs(seen.mean(0)) + 2.0 ** -16 * np.abs(seen).mean(0)).all()
