@@ -1143,7 +1143,7 @@ uint64_t tiles_of_tokens(const Params& p) {
 // in that plan: 934 and 60 us.)
 uint32_t tile_ranks(const Params& p) {
   if (p.nseq <= kOrdered || tiles_of_plan(p) <= 2 * tiles_of_tokens(p)) return 0;
-  return static_cast<uint32_t>(tiles_of_tokens(p));
+  return static_cast<uint32_t>(std::max<uint64_t>(tiles_of_tokens(p), 1));
 }
 
 uint64_t tile_ctas(const Params& p) {

@@ -89,3 +89,19 @@ def test_many_sequences_in_a_plan_for_long_prompts(hlkv_lib, cuda_device, nseq, 
     n = sum(lens)
     assert (got[n:] == 0x1234).all()
     assert (np.abs(got.cpu().numpy().view(np.float16).astype(np.float64)[:n] - want[:n]) <= tol[:n]).all()
+
+
+def test_few_tokens_of_many_sequences(hlkv_lib, cuda_device):
+    """Fewer rows in the whole batch than a row tile needs, in a plan for long prompts of many sequences."""
+    import torch
+    lens = [0] * 200
+    lens[3], lens[150] = 1, 2
+    b = Batch(hlkv_lib, 16, 1, 64, [[16, 9]] * 200, lens, seed=1)
+    b.plan = hlkv_lib.BatchPlan(200, b.plan.c.block_cap, b.cap, 8192)
+    b.fill_plan()
+    x, d_q = b.queries(4, 1)
+    got = b.run(d_q, 0.125)
+    torch.cuda.synchronize()
+    want, tol, err = b.want(x, 0.125)
+    assert int(b.err.item()) == err == 0
+    assert (np.abs(got.cpu().numpy().view(np.float16).astype(np.float64) - want) <= tol).all()
