@@ -15,15 +15,15 @@
 // A code's binary16 value is exact (E4M3, E5M2, an INT4 code's integer), so the parameters stay out of
 // the matrices: the K row's scale multiplies the score in binary32 and its bias enters as
 // bias * sum(q); the V row's scale multiplies the weight, and its bias is summed apart in binary32.
-// A weight is rounded once, to binary16 (2^-12 of it; the matrix unit takes no wider one at this rate), in a unit of its row
+// A weight is rounded once, to binary16 (2^-11 of it at most; the matrix unit takes no wider one at this rate), in a unit of its row
 // that follows the row's weights: those down to 2^-20 of the largest one stay in binary16's normal range, whatever sizes other
 // rows' and tokens' values have.
 // The order of contraction is free, so every lane takes contiguous bytes of a row and pairs them
 // where they lie: K elements (j, j + 4) of each 8, V tokens (2q, 2q + 1).
 //
-// Measured (8 KV heads of 128, 32 query heads): 64 sequences of 8192 tokens, most in INT4, one new token each, 212 us:
-// 3.9 TB/s, 0.60 of the copy rate; what is left is the consumers' instructions, about as many for an INT4 tile as
-// for an FP16 one of 3.5 times the bytes.  32 windows of 4100 tokens with four new tokens each, 132 us, of which the
+// Measured (8 KV heads of 128, 32 query heads): 64 sequences of 8192 tokens, most in INT4, one new token each, 213 us:
+// 3.9 TB/s, 0.59 of the copy rate; what is left is the consumers' instructions, about as many for an INT4 tile as
+// for an FP16 one of 3.5 times the bytes.  32 windows of 4100 tokens with four new tokens each, 131 us, of which the
 // copies alone take 49: every tile is converted once for each 8 of the 16 rows.  Four sequences of 300 to 1100
 // tokens, 27 us: 3 to launch, 12 until the first tiles lie in shared memory (five dependent trips to memory), 6 of
 // arithmetic, 6 to join the partials.
@@ -1334,7 +1334,8 @@ cudaError_t launch(const Params& p, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   // A warp a row where a unit has few partials (32 windows of 16 rows, 5 each: 132 us with it, 137 us with a CTA a row),
-  // a CTA a row where it has many (4 short sequences, 37 each: 27 us with it, 37 us with a warp a row).
+  // a CTA a row where it has many (4 short sequences, 37 each: 27 us with it, 37 us with a warp a row).  The border lies
+  // between these two, by no other case.
   const uint32_t rows = p.nseq * p.H * p.slot_rows;
   if (uint64_t{p.nseq} * p.head_groups * 12 > p.ctas) {
     cfg.gridDim = dim3((rows + kMergeWarps - 1) / kMergeWarps);

@@ -12,18 +12,20 @@
 // the other's products run.  Tensor memory: S0, S1, O0, O1; P overwrites S.
 // As in the stream kernel a code's binary16 value is exact and its parameters stay outside: the K row's scale and
 // bias in the score, the V row's scale in the weight, its bias in a sum of its own, all in binary32.  A weight is
-// rounded once, to binary16 (2^-12 of it; the matrix unit takes no wider one at this rate), against a reference of its row
+// rounded once, to binary16 (2^-11 of it at most; the matrix unit takes no wider one at this rate), against a reference of its row
 // that follows scores and value scales together.
 // Codes are laid in the order (0, 4, 1, 5, 2, 6, 3, 7) of each 8, where the formats' words hold them: Q's elements
 // lie the same way, and the outputs are put back in order at the end.
 //
 // Measured (8 KV heads of 128, 32 query heads; six chunks of up to 1645 new tokens over contexts of up to 8024, formats
-// mixed): 950 us, 393 TFLOP/s, 0.24 of the matrix rate; the caches of one format alone: FP16 816, E4M3 885, INT4 993 us.
-// The products alone would take 370 us, the conversion without the softmax 640, the softmax without the conversion
-// 950.  The softmax's two warps per scheduler wait on their own chains (an issue every 2.2 cycles), and the per-token
+// mixed): 945 us, 394 TFLOP/s, 0.24 of the matrix rate; the caches of one format alone: FP16 757, E4M3 927, INT4 1008 us.
+// The products of the tiles that are walked, 388 GFLOP, would take 234 us at the matrix rate; on copies that left the other
+// part out the conversion took 640 us and the softmax 950.  The softmax's two warps per scheduler wait on their own chains (an issue every 2.2 cycles), and the per-token
 // parameters are broadcast from shared memory: a float4 load returns 512 bytes to a warp, 2048 cycles of a tile for FP8
-// and 4096 for INT4.  Five prompts of heads of 64 with a window of 1024: 154 us; a CTA there walks ten tiles, of which
-// the last and the sinks' are short.  250 new tokens over 8000, four row tiles a head: 124 us, and 340 without the split.
+// and 4096 for INT4.  Five prompts of heads of 64 with a window of 1024: 155 us; a CTA there walks 6.5 tiles on
+// average, of which the last and the sinks' are short.  250 new tokens over 8000, four row tiles a head: 139 us.
+// References of one row each, next to a unit that 128 tokens shared, took chunks from 954 to 950 us (FP16 alone 827 to 757,
+// E4M3 924 to 927, INT4 994 to 1008), the heads of 64 from 154 to 158 and few rows over 8000 tokens from 73 to 77.
 // Tried and slower than 928 us (the same without the split over tokens, whose code costs 2 %): halves of 64 tokens with scores of their own (1020 us), products issued by a softmax warp (1190),
 // half the loads in flight (1070), FP8 and INT4 rows in 16-byte pieces a tile ahead (985).
 #include <algorithm>
@@ -593,8 +595,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // and the exponent of its 16 tokens' value scales (its own where these lie far apart), so that a weight, the
         // exponential times the scale, is at most 2^14 where no sum passes the reference by more than kAbove.  Where one
         // does, the reference moves to kBelow under it, by a whole number, and what was made with the old one (O, the
-        // sums, this tile's weights so far) is scaled by a power of two.  So the largest weight is in [2^5, 2^14], and
-        // binary16 holds those down to 2^-19 of it without a loss, whatever other rows and tokens hold.
+        // sums, this tile's weights so far) is scaled by a power of two.  So the largest weight is in [2^5, 2^14] (2^-1 where
+        // it is of a token whose scale is 2^6 below its neighbours'), and binary16 holds those down to 2^-19 (2^-13)
+        // of it without a loss, whatever other rows and tokens hold.
         constexpr float kAbove = 14.0f, kBelow = 6.0f;
 #pragma unroll 1
         for (uint32_t c = 0; c < (n + 31) / 32; ++c) {  // the products take no further tokens

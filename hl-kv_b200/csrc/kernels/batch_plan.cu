@@ -59,7 +59,7 @@ struct Sum {
 };
 
 // What a block of v tokens costs the attention, which works on tiles of 16 tokens: in proportion to the
-// time measured for caches of one format (2.0, 1.0 and 1.1 us a tile of 8 heads of 128 per SM).
+// time measured for caches of one format (2.0, 1.0 and 1.1 us a tile of 8 heads of 128 per SM); used for every shape.
 __device__ __forceinline__ uint32_t block_cost(uint32_t info, uint32_t v) {
   const uint32_t f = info & 0xFu;
   return (v + 15) / 16 * (f == dev::kFp16 ? 14u : 7u);

@@ -120,7 +120,9 @@ __device__ __forceinline__ bool reciprocal_ok(float scale) { return scale >= 0x1
 // rules are dev::encode_row's (the reference's quantize_reference) but for the scale, which is the
 // product amax * (1 / max_finite) or range * (1 / 15) with the reciprocal in binary32 instead of the
 // quotient: within 1.5 units in the last place of the exact value where the quotient is within half
-// a unit, and no division; codes are the IEEE quotients by that scale, rounded to nearest even.
+// a unit.  That is the operator's definition, not a gain (8192 tokens take 49.7 us with the gather, and 49.8 with the
+// quotient): a row's bytes can differ from append_encode's of the same values.  Codes are the IEEE quotients by
+// that scale, rounded to nearest even.
 template <int kD>
 __device__ __forceinline__ uint32_t encode_row_f32(uint32_t f, const float (&x)[16], uint32_t lane, uint32_t mask,
                                                    uint8_t* payload, uint32_t row, uint64_t code_bytes) {

@@ -428,7 +428,8 @@ typedef struct {
  * targets).  An FP16 block takes them rounded once; a quantized row follows quantize_reference's
  * rules as hlkv_append_encode does, with the scale computed as amax * (1 / max_finite) or range *
  * (1 / 15), the reciprocal in binary32: within two units in the last place of its quotient, so
- * that a value midway between two codes may take the other one.
+ * that a value midway between two codes may take the other one.  The bytes of a K or V row can so differ
+ * from those that hlkv_append_encode stores for the same values.
  *  - d_q, d_k, d_v, d_q_out: binary16, heads of head_dim contiguous per token ([q_heads] or
  *    [kv_heads]), token strides in elements (multiples of 8); 16-byte aligned.  Slices of a fused
  *    projection need no copy.  d_q_out may be d_q with the same stride, and overlaps nothing else.
@@ -454,8 +455,12 @@ int hlkv_rotary_append(const HlkvPools* pools, const HlkvLayout* layout, const H
  *   out[i][qh] = softmax_t(softmax_scale <q, k_t>) . v_t   over the t with
  *   t <= p  and  (window == 0  or  p - t < window  or  t < sinks),   p = the token's position.
  * K and V are the values of the codes under their parameters (code * scale, or code * scale +
- * bias), not rounded to binary16 first; sums, maxima and the running state are binary32; the
- * result is rounded to binary16.  A row that sees no token is zeros.  Tokens that a row does not
+ * bias), not rounded to binary16 first; scores, sums, maxima and the running state are binary32.  A
+ * weight (a token's exponential times its V row's scale) is rounded to binary16 before it multiplies the
+ * codes, 2^-11 of it at most: outputs are off by about 2e-4 of their size on top of their own rounding.  Its
+ * unit follows the row's largest weight: weights down to 2^-13 of that one (in most batches 2^-19) keep this
+ * precision whatever the sizes of the values are (up to 2^58), smaller ones are off by 2^-24 of it at most.
+ * The result is rounded to binary16.  A row that sees no token is zeros.  Tokens that a row does not
  * see do not touch it, whatever they hold.
  *  - d_q and d_out: binary16, token rows at the plan's d_token_first[i] + r, heads contiguous
  *    ([q_heads][head_dim]), token strides in elements (multiples of 8), 16-byte aligned; d_out
