@@ -198,3 +198,30 @@ def test_scores_of_minus_infinity(hlkv_lib, cuda_device, q, hidden):
         seen = v[hidden:ctx - q[0] + r + 1, 0].astype(np.float64)  # of equal weight
         # the weights are powers of two; the result's rounding, and the sums'
         assert (np.abs(g[r] - seen.mean(0)) <= 2.0 ** -11 * np.abs(seen.mean(0)) + 2.0 ** -16 * np.abs(seen).mean(0)).all()
+
+
+@pytest.mark.parametrize("probs", [(0, 0, 1, 0), (0, 0, 0, 1), (0, 1, 1, 1)])
+@pytest.mark.parametrize("window", [0, 1500])
+@pytest.mark.parametrize("q", [[1], [40]])
+def test_value_scales_far_apart_when_split(hlkv_lib, cuda_device, probs, window, q):
+    """Parts of a row's tokens on several CTAs, some of them with nothing but zeros, joined."""
+    rng = np.random.default_rng(window)
+
+    def change(wl):
+        ids = wl.table.sequence_block_ids(wl.seqs[0])[1]
+        where = {f: [] for f in (1, 2, 3)}
+        for j, bid in enumerate(ids):
+            slot, info, _, _ = wl.table.device_descriptor(bid)
+            where[info & 15].append((slot, j))
+        for f, slots in where.items():
+            if not slots:
+                continue
+            host, codes, par = _value_rows(wl, f)
+            for slot, j in slots:
+                par[slot] *= np.float32(2.0) ** np.float32(rng.uniform(-12, 4))
+                if 60 <= j < 110:  # 800 tokens of zeros
+                    codes[slot], par[slot] = 0, 0.0 if f == 3 else 1.0
+            _write(wl, f, host)
+
+    b = Batch(hlkv_lib, 16, 1, 128, [[16] * 150], q, probs=probs, window=window, sinks=5 if window else 0, seed=7, change=change)
+    _attend(b, 4, 128 ** -0.5)
